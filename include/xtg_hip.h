@@ -46,7 +46,8 @@ typedef struct xtg_bf16 {
 } xtg_bf16;
 
 enum { XTG_X_F32 = 0, XTG_X_BF16 = 1 };   /* activation element type of the device matmul */
-enum { XTG_KV_BF16 = 0, XTG_KV_FP8 = 1 }; /* xtg::KvDtype (engine/include/xtg/kv.h:18) */
+enum { XTG_KV_BF16 = 0, XTG_KV_FP8 = 1,   /* xtg::KvDtype (engine/include/xtg/kv.h:18) */
+       XTG_KV_NVFP4 = 2 };                /* no counterpart in the reference: E2M1 codes, an E4M3 scale per 16 dims */
 /* The recurrent sublayers' KV mode (the pack's kv_mode option, packs/dory/dory.cpp:150-151): per_loop keeps one cache
  * per loop; last_loop keeps one cache that only the last loop writes (dory.cpp:534-537). */
 enum { XTG_KV_PER_LOOP = 0, XTG_KV_LAST_LOOP = 1 };
@@ -127,8 +128,9 @@ int xtg_hip_matmul_bf16_dev(xtg_hip* h, const xtg_bf16* w, const void* x, int x_
 
 /* Replaces xtg::KvCache(kv_heads, head_dim, slots, ring, dtype) (kv.h:24, kv.cpp:42-63): ring > 0 makes a ring of
  * `ring` slots (slot = position mod ring), else a linear cache of `slots` positions, in device memory: BF16
- * (XTG_KV_BF16) or E4M3 codes with one FP32 scale per (position, KV head) (XTG_KV_FP8). Every slot starts empty.
- * NULL on failure. */
+ * (XTG_KV_BF16), E4M3 codes with one FP32 scale per (position, KV head) (XTG_KV_FP8), or E2M1 codes with an E4M3
+ * scale per 16 dims (XTG_KV_NVFP4, 0.5625 bytes per value). Every slot starts empty. NULL on failure. An NVFP4 cache is
+ * read by xtg_hip_attention_ext; the other attention calls and the Dory session refuse it. */
 xtg_hip_kv* xtg_hip_kv_create(xtg_hip* h, int kv_heads, int head_dim, int64_t slots, int ring, int dtype, char* err,
                               int err_len);
 void xtg_hip_kv_destroy(xtg_hip* h, xtg_hip_kv* kv);
@@ -138,12 +140,30 @@ void xtg_hip_kv_destroy(xtg_hip* h, xtg_hip_kv* kv);
  * beyond its capacity ("KV cache full"). */
 int xtg_hip_kv_store(xtg_hip* h, xtg_hip_kv* kv, int64_t pos, int n, const float* k, const float* v, char* err,
                      int err_len);
+/* An NVFP4 cache's values are code * scale * global, with one global for K and one for V: powers of two from 2^-60 to
+ * 2^60, 1 unless this call sets them, which is possible as long as nothing has been written (or after
+ * xtg_hip_kv_release). Of each 16 dims, the scale is the E4M3 value nearest to (largest magnitude) / (6 * global), ties to
+ * even, at most 448 and, unless all 16 are zero, at least 2^-9; each code is the E2M1 value nearest to
+ * value / (scale * global), ties to even, at most 6. So magnitudes up to 2688 * global are held, and blocks whose largest
+ * is under 0.1 * global lose precision. A row with an infinity or a NaN among a KV head's K or V reads back as NaN, and
+ * attention gives NaN to the queries that see it and to no others. A captured graph keeps the globals of its capture. */
+int xtg_hip_kv_globals(xtg_hip* h, xtg_hip_kv* kv, float k_global, float v_global, char* err, int err_len);
+/* xtg_hip_kv_store for rows of either type (k, v: device [n][kv_heads][head_dim], x_dtype XTG_X_F32 or XTG_X_BF16,
+ * 16-byte aligned) and every cache dtype; queued. */
+int xtg_hip_kv_write(xtg_hip* h, xtg_hip_kv* kv, int64_t pos, int n, const void* k, const void* v, int x_dtype,
+                     char* err, int err_len);
+/* The other way: the rows of positions pos .. pos + n - 1 of every KV head, as the cache holds them, into device k, v
+ * [n][kv_heads][head_dim] of x_dtype (16-byte aligned; an FP8 cache's values are rounded to BF16, the others are exact);
+ * zeros for positions that the cache does not hold. Queued. */
+int xtg_hip_kv_read(xtg_hip* h, const xtg_hip_kv* kv, int64_t pos, int n, void* k, void* v, int x_dtype, char* err,
+                    int err_len);
 /* Replaces KvCache::load (kv.h:37, kv.cpp:114-138): FP32 K and V rows of head `head` for positions p0 .. p1 - 1
  * into host k, v [p1 - p0][head_dim]; waits for queued work. */
 int xtg_hip_kv_load(xtg_hip* h, const xtg_hip_kv* kv, int head, int64_t p0, int64_t p1, float* k, float* v, char* err,
                     int err_len);
-/* Replaces KvCache::save / restore / release (kv.h:45-48): the whole cache (K, V, FP8 scales and slot positions,
- * in the device layout) as xtg_hip_kv_bytes() host bytes and back; release empties every slot. */
+/* Replaces KvCache::save / restore / release (kv.h:45-48): the whole cache (K, V, FP8 or NVFP4 scales, slot positions,
+ * in the device layout, and an NVFP4 cache's globals, which have to be those of the cache it goes to) as
+ * xtg_hip_kv_bytes() host bytes and back; release empties every slot. */
 int64_t xtg_hip_kv_bytes(xtg_hip* h, const xtg_hip_kv* kv);
 int xtg_hip_kv_save(xtg_hip* h, const xtg_hip_kv* kv, void* out, size_t bytes, char* err, int err_len);
 int xtg_hip_kv_restore(xtg_hip* h, xtg_hip_kv* kv, const void* in, size_t bytes, char* err, int err_len);
@@ -184,6 +204,38 @@ int xtg_hip_attention(xtg_hip* h, const xtg_attn_args* a, char* err, int err_len
  * the owning backend's stream run in order; each rewrites every partial it reads. */
 #define XTG_HIP_ATTN_SCRATCH_BYTES (16u << 20)
 int xtg_hip_attention_noalloc(xtg_hip* h, const xtg_attn_args* a, char* err, int err_len);
+
+/* Attention with capped, biased and masked scores, over a cache of any dtype (no counterpart in the reference). Row i of
+ * the call, at position t = pos0 + i, sees the keys at positions p with
+ *     first[i] <= p < end[i],   and p > t - window where window > 0;
+ * first NULL: from 0; end NULL: to t (end[i] = t + 1). A document's start in `first` keeps packed documents apart; an
+ * `end` past t lets the rows of a prefix see all of it; first[i] >= end[i] (a padding row) leaves nothing. Its score for
+ * a key is s = (q . k) * scale, then softcap * tanh(s / softcap) where softcap > 0, then minus slopes[head] * |t - p|
+ * where slopes is given. A row that sees nothing gets zeros.
+ * The keys are the cache's (NULL: none) at positions before pos0, as their slots say, and the call's own k, v at pos0 ..
+ * pos0 + n_q - 1, not yet stored; with k and v NULL they are the cache's alone, the call's own rows among them.
+ * Rows are x_dtype: BF16, or FP32, of which q, k and v are rounded to BF16 as they are read (as a cache rounds what it
+ * stores) and out is not. Scores, their maxima and sums and the output are held in FP32; the softmax weights enter the
+ * product with V as f16 (11 bits; NVFP4 caches) or BF16 (8 bits; others, and own keys). No gradient. head_dim 64, 128 or
+ * 256; out overlaps no input. Queued; the first call of a shape sizes scratch memory (make it before a graph capture). */
+typedef struct xtg_attn_ext {
+  int n_q;
+  int64_t pos0;
+  int heads, kv_heads, head_dim;
+  int window;
+  float scale;
+  const void* q;          /* device [n_q][heads][head_dim], 16-byte aligned, as k, v and out */
+  const void* k;          /* device [n_q][kv_heads][head_dim] */
+  const void* v;
+  const xtg_hip_kv* cache;
+  void* out;              /* device [n_q][heads][head_dim] */
+  int x_dtype;            /* XTG_X_F32 or XTG_X_BF16, of q, k, v and out */
+  float softcap;          /* 0: none */
+  const float* slopes;    /* device [heads], or NULL */
+  const int32_t* first;   /* device [n_q], or NULL */
+  const int32_t* end;     /* device [n_q], or NULL */
+} xtg_attn_ext;
+int xtg_hip_attention_ext(xtg_hip* h, const xtg_attn_ext* a, char* err, int err_len);
 
 /* ----------------------------------------------------------------------------------------- row kernels */
 

@@ -14,7 +14,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("XTG_HIP_LIB") or os.path.join(HERE, "libxtg_hip.so")
 
 X_F32, X_BF16 = 0, 1
-KV_BF16, KV_FP8 = 0, 1
+KV_BF16, KV_FP8, KV_NVFP4 = 0, 1, 2
 LOGITS_NONE, LOGITS_LAST, LOGITS_ALL = 0, 1, 2   # xtg::Logits order (engine/include/xtg/model.h:28)
 
 # Every function the header declares, with its ctypes signature: (name, restype, argtypes).
@@ -44,6 +44,13 @@ class AttnArgs(ctypes.Structure):
     _fields_ = [("n_q", _I), ("pos0", ctypes.c_int64), ("heads", _I), ("kv_heads", _I), ("head_dim", _I),
                 ("window", _I), ("scale", ctypes.c_float), ("q", _P), ("k", _P), ("v", _P), ("cache", _P),
                 ("out", _P)]
+
+
+class AttnExt(ctypes.Structure):
+    """xtg_attn_ext."""
+    _fields_ = [("n_q", _I), ("pos0", ctypes.c_int64), ("heads", _I), ("kv_heads", _I), ("head_dim", _I),
+                ("window", _I), ("scale", ctypes.c_float), ("q", _P), ("k", _P), ("v", _P), ("cache", _P), ("out", _P),
+                ("x_dtype", _I), ("softcap", ctypes.c_float), ("slopes", _P), ("first", _P), ("end", _P)]
 
 
 _F = ctypes.c_float
@@ -79,6 +86,9 @@ SIGNATURES = [
     ("xtg_hip_kv_create", _P, [_P, _I, _I, _I64, _I, _I] + _ERR),
     ("xtg_hip_kv_destroy", None, [_P, _P]),
     ("xtg_hip_kv_store", _I, [_P, _P, _I64, _I, _P, _P] + _ERR),
+    ("xtg_hip_kv_globals", _I, [_P, _P, _F, _F] + _ERR),
+    ("xtg_hip_kv_write", _I, [_P, _P, _I64, _I, _P, _P, _I] + _ERR),
+    ("xtg_hip_kv_read", _I, [_P, _P, _I64, _I, _P, _P, _I] + _ERR),
     ("xtg_hip_kv_load", _I, [_P, _P, _I, _I64, _I64, _P, _P] + _ERR),
     ("xtg_hip_kv_bytes", _I64, [_P, _P]),
     ("xtg_hip_kv_save", _I, [_P, _P, _P, _SZ] + _ERR),
@@ -88,6 +98,7 @@ SIGNATURES = [
     ("xtg_hip_kv_release", _I, [_P, _P] + _ERR),
     ("xtg_hip_attention", _I, [_P, ctypes.POINTER(AttnArgs)] + _ERR),
     ("xtg_hip_attention_noalloc", _I, [_P, ctypes.POINTER(AttnArgs)] + _ERR),
+    ("xtg_hip_attention_ext", _I, [_P, ctypes.POINTER(AttnExt)] + _ERR),
     ("xtg_hip_qk_rope_norm", _I, [_P, _P, _P, _I, _I, _I, _I, _I64, _F, _P] + _ERR),
     ("xtg_hip_slerp_residual", _I, [_P, _P, _P, _P, _I, _I] + _ERR),
     ("xtg_hip_swiglu_norm", _I, [_P, _P, _P, _P, _P, _I, _I] + _ERR),
@@ -445,6 +456,20 @@ class HipBackend:
         err = _errbuf()
         _check(lib().xtg_hip_attention_noalloc(self.h, ctypes.byref(a), err, len(err)), err)
 
+    def attention_ext(self, cache, q, k, v, out, n_q, pos0, heads, kv_heads, head_dim, x_dtype=X_F32, window=0,
+                      scale=None, softcap=0.0, slopes=None, first=None, end=None):
+        """Queued device attention with capped, biased and masked scores (xtg_hip_attention_ext) over a cache of any
+        dtype (None: the call's own keys alone): row i, at t = pos0 + i, sees positions first[i] <= p < end[i] (None:
+        from 0, to t) and p > t - window; scores softcap * tanh(scale * q.k / softcap) - slopes[head] * |t - p|. k and
+        v None: the call's own rows are in the cache. q, k, v, out: device rows of x_dtype; slopes: device FP32
+        [heads]; first, end: device int32 [n_q]."""
+        sc = head_dim ** -0.5 if scale is None else scale
+        a = AttnExt(n_q, pos0, heads, kv_heads, head_dim, window, sc, _ptr(q), _ptr(k), _ptr(v),
+                    cache.h if cache is not None else None, _ptr(out), x_dtype, softcap, _ptr(slopes), _ptr(first),
+                    _ptr(end))
+        err = _errbuf()
+        _check(lib().xtg_hip_attention_ext(self.h, ctypes.byref(a), err, len(err)), err)
+
     # ---- the Dory decode step
     def dory(self, weights):
         """A decode session over DoryWeights (xtier_go_amd.workloads); the weights stay referenced by it."""
@@ -582,6 +607,22 @@ class KvCache:
         """Rows pos .. pos + n - 1 from device FP32 k, v [n][kv_heads][head_dim] (queued)."""
         err = _errbuf()
         _check(lib().xtg_hip_kv_store(self.b.h, self.h, pos, n, _ptr(k), _ptr(v), err, len(err)), err)
+
+    def globals(self, k_global, v_global):
+        """The two powers of two that an NVFP4 cache's scales are multiplied by; before anything is written."""
+        err = _errbuf()
+        _check(lib().xtg_hip_kv_globals(self.b.h, self.h, k_global, v_global, err, len(err)), err)
+
+    def write(self, pos, n, k, v, x_dtype=X_F32):
+        """store for device rows of x_dtype (queued)."""
+        err = _errbuf()
+        _check(lib().xtg_hip_kv_write(self.b.h, self.h, pos, n, _ptr(k), _ptr(v), x_dtype, err, len(err)), err)
+
+    def read(self, pos, n, k, v, x_dtype=X_F32):
+        """The rows of positions pos .. pos + n - 1 as the cache holds them into device k, v [n][kv_heads][head_dim] of
+        x_dtype, zeros where it holds none (queued)."""
+        err = _errbuf()
+        _check(lib().xtg_hip_kv_read(self.b.h, self.h, pos, n, _ptr(k), _ptr(v), x_dtype, err, len(err)), err)
 
     def store_host(self, pos, k, v):
         """Convenience: upload FP32 host rows, then store them."""

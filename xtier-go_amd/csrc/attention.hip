@@ -54,43 +54,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4;      // waves per work-group (one split)
 constexpr int kTile = 32;      // slots per tile
 
-// ------------------------------------------------------------------------------------------------ layout maths
-
-__host__ __device__ inline size_t k_index(int h, int slot, int dim, int slots_pad, int d) {
-  const int b = slot >> 4, i = slot & 15, c = dim >> 5, g = (dim & 31) >> 3, e = dim & 7;
-  return ((((size_t(h) * size_t(slots_pad >> 4) + size_t(b)) * size_t(d >> 5) + size_t(c)) * 64 + size_t(g * 16 + i)) * 8) +
-         size_t(e);
-}
-
-__host__ __device__ inline size_t v_index(int h, int slot, int dim, int slots_pad, int d) {
-  const int t = slot >> 5, kk = slot & 31;
-  const int half = kk >> 4, r = kk & 15;   // key 16 half + 4 g + (e & 3)
-  const int g = r >> 2, e = half * 4 + (r & 3);
-  const int dd = dim >> 4, i = dim & 15;
-  return ((((size_t(h) * size_t(slots_pad >> 5) + size_t(t)) * size_t(d >> 4) + size_t(dd)) * 64 + size_t(g * 16 + i)) * 8) +
-         size_t(e);
-}
-
-__host__ __device__ inline size_t k8_index(int h, int slot, int dim, int slots_pad, int d) {
-  const int b = slot >> 4, i = slot & 15, c = dim >> 5, g = (dim & 31) >> 3, e = dim & 7;
-  return ((((size_t(h) * size_t(slots_pad >> 4) + size_t(b)) * size_t(d >> 6) + size_t(c >> 1)) * 64 +
-           size_t(g * 16 + i)) * 16) + size_t((c & 1) * 8 + e);
-}
-
-__host__ __device__ inline size_t v8_index(int h, int slot, int dim, int slots_pad, int d) {
-  const int t = slot >> 5, kk = slot & 31;
-  const int half = kk >> 4, r = kk & 15;
-  const int g = r >> 2, e = half * 4 + (r & 3);
-  const int dd = dim >> 4, i = dim & 15;
-  return ((((size_t(h) * size_t(slots_pad >> 5) + size_t(t)) * size_t(d >> 5) + size_t(dd >> 1)) * 64 +
-           size_t(g * 16 + i)) * 16) + size_t((dd & 1) * 8 + e);
-}
-
-size_t kv_k_index(int h, int slot, int dim, int slots_pad, int d) { return k_index(h, slot, dim, slots_pad, d); }
-size_t kv_v_index(int h, int slot, int dim, int slots_pad, int d) { return v_index(h, slot, dim, slots_pad, d); }
-size_t kv_k8_index(int h, int slot, int dim, int slots_pad, int d) { return k8_index(h, slot, dim, slots_pad, d); }
-size_t kv_v8_index(int h, int slot, int dim, int slots_pad, int d) { return v8_index(h, slot, dim, slots_pad, d); }
-
 __device__ inline uint16_t f32_to_bf16_bits(float f) {
   // round to nearest even; a NaN stays a quiet NaN (engine/include/xtg/fp.h:18-24)
   uint32_t b = __float_as_uint(f);
@@ -138,7 +101,7 @@ __device__ inline void store_fp8_row(const float (&x)[D / 64], uint8_t* __restri
 #pragma unroll
   for (int u = 0; u < D / 64; ++u) {
     const int dim = lane + 64 * u;
-    const size_t at = is_v ? v8_index(h, slot, dim, slots_pad, D) : k8_index(h, slot, dim, slots_pad, D);
+    const size_t at = is_v ? kv_v8_index(h, slot, dim, slots_pad, D) : kv_k8_index(h, slot, dim, slots_pad, D);
     c8[at] = uint8_t(e4m3_code(x[u] * inv));
   }
   if (lane == 0) scl[size_t(h) * size_t(slots_pad) + size_t(slot)] = sc;
@@ -148,7 +111,8 @@ __device__ inline void store_fp8_row(const float (&x)[D / 64], uint8_t* __restri
 
 // One thread per (row, head, dim) of the rows kept (a ring keeps the last `slots` rows of a long call:
 // engine/src/kv.cpp:75-80); slot_pos is written by the dim-0 thread of head 0.
-__global__ void __launch_bounds__(256) kv_store_kernel(const float* __restrict__ k, const float* __restrict__ v,
+template <class X>
+__global__ void __launch_bounds__(256) kv_store_kernel(const X* __restrict__ k, const X* __restrict__ v,
                                                        uint16_t* __restrict__ ck, uint16_t* __restrict__ cv,
                                                        int* __restrict__ slot_pos, long long pos, int first, int n,
                                                        int kv_heads, int d, long long slots, int ring, int slots_pad) {
@@ -161,14 +125,14 @@ __global__ void __launch_bounds__(256) kv_store_kernel(const float* __restrict__
   const long long p = pos + r;
   const int slot = int(ring ? p % slots : p);
   const size_t src = (size_t(r) * size_t(kv_heads) + size_t(h)) * size_t(d) + size_t(dim);
-  ck[k_index(h, slot, dim, slots_pad, d)] = f32_to_bf16_bits(k[src]);
-  cv[v_index(h, slot, dim, slots_pad, d)] = f32_to_bf16_bits(v[src]);
+  ck[kv_k_index(h, slot, dim, slots_pad, d)] = f32_to_bf16_bits(float(k[src]));
+  cv[kv_v_index(h, slot, dim, slots_pad, d)] = f32_to_bf16_bits(float(v[src]));
   if (h == 0 && dim == 0) slot_pos[slot] = int(p);
 }
 
 // FP8: one wave per (row kept, head, K or V), 4 waves per work-group; slot_pos by the first wave of each row.
-template <int D>
-__global__ void __launch_bounds__(256) kv_store_fp8_kernel(const float* __restrict__ k, const float* __restrict__ v,
+template <int D, class X>
+__global__ void __launch_bounds__(256) kv_store_fp8_kernel(const X* __restrict__ k, const X* __restrict__ v,
                                                            uint8_t* __restrict__ ck, uint8_t* __restrict__ cv,
                                                            float* __restrict__ ks, float* __restrict__ vs,
                                                            int* __restrict__ slot_pos, long long pos, int first,
@@ -182,40 +146,49 @@ __global__ void __launch_bounds__(256) kv_store_fp8_kernel(const float* __restri
   const bool is_v = rem & 1;
   const long long p = pos + r;
   const int slot = int(ring ? p % slots : p);
-  const float* src = (is_v ? v : k) + (size_t(r) * size_t(kv_heads) + size_t(h)) * D;
+  const X* src = (is_v ? v : k) + (size_t(r) * size_t(kv_heads) + size_t(h)) * D;
   float x[D / 64];
 #pragma unroll
-  for (int u = 0; u < D / 64; ++u) x[u] = src[(threadIdx.x & 63) + 64 * u];
+  for (int u = 0; u < D / 64; ++u) x[u] = float(src[(threadIdx.x & 63) + 64 * u]);
   store_fp8_row<D>(x, is_v ? cv : ck, is_v ? vs : ks, is_v, h, slot, slots_pad);
   if (rem == 0 && (threadIdx.x & 63) == 0) slot_pos[slot] = int(p);
 }
 
-std::string launch_kv_store(const DevKv& c, long long pos, int n, const float* k, const float* v,
-                            hipStream_t stream) {
-  int first = 0;
-  if (c.ring && n > c.slots) first = int(n - c.slots);
-  if (n - first <= 0) return std::string();
+template <class X>
+static std::string launch_kv_store_rows(const DevKv& c, long long pos, int first, int n, const X* k, const X* v,
+                                        hipStream_t stream) {
   if (c.fp8) {
     const long long waves = (long long)(n - first) * 2 * c.kv_heads;
     const dim3 grid{unsigned((waves + 3) / 4)}, block{256};
     auto* ck = static_cast<uint8_t*>(c.k);
     auto* cv = static_cast<uint8_t*>(c.v);
-#define XTG_STORE8(D)                                                                                        \
-  if (c.head_dim == D)                                                                                      \
-    hipLaunchKernelGGL(kv_store_fp8_kernel<D>, grid, block, 0, stream, k, v, ck, cv, c.kscale, c.vscale,     \
+#define XTG_STORE8(D)                                                                                         \
+  if (c.head_dim == D)                                                                                       \
+    hipLaunchKernelGGL((kv_store_fp8_kernel<D, X>), grid, block, 0, stream, k, v, ck, cv, c.kscale, c.vscale, \
                        c.slot_pos, pos, first, n, c.kv_heads, (long long)c.slots, c.ring ? 1 : 0, c.slots_pad);
     XTG_STORE8(64) XTG_STORE8(128) XTG_STORE8(256)
 #undef XTG_STORE8
     HIP_CHECK(hipGetLastError());
-    return strf("kv_store_fp8_kernel<%d>", c.head_dim);
+    return strf(sizeof(X) == 2 ? "kv_store_fp8_kernel<%d, bf16>" : "kv_store_fp8_kernel<%d>", c.head_dim);
   }
   const long long total = (long long)(n - first) * c.kv_heads * c.head_dim;
   const unsigned blocks = unsigned((total + 255) / 256);
-  hipLaunchKernelGGL(kv_store_kernel, dim3(blocks), dim3(256), 0, stream, k, v, static_cast<uint16_t*>(c.k),
+  hipLaunchKernelGGL(kv_store_kernel<X>, dim3(blocks), dim3(256), 0, stream, k, v, static_cast<uint16_t*>(c.k),
                      static_cast<uint16_t*>(c.v), c.slot_pos, pos, first, n, c.kv_heads, c.head_dim,
                      (long long)c.slots, c.ring ? 1 : 0, c.slots_pad);
   HIP_CHECK(hipGetLastError());
-  return "kv_store_kernel";
+  return sizeof(X) == 2 ? "kv_store_kernel<bf16>" : "kv_store_kernel";
+}
+
+std::string launch_kv_store(const DevKv& c, long long pos, int n, const void* k, const void* v, hipStream_t stream,
+                            bool bf16) {
+  int first = 0;
+  if (c.ring && n > c.slots) first = int(n - c.slots);
+  if (n - first <= 0) return std::string();
+  if (c.fp4) return launch_kv_store4(c, pos, first, n, k, v, bf16, stream);
+  if (bf16)
+    return launch_kv_store_rows(c, pos, first, n, static_cast<const __bf16*>(k), static_cast<const __bf16*>(v), stream);
+  return launch_kv_store_rows(c, pos, first, n, static_cast<const float*>(k), static_cast<const float*>(v), stream);
 }
 
 
@@ -1840,7 +1813,7 @@ __device__ inline void produce_row(const ProduceArgs& a, int kvh, int r, float* 
     if (e < nk * D) {
       sv[e] = vv[u];
       if (a.store && !a.fp8 && e / D == nk - 1)
-        static_cast<uint16_t*>(a.cv)[v_index(kvh, int(slot_r), e % D, a.slots_pad, D)] = f32_to_bf16_bits(vv[u]);
+        static_cast<uint16_t*>(a.cv)[kv_v_index(kvh, int(slot_r), e % D, a.slots_pad, D)] = f32_to_bf16_bits(vv[u]);
     }
   }
   if (a.store && kvh == 0 && tid == 0) a.slot_pos[slot_r] = int(a.pos0 + r);
@@ -1895,8 +1868,8 @@ __device__ inline void produce_row(const ProduceArgs& a, int kvh, int r, float* 
           }
           if (a.store && !a.fp8) {
             uint16_t* ck = static_cast<uint16_t*>(a.ck);
-            ck[k_index(kvh, int(slot_r), i, a.slots_pad, D)] = f32_to_bf16_bits(o1[u]);
-            ck[k_index(kvh, int(slot_r), i + HALF, a.slots_pad, D)] = f32_to_bf16_bits(o2[u]);
+            ck[kv_k_index(kvh, int(slot_r), i, a.slots_pad, D)] = f32_to_bf16_bits(o1[u]);
+            ck[kv_k_index(kvh, int(slot_r), i + HALF, a.slots_pad, D)] = f32_to_bf16_bits(o2[u]);
           }
         }
       }

@@ -17,26 +17,63 @@ struct DevKv {
   int slots_pad = 0;
   bool ring = false;
   bool fp8 = false;            // E4M3 codes + an FP32 scale per (slot, head) (kv.cpp:94-108), else BF16
-  void* k = nullptr;           // kv_heads * slots_pad * head_dim elements (2 bytes BF16, 1 byte FP8)
+  bool fp4 = false;            // NVFP4: E2M1 codes + an E4M3 scale per 16 dims (kv4.hpp)
+  void* k = nullptr;           // kv_heads * slots_pad * head_dim elements (2 bytes BF16, 1 byte FP8, a half NVFP4)
   void* v = nullptr;
-  float* kscale = nullptr;     // FP8: [kv_heads][slots_pad]
+  float* kscale = nullptr;     // FP8: [kv_heads][slots_pad]; NVFP4: the E4M3 bytes (scales4)
   float* vscale = nullptr;
   int* slot_pos = nullptr;     // slots_pad, -1 = empty
+  float kglobal = 1.f, vglobal = 1.f;   // NVFP4: what every scale is multiplied by, powers of two
+  bool written = false;        // something has been written since it was created or released
   size_t elems() const { return size_t(kv_heads) * size_t(slots_pad) * size_t(head_dim); }
-  size_t data_bytes() const { return elems() * (fp8 ? 1 : 2); }
-  size_t scale_bytes() const { return fp8 ? size_t(kv_heads) * size_t(slots_pad) * sizeof(float) : 0; }
+  size_t data_bytes() const { return fp4 ? elems() / 2 : elems() * (fp8 ? 1 : 2); }
+  size_t scale_bytes() const {
+    return fp4 ? elems() / 16 : fp8 ? size_t(kv_heads) * size_t(slots_pad) * sizeof(float) : 0;
+  }
+  int dtype() const { return fp4 ? 2 : fp8 ? 1 : 0; }   // XTG_KV_*
 };
 
-// Element offsets of (head, slot, dim) in the K and V layouts (for host-side load / save), BF16 and FP8.
-size_t kv_k_index(int h, int slot, int dim, int slots_pad, int d);
-size_t kv_v_index(int h, int slot, int dim, int slots_pad, int d);
-size_t kv_k8_index(int h, int slot, int dim, int slots_pad, int d);
-size_t kv_v8_index(int h, int slot, int dim, int slots_pad, int d);
+// Element offsets of (head, slot, dim) in the K and V layouts, BF16 and FP8.
+__host__ __device__ inline size_t kv_k_index(int h, int slot, int dim, int slots_pad, int d) {
+  const int b = slot >> 4, i = slot & 15, c = dim >> 5, g = (dim & 31) >> 3, e = dim & 7;
+  return ((((size_t(h) * size_t(slots_pad >> 4) + size_t(b)) * size_t(d >> 5) + size_t(c)) * 64 + size_t(g * 16 + i)) * 8) +
+         size_t(e);
+}
 
-// The rows of positions pos .. pos + n - 1 from FP32 device k, v [n][kv_heads][head_dim]; a ring keeps the last
-// `slots` rows.
-std::string launch_kv_store(const DevKv& c, long long pos, int n, const float* k, const float* v,
-                            hipStream_t stream);
+__host__ __device__ inline size_t kv_v_index(int h, int slot, int dim, int slots_pad, int d) {
+  const int t = slot >> 5, kk = slot & 31;
+  const int half = kk >> 4, r = kk & 15;   // key 16 half + 4 g + (e & 3)
+  const int g = r >> 2, e = half * 4 + (r & 3);
+  const int dd = dim >> 4, i = dim & 15;
+  return ((((size_t(h) * size_t(slots_pad >> 5) + size_t(t)) * size_t(d >> 4) + size_t(dd)) * 64 + size_t(g * 16 + i)) * 8) +
+         size_t(e);
+}
+
+__host__ __device__ inline size_t kv_k8_index(int h, int slot, int dim, int slots_pad, int d) {
+  const int b = slot >> 4, i = slot & 15, c = dim >> 5, g = (dim & 31) >> 3, e = dim & 7;
+  return ((((size_t(h) * size_t(slots_pad >> 4) + size_t(b)) * size_t(d >> 6) + size_t(c >> 1)) * 64 +
+           size_t(g * 16 + i)) * 16) + size_t((c & 1) * 8 + e);
+}
+
+__host__ __device__ inline size_t kv_v8_index(int h, int slot, int dim, int slots_pad, int d) {
+  const int t = slot >> 5, kk = slot & 31;
+  const int half = kk >> 4, r = kk & 15;
+  const int g = r >> 2, e = half * 4 + (r & 3);
+  const int dd = dim >> 4, i = dim & 15;
+  return ((((size_t(h) * size_t(slots_pad >> 5) + size_t(t)) * size_t(d >> 5) + size_t(dd >> 1)) * 64 +
+           size_t(g * 16 + i)) * 16) + size_t((dd & 1) * 8 + e);
+}
+
+// The rows of positions pos .. pos + n - 1 from device k, v [n][kv_heads][head_dim], FP32 or (bf16) BF16; a ring keeps
+// the last `slots` rows.
+std::string launch_kv_store(const DevKv& c, long long pos, int n, const void* k, const void* v, hipStream_t stream,
+                            bool bf16 = false);
+// The same into an NVFP4 cache (kv4.hip); launch_kv_store calls it.
+std::string launch_kv_store4(const DevKv& c, long long pos, int first, int n, const void* k, const void* v, bool bf16,
+                             hipStream_t stream);
+// The rows of positions pos .. pos + n - 1 of a cache of any dtype into device k, v [n][kv_heads][head_dim], FP32 or
+// BF16; zeros for a position that the cache does not hold (kv4.hip).
+std::string launch_kv_read(const DevKv& c, long long pos, int n, void* k, void* v, bool bf16, hipStream_t stream);
 
 // How one attention call (n_q query rows at pos0) is cut up. Query rows go in blocks of rpb rows (at most 32
 // (row, head) columns per KV head); each block's key tiles go to `splits` work-groups per KV head, plus `own`

@@ -7,6 +7,7 @@
 #include <memory>
 
 #include "common.hpp"
+#include "kv4.hpp"
 
 namespace xtg::hip {
 
@@ -360,7 +361,8 @@ void Backend::matmul_bf16(const xtg_bf16& w, const float* x, int m, float* y) {
 
 DevKv* Backend::kv_create(int kv_heads, int head_dim, long long slots, int ring, int dtype) {
   XTG_CHECK(!capturing_, "kv_create: not during a graph capture");
-  XTG_CHECK(dtype == XTG_KV_BF16 || dtype == XTG_KV_FP8, "kv_create: unknown KV dtype %d", dtype);
+  XTG_CHECK(dtype == XTG_KV_BF16 || dtype == XTG_KV_FP8 || dtype == XTG_KV_NVFP4, "kv_create: unknown KV dtype %d",
+            dtype);
   XTG_CHECK(head_dim == 64 || head_dim == 128 || head_dim == 256, "kv_create: head_dim %d (64, 128 or 256)",
             head_dim);
   XTG_CHECK(kv_heads > 0, "kv_create: %d KV heads", kv_heads);
@@ -373,11 +375,12 @@ DevKv* Backend::kv_create(int kv_heads, int head_dim, long long slots, int ring,
   c->slots_pad = int((n + 31) / 32 * 32);
   c->ring = ring > 0;
   c->fp8 = dtype == XTG_KV_FP8;
+  c->fp4 = dtype == XTG_KV_NVFP4;
   try {
     HIP_CHECK(hipMalloc(&c->k, c->data_bytes()));
     HIP_CHECK(hipMalloc(&c->v, c->data_bytes()));
     HIP_CHECK(hipMalloc(&c->slot_pos, size_t(c->slots_pad) * sizeof(int)));
-    if (c->fp8) {
+    if (c->scale_bytes()) {
       HIP_CHECK(hipMalloc(&c->kscale, c->scale_bytes()));
       HIP_CHECK(hipMalloc(&c->vscale, c->scale_bytes()));
     }
@@ -397,12 +400,13 @@ DevKv* Backend::kv_create(int kv_heads, int head_dim, long long slots, int ring,
 void Backend::clear_kv(DevKv* c) {
   HIP_CHECK(hipMemsetAsync(c->k, 0, c->data_bytes(), stream_));
   HIP_CHECK(hipMemsetAsync(c->v, 0, c->data_bytes(), stream_));
-  if (c->fp8) {
+  if (c->scale_bytes()) {
     HIP_CHECK(hipMemsetAsync(c->kscale, 0, c->scale_bytes(), stream_));
     HIP_CHECK(hipMemsetAsync(c->vscale, 0, c->scale_bytes(), stream_));
   }
   HIP_CHECK(hipMemsetAsync(c->slot_pos, 0xff, size_t(c->slots_pad) * sizeof(int), stream_));
   HIP_CHECK(hipStreamSynchronize(stream_));
+  c->written = false;
 }
 
 void Backend::kv_destroy(DevKv* c) {
@@ -416,15 +420,56 @@ void Backend::kv_destroy(DevKv* c) {
   delete c;
 }
 
-void Backend::kv_store(DevKv* c, long long pos, int n, const float* k, const float* v) {
-  XTG_CHECK(kvs_.count(c), "kv_store: unknown cache");
-  XTG_CHECK(n >= 0 && pos >= 0, "kv_store: %d rows at %lld", n, pos);
+void Backend::kv_globals(DevKv* c, float kglobal, float vglobal) {
+  XTG_CHECK(kvs_.count(c), "kv_globals: unknown cache");
+  XTG_CHECK(c->fp4, "kv_globals: not an NVFP4 cache");
+  XTG_CHECK(!c->written, "kv_globals: the cache has been written (release it first)");
+  for (float g : {kglobal, vglobal}) {
+    int e = 0;
+    XTG_CHECK(g > 0.f && std::frexp(g, &e) == 0.5f && e >= -59 && e <= 61,
+              "kv_globals: %g is not a power of two from 2^-60 to 2^60", double(g));
+  }
+  c->kglobal = kglobal;
+  c->vglobal = vglobal;
+}
+
+void Backend::check_rows(const char* what, const DevKv* c, long long pos, int n, const void* k, const void* v,
+                         int x_dtype) const {
+  XTG_CHECK(kvs_.count(const_cast<DevKv*>(c)), "%s: unknown cache", what);
+  XTG_CHECK(n >= 0 && pos >= 0, "%s: %d rows at %lld", what, n, pos);
   // kv.cpp:78: a linear cache holds positions below its capacity
   XTG_CHECK(c->ring || pos + n <= c->slots, "KV cache full: position %lld of %lld", pos + n, c->slots);
-  XTG_CHECK(pos + n < (1LL << 31), "kv_store: position %lld beyond the 32-bit slot positions", pos + n);
+  XTG_CHECK(pos + n < (1LL << 31), "%s: position %lld beyond the 32-bit slot positions", what, pos + n);
+  XTG_CHECK(x_dtype == kXF32 || x_dtype == kXBF16, "%s: unknown row type %d", what, x_dtype);
+  XTG_CHECK(n == 0 || (k && v), "%s: NULL rows", what);
+}
+
+void Backend::kv_store(DevKv* c, long long pos, int n, const float* k, const float* v) {
+  check_rows("kv_store", c, pos, n, k, v, kXF32);
+  if (c->fp4) {
+    kv_write(c, pos, n, k, v, kXF32);
+    return;
+  }
   if (n == 0) return;
-  XTG_CHECK(k && v, "kv_store: NULL rows");
+  c->written = true;
   timed([&] { return launch_kv_store(*c, pos, n, k, v, stream_); });
+}
+
+static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+void Backend::kv_write(DevKv* c, long long pos, int n, const void* k, const void* v, int x_dtype) {
+  check_rows("kv_write", c, pos, n, k, v, x_dtype);
+  if (n == 0) return;
+  XTG_CHECK(aligned16(k) && aligned16(v), "kv_write: rows must be 16-byte aligned");
+  c->written = true;
+  timed([&] { return launch_kv_store(*c, pos, n, k, v, stream_, x_dtype == kXBF16); });
+}
+
+void Backend::kv_read(const DevKv* c, long long pos, int n, void* k, void* v, int x_dtype) {
+  check_rows("kv_read", c, pos, n, k, v, x_dtype);
+  if (n == 0) return;
+  XTG_CHECK(aligned16(k) && aligned16(v), "kv_read: rows must be 16-byte aligned");
+  timed([&] { return launch_kv_read(*c, pos, n, k, v, x_dtype == kXBF16, stream_); });
 }
 
 namespace {
@@ -460,7 +505,16 @@ void Backend::kv_load(const DevKv* c, int h, long long p0, long long p1, float* 
     const int slot = int(c->ring ? p % c->slots : p);
     float* ok = k + size_t(p - p0) * size_t(d);
     float* ov = v + size_t(p - p0) * size_t(d);
-    if (c->fp8) {
+    if (c->fp4) {
+      const uint8_t* s4 = hv + c->data_bytes();
+      for (int j = 0; j < d; ++j) {
+        const Code4 ck = k4_code(h, slot, j, c->slots_pad, d), cv = v4_code(h, slot, j, c->slots_pad, d);
+        ok[j] = e2m1_value(hk[ck.byte] >> (4 * ck.high) & 15) *
+                e4m3_scale_value(s4[k4_scale(h, slot, j, c->slots_pad, d)]) * c->kglobal;
+        ov[j] = e2m1_value(hv[cv.byte] >> (4 * cv.high) & 15) *
+                e4m3_scale_value(s4[c->scale_bytes() + v4_scale(h, slot, j, c->slots_pad, d)]) * c->vglobal;
+      }
+    } else if (c->fp8) {
       const size_t si = size_t(h) * size_t(c->slots_pad) + size_t(slot);
       for (int j = 0; j < d; ++j) {   // kv.cpp:128-136: code value times the row's scale
         ok[j] = e4m3_value(hk[kv_k8_index(h, slot, j, c->slots_pad, d)]) * ks[si];
@@ -479,9 +533,11 @@ void Backend::kv_load(const DevKv* c, int h, long long p0, long long p1, float* 
   }
 }
 
-// Snapshot layout: K data, V data, K scales, V scales (FP8 only), slot positions, each in its device layout.
+// Snapshot layout: K data, V data, K scales, V scales (FP8 and NVFP4), slot positions, each in its device layout, and
+// an NVFP4 cache's two globals.
 size_t Backend::kv_bytes(const DevKv* c) const {
-  return 2 * c->data_bytes() + 2 * c->scale_bytes() + size_t(c->slots_pad) * sizeof(int);
+  return 2 * c->data_bytes() + 2 * c->scale_bytes() + size_t(c->slots_pad) * sizeof(int) +
+         (c->fp4 ? 2 * sizeof(float) : 0);
 }
 
 void Backend::snapshot(const DevKv* c, void* out) {
@@ -496,6 +552,10 @@ void Backend::snapshot(const DevKv* c, void* out) {
   HIP_CHECK(hipMemcpyAsync(o + 2 * db + 2 * sb, c->slot_pos, size_t(c->slots_pad) * sizeof(int),
                            hipMemcpyDeviceToHost, stream_));
   HIP_CHECK(hipStreamSynchronize(stream_));
+  if (c->fp4) {
+    const float g[2] = {c->kglobal, c->vglobal};
+    std::memcpy(o + kv_bytes(c) - sizeof g, g, sizeof g);
+  }
 }
 
 void Backend::kv_save(const DevKv* c, void* out, size_t bytes) {
@@ -511,6 +571,14 @@ void Backend::kv_restore(DevKv* c, const void* in, size_t bytes) {
   XTG_CHECK(bytes == kv_bytes(c), "KV snapshot of %zu bytes for a cache of %zu", bytes, kv_bytes(c));
   const char* s = static_cast<const char*>(in);
   const size_t db = c->data_bytes(), sb = c->scale_bytes();
+  if (c->fp4) {
+    float g[2];
+    std::memcpy(g, s + bytes - sizeof g, sizeof g);
+    XTG_CHECK(g[0] == c->kglobal && g[1] == c->vglobal,
+              "KV snapshot with globals %g, %g for a cache with %g, %g", double(g[0]), double(g[1]),
+              double(c->kglobal), double(c->vglobal));
+  }
+  c->written = true;
   HIP_CHECK(hipMemcpyAsync(c->k, s, db, hipMemcpyHostToDevice, stream_));
   HIP_CHECK(hipMemcpyAsync(c->v, s + db, db, hipMemcpyHostToDevice, stream_));
   if (sb) {
@@ -531,12 +599,14 @@ void Backend::kv_release(DevKv* c) {
 void Backend::kv_copy(const DevKv* src, DevKv* dst) {
   XTG_CHECK(kvs_.count(const_cast<DevKv*>(src)) && kvs_.count(dst), "kv_copy: unknown cache");
   XTG_CHECK(src->kv_heads == dst->kv_heads && src->head_dim == dst->head_dim && src->slots == dst->slots &&
-                src->ring == dst->ring && src->fp8 == dst->fp8,
+                src->ring == dst->ring && src->dtype() == dst->dtype(),
             "kv_copy: caches of different shapes or dtypes");
+  XTG_CHECK(src->kglobal == dst->kglobal && src->vglobal == dst->vglobal, "kv_copy: caches of different globals");
   if (src == dst) return;
+  dst->written = true;
   HIP_CHECK(hipMemcpyAsync(dst->k, src->k, src->data_bytes(), hipMemcpyDeviceToDevice, stream_));
   HIP_CHECK(hipMemcpyAsync(dst->v, src->v, src->data_bytes(), hipMemcpyDeviceToDevice, stream_));
-  if (src->fp8) {
+  if (src->scale_bytes()) {
     HIP_CHECK(hipMemcpyAsync(dst->kscale, src->kscale, src->scale_bytes(), hipMemcpyDeviceToDevice, stream_));
     HIP_CHECK(hipMemcpyAsync(dst->vscale, src->vscale, src->scale_bytes(), hipMemcpyDeviceToDevice, stream_));
   }
@@ -548,6 +618,7 @@ void Backend::check_attention(const DevKv* c, int n_q, long long pos0, const flo
                               const float* out) const {
   XTG_CHECK(kvs_.count(const_cast<DevKv*>(c)), "attention: unknown cache");
   XTG_CHECK(n_q >= 1 && pos0 >= 0, "attention: %d rows at %lld", n_q, pos0);
+  XTG_CHECK(!c->fp4, "attention: an NVFP4 cache is read by xtg_hip_attention_ext");
   XTG_CHECK(q && k && v && out, "attention: NULL argument");
   for (const void* p : {static_cast<const void*>(q), static_cast<const void*>(k), static_cast<const void*>(v),
                         static_cast<const void*>(out)})
@@ -603,10 +674,35 @@ void Backend::attention(const DevKv* c, int n_q, long long pos0, int heads, int 
   attention_launches(c, p, n_q, pos0, heads, window, scale, q, k, v, out, static_cast<float*>(part_));
 }
 
+void Backend::attention_ext(const ExtCall& a) {
+  XTG_CHECK(a.n_q >= 1 && a.pos0 >= 0 && a.pos0 + a.n_q < (1LL << 31), "attention_ext: %d rows at %lld", a.n_q, a.pos0);
+  XTG_CHECK(a.d == 64 || a.d == 128 || a.d == 256, "attention_ext: head_dim %d (64, 128 or 256)", a.d);
+  XTG_CHECK(a.kv_heads >= 1 && a.heads >= 1 && a.heads % a.kv_heads == 0 && a.kv_heads < 65536,
+            "attention_ext: %d heads over %d KV heads", a.heads, a.kv_heads);
+  XTG_CHECK((long long)a.n_q * (a.heads / a.kv_heads) < (1LL << 31), "attention_ext: %d rows of %d heads", a.n_q, a.heads);
+  XTG_CHECK(a.x_dtype == kXF32 || a.x_dtype == kXBF16, "attention_ext: unknown row type %d", a.x_dtype);
+  XTG_CHECK(std::isfinite(a.scale), "attention_ext: scale %g", double(a.scale));
+  XTG_CHECK(std::isfinite(a.softcap) && a.softcap >= 0.f, "attention_ext: softcap %g", double(a.softcap));
+  XTG_CHECK(a.q && a.out, "attention_ext: NULL argument");
+  XTG_CHECK(!a.k == !a.v, "attention_ext: one of k and v is NULL (both, or neither)");
+  XTG_CHECK(a.k || a.cache, "attention_ext: neither a cache nor keys of the call");
+  for (const void* p : {a.q, a.k, a.v, static_cast<const void*>(a.out)})
+    XTG_CHECK(aligned16(p), "attention_ext: rows must be 16-byte aligned");
+  for (const void* p : {static_cast<const void*>(a.slopes), static_cast<const void*>(a.first), static_cast<const void*>(a.end)})
+    XTG_CHECK(reinterpret_cast<uintptr_t>(p) % 4 == 0, "attention_ext: slopes, first and end must be 4-byte aligned");
+  if (a.cache) {
+    XTG_CHECK(kvs_.count(const_cast<DevKv*>(a.cache)), "attention_ext: unknown cache");
+    XTG_CHECK(a.cache->kv_heads == a.kv_heads && a.cache->head_dim == a.d,
+              "attention_ext: a cache of %d KV heads of %d for a call of %d of %d", a.cache->kv_heads,
+              a.cache->head_dim, a.kv_heads, a.d);
+  }
+  timed([&] { return launch_attn_ext(a, stream_); });
+}
+
 void Backend::attn_step(DevKv* c, int m, long long pos0, int heads, int window, float scale, float theta, float* q,
                         float* k, const float* v, const float* qscale, const float* g, const float* gscale,
                         float* out, void* op, bool store, float* gate_rec) {
-  XTG_CHECK(kvs_.count(c), "attention step: unknown cache");
+  XTG_CHECK(kvs_.count(c) && !c->fp4, "attention step: unknown cache, or an NVFP4 one");
   XTG_CHECK(!gate_rec || (m == 1 && out && !op), "attention step: the gate's records take one row, out and no operand");
   XTG_CHECK(m >= 1 && pos0 >= 0, "attention step: %d rows at %lld", m, pos0);
   XTG_CHECK(pos0 + m < (1LL << 31), "attention step: position %lld beyond the 32-bit slot positions", pos0 + m);

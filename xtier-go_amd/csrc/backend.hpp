@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "attention.hpp"
+#include "attention_ext.hpp"
 #include "common.hpp"
 #include "kernels.hpp"
 #include "rows.hpp"
@@ -71,6 +72,11 @@ class Backend {
   DevKv* kv_create(int kv_heads, int head_dim, long long slots, int ring, int dtype);
   void kv_destroy(DevKv* c);
   void kv_store(DevKv* c, long long pos, int n, const float* k, const float* v);            // device k, v
+  // NVFP4: what the cache's scales are multiplied by, powers of two; before anything is written
+  void kv_globals(DevKv* c, float kglobal, float vglobal);
+  // rows of either type into a cache of any dtype, and back (zeros where the cache does not hold the position)
+  void kv_write(DevKv* c, long long pos, int n, const void* k, const void* v, int x_dtype);
+  void kv_read(const DevKv* c, long long pos, int n, void* k, void* v, int x_dtype);
   void kv_load(const DevKv* c, int h, long long p0, long long p1, float* k, float* v);      // host k, v
   size_t kv_bytes(const DevKv* c) const;
   void kv_save(const DevKv* c, void* out, size_t bytes);
@@ -86,6 +92,8 @@ class Backend {
   // another open backend on the device holds the array (attn_scratch_claim: the first caller keeps it until closed).
   void attention_noalloc(const DevKv* c, int n_q, long long pos0, int heads, int window, float scale, const float* q,
                          const float* k, const float* v, float* out);
+  // Attention over a cache of any dtype with capped, biased and masked scores (attention_ext.hpp).
+  void attention_ext(const ExtCall& a);
   // The attention half of a Dory sublayer (packs/dory/dory.cpp:482-515) on device rows q [m][heads][d],
   // k / v [m][kv_heads][d], g [m][heads * d]: RoPE + norms of q (rewritten) and k, the attention over the cache
   // and this call's keys, the store of k / v into the cache, then out (optional) and op (optional, the
@@ -168,6 +176,8 @@ class Backend {
 
  private:
   void ensure(void*& buf, size_t& size, size_t need);
+  void check_rows(const char* what, const DevKv* c, long long pos, int n, const void* k, const void* v,
+                  int x_dtype) const;
   void check_attention(const DevKv* c, int n_q, long long pos0, const float* q, const float* k, const float* v,
                        const float* out) const;
   // the attention call's launches on partials `part`: for a call of one row block with cached keys to scan, its own

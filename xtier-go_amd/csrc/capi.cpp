@@ -157,6 +157,29 @@ int xtg_hip_kv_store(xtg_hip* h, xtg_hip_kv* kv, int64_t pos, int n, const float
   });
 }
 
+int xtg_hip_kv_globals(xtg_hip* h, xtg_hip_kv* kv, float k_global, float v_global, char* err, int err_len) {
+  return guarded(err, err_len, [&] {
+    XTG_CHECK(h && kv, "kv_globals: NULL argument");
+    h->b->kv_globals(reinterpret_cast<xtg::hip::DevKv*>(kv), k_global, v_global);
+  });
+}
+
+int xtg_hip_kv_write(xtg_hip* h, xtg_hip_kv* kv, int64_t pos, int n, const void* k, const void* v, int x_dtype,
+                     char* err, int err_len) {
+  return guarded(err, err_len, [&] {
+    XTG_CHECK(h && kv, "kv_write: NULL argument");
+    h->b->kv_write(reinterpret_cast<xtg::hip::DevKv*>(kv), pos, n, k, v, x_dtype);
+  });
+}
+
+int xtg_hip_kv_read(xtg_hip* h, const xtg_hip_kv* kv, int64_t pos, int n, void* k, void* v, int x_dtype, char* err,
+                    int err_len) {
+  return guarded(err, err_len, [&] {
+    XTG_CHECK(h && kv, "kv_read: NULL argument");
+    h->b->kv_read(reinterpret_cast<const xtg::hip::DevKv*>(kv), pos, n, k, v, x_dtype);
+  });
+}
+
 int xtg_hip_kv_load(xtg_hip* h, const xtg_hip_kv* kv, int head, int64_t p0, int64_t p1, float* k, float* v, char* err,
                     int err_len) {
   return guarded(err, err_len, [&] {
@@ -224,6 +247,15 @@ int xtg_hip_attention_noalloc(xtg_hip* h, const xtg_attn_args* a, char* err, int
               "attention_noalloc: %d KV heads of %d for a cache of %d of %d", a->kv_heads, a->head_dim, c->kv_heads,
               c->head_dim);
     h->b->attention_noalloc(c, a->n_q, a->pos0, a->heads, a->window, a->scale, a->q, a->k, a->v, a->out);
+  });
+}
+
+int xtg_hip_attention_ext(xtg_hip* h, const xtg_attn_ext* a, char* err, int err_len) {
+  return guarded(err, err_len, [&] {
+    XTG_CHECK(h && a, "attention_ext: NULL argument");
+    h->b->attention_ext({reinterpret_cast<const xtg::hip::DevKv*>(a->cache), a->n_q, a->pos0, a->heads, a->kv_heads,
+                         a->head_dim, a->window, a->scale, a->q, a->k, a->v, a->out, a->x_dtype, a->softcap, a->slopes,
+                         a->first, a->end});
   });
 }
 

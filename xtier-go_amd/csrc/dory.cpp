@@ -67,6 +67,7 @@ void DorySession::build(const xtg_dory_layer* layers, const float* logit_scale) 
   const int n_layers = c.n_in + c.n_rec + c.n_out;
   XTG_CHECK(n_layers > 0 && c.loops >= 1, "dory: %d sublayers, %d loops", n_layers, c.loops);
   XTG_CHECK(c.heads % c.kv_heads == 0 && c.head_dim % 2 == 0, "dory: unsupported attention shape");
+  XTG_CHECK(c.kv_dtype == XTG_KV_BF16 || c.kv_dtype == XTG_KV_FP8, "dory: KV dtype %d (BF16 or FP8)", c.kv_dtype);
   XTG_CHECK(c.kv_mode == XTG_KV_PER_LOOP || c.kv_mode == XTG_KV_LAST_LOOP, "dory: kv_mode %d (per_loop | last_loop)",
             c.kv_mode);
   const int H = c.hidden, Q = c.heads * c.head_dim, KV = c.kv_heads * c.head_dim, F = c.ffn;
