@@ -66,7 +66,9 @@ def stored_fp8(x):
 
 def attend(q, k, v, at, pos0, scale, window=0, softcap=0.0, slopes=None, first=None, end=None):
     """q [n][heads][d] over keys k, v [m][kv][d] at positions `at` [m] (64-bit values). Returns the outputs, the sum of
-    |weight * value| that each is made of, and the largest sum of |q.k| * scale of a score (for tolerances)."""
+    |weight * value| that each is made of with 2^-32 of the sum of |value| (weights are at least the size of f16's
+    smallest step, 2^-24, or lost: with the largest at 2^7 or more, by half a step, 2^-32 of it), and the largest sum
+    of |q.k| * scale of a score (for tolerances)."""
     q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
     n, heads, d = q.shape
     kvh = k.shape[1]
@@ -76,7 +78,7 @@ def attend(q, k, v, at, pos0, scale, window=0, softcap=0.0, slopes=None, first=N
         lo = np.maximum(lo, t - window + 1)
     hi = t + 1 if end is None else np.asarray(end)
     seen = (at[None, :] >= lo[:, None]) & (at[None, :] < hi[:, None]) & (at[None, :] >= 0)
-    out, size, most = np.zeros_like(q), np.zeros_like(q), 0.0
+    out, size, floor, most = np.zeros_like(q), np.zeros_like(q), np.zeros_like(q), 0.0
     with np.errstate(all="ignore"):
         for h in range(heads):
             kh, vh = k[:, h * kvh // heads], v[:, h * kvh // heads]
@@ -97,7 +99,8 @@ def attend(q, k, v, at, pos0, scale, window=0, softcap=0.0, slopes=None, first=N
                 p /= p.sum()
                 out[i, h] = (p[:, None] * vh[w]).sum(0)
                 size[i, h] = (p[:, None] * np.abs(vh[w])).sum(0)
-    return out, size, most
+                floor[i, h] = np.abs(vh[w]).sum(0) * 2.0 ** -32
+    return out, (size, floor), most
 
 
 def tolerance(out, size, most, d, weight_bits, x_dtype):
@@ -108,5 +111,5 @@ def tolerance(out, size, most, d, weight_bits, x_dtype):
     terms: 2^-9 of the largest bound, 2^-17 in practice for sums of mixed order: 2^-14 is allowed); BF16 rows are
     rounded once more, by half a step, 2^-8."""
     e = (d + 16) * 2.0 ** -24 * (most + 1.0)
-    tol = size * (2.0 ** -weight_bits + 2 * e + 2.0 ** -14) + 1e-30
+    tol = size[0] * (2.0 ** -weight_bits + 2 * e + 2.0 ** -14) + size[1] + 1e-30
     return tol + (np.abs(out) + tol) * 2.0 ** -8 if x_dtype == BF16 else tol

@@ -3,6 +3,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <functional>
 #include <string>
 
 #include "attention.hpp"
@@ -25,6 +26,22 @@ struct ExtCall {
   const int* end;
 };
 
-std::string launch_attn_ext(const ExtCall& a, hipStream_t stream);
+// How a call is cut up. A q-col is a (row, q head of a KV head); a work-group takes `cols` of them for one KV head and
+// one of `splits` parts of the keys, and leaves a record (accumulator, maximum, sum) for each where there are more
+// than one. few: at most 32 q-cols, one block of them, whose work-groups' waves take cache tiles of their own; the last
+// record is the call's own keys'. Otherwise blocks of 128 q-cols share tiles, the call's own keys packed as tiles too.
+struct ExtPlan {
+  bool few = false;
+  int cols = 128, blocks = 1, splits = 1;
+  int tile_lo = 0, tiles = 0;    // few: the cache's 32-slot tiles to scan; else tile_lo = 0 and the slots to scan
+  size_t pack_bytes = 0;         // own keys and values as BF16 tiles
+  size_t record_bytes = 0;
+  size_t scratch_bytes() const { return pack_bytes + record_bytes; }
+};
+ExtPlan ext_plan(const ExtCall& a, int cus);
+
+// Queues the call's launches on scratch of the plan's size, each a callable that returns its name, given to `timed`.
+using Timed = std::function<void(const std::function<std::string()>&)>;
+void launch_attn_ext(const ExtCall& a, const ExtPlan& p, void* scratch, hipStream_t stream, const Timed& timed);
 
 }  // namespace xtg::hip

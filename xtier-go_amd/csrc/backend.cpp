@@ -16,6 +16,7 @@ Backend::Backend(int device) : device_(device) {
   HIP_CHECK(hipGetDeviceCount(&count));
   XTG_CHECK(device >= 0 && device < count, "no HIP device %d (%d present)", device, count);
   HIP_CHECK(hipSetDevice(device));
+  HIP_CHECK(hipDeviceGetAttribute(&cus_, hipDeviceAttributeMultiprocessorCount, device));
   HIP_CHECK(hipStreamCreateWithFlags(&stream_, hipStreamNonBlocking));
   attn_scratch_ = attn_scratch_ptr(device);   // with the device current, once per device
   const std::vector<float2> ident(128, make_float2(1.f, 0.f));   // head_dim up to 256
@@ -37,7 +38,7 @@ Backend::~Backend() {
   for (auto& kv : weights_) (void)hipFree(kv.second.tiles);
   for (auto& kv : bf16_weights_) (void)hipFree(kv.second.tiles);
   for (void* p : allocs_) (void)hipFree(p);
-  for (void* p : {op_, opb_, hx_, hy_, part_, kproc_, stage_, sample_, static_cast<void*>(ident_rope_)})
+  for (void* p : {op_, opb_, hx_, hy_, part_, kproc_, stage_, sample_, ext_, static_cast<void*>(ident_rope_)})
     if (p) (void)hipFree(p);
   for (void* p : retired_) (void)hipFree(p);
   for (DevKv* c : kvs_) {
@@ -696,7 +697,9 @@ void Backend::attention_ext(const ExtCall& a) {
               "attention_ext: a cache of %d KV heads of %d for a call of %d of %d", a.cache->kv_heads,
               a.cache->head_dim, a.kv_heads, a.d);
   }
-  timed([&] { return launch_attn_ext(a, stream_); });
+  const ExtPlan p = ext_plan(a, cus_);
+  ensure(ext_, ext_size_, p.scratch_bytes());
+  launch_attn_ext(a, p, ext_, stream_, [&](auto&& launch) { timed(launch); });
 }
 
 void Backend::attn_step(DevKv* c, int m, long long pos0, int heads, int window, float scale, float theta, float* q,

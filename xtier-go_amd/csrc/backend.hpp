@@ -230,6 +230,9 @@ class Backend {
   size_t kproc_size_ = 0;
   void* sample_ = nullptr;   // sampling scratch: weights and the radix sort's buffers
   size_t sample_size_ = 0;
+  void* ext_ = nullptr;      // attention_ext: packed own keys and records
+  size_t ext_size_ = 0;
+  int cus_ = 0;
   std::unordered_set<DevKv*> kvs_;
   std::vector<std::pair<std::pair<float, int>, float*>> inv_freq_;
   struct RopeTable {
