@@ -71,39 +71,31 @@ __host__ __device__ inline float e4m3_scale_value(uint8_t s) {
   return e == 0 ? float(m) * 0.001953125f : __builtin_ldexpf(1.f + float(m) / 8.f, e - 7);
 }
 
-// The E4M3 code of the scale of a block whose largest magnitude (over the global) is amax, finite: the nearest value
-// to amax / 6, ties to even, at most 448, at least 2^-9 where amax > 0. The quotient is rounded to odd first (its last
-// bit set wherever it is not exact), so that the second rounding is that of the exact quotient.
-__device__ inline uint32_t block_scale_code(float amax) {
-  if (amax >= 2688.f) return 0x7eu;
-  const float y = amax / 6.f;
-  const float r = fmaf(-y, 6.f, amax);
-  uint32_t a = __float_as_uint(y);
-  if (r != 0.f && !(a & 1u)) a = r > 0.f ? a | 1u : a - 1u;
-  if (a < 0x3c800000u) {                       // below 2^-6: whole steps of 2^-9
-    const float t = __uint_as_float(a) * 512.f, lo = floorf(t), frac = t - lo;
-    uint32_t n = uint32_t(lo);
-    n += frac > 0.5f || (frac == 0.5f && (n & 1u)) ? 1u : 0u;
-    return n == 0u && amax > 0.f ? 1u : n;
-  }
-  const uint32_t u = a + 0x7ffffu + ((a >> 20) & 1u);
-  const uint32_t code = (((u >> 23) - 120u) << 3) | ((u >> 20) & 7u);
-  return code > 0x7eu ? 0x7eu : code;
+// The quantisation of a block of 16 whose largest magnitude over the global (a power of two, ginv its inverse) is amax: the scale is the
+// E4M3 value nearest to amax / 6, ties to even, at most 448, at least 2^-9 where amax > 0; a code is the E2M1 value
+// nearest to x / scale. Both quotients are rounded to FP32 first, which the second rounding does not see: a quotient by
+// b 2^q (1 <= b < 2) that is not a midpoint m of the second grid is off it by an ulp of its numerator over b 2^q or more,
+// which is over half an ulp of m, so it never rounds onto m.
+struct BlockScale {
+  uint32_t code;     // E4M3
+  float s, inv;      // its value with the global, and the inverse (0 for a block of zeros)
+};
+
+// x / s for inv = 1 / s: the product is off by an ulp or two, one step makes it the nearest.
+__device__ inline float quotient(float x, float s, float inv) {
+  const float y = x * inv;
+  return fmaf(fmaf(-y, s, x), inv, y);
 }
 
-// The E2M1 code of x in a block of scale s (its global included): the nearest of 0, 0.5, .., 6 times s, ties to the
-// even code, from comparisons with the midpoints, which are exact in FP32.
-__device__ inline uint32_t e2m1_code(float x, float s) {
-  const float a = fabsf(x);
-  uint32_t n = a > 0.25f * s;
-  n += a >= 0.75f * s;
-  n += a > 1.25f * s;
-  n += a >= 1.75f * s;
-  n += a > 2.5f * s;
-  n += a >= 3.5f * s;
-  n += a > 5.f * s;
-  n = s > 0.f ? n : 0u;
-  return n | (x < 0.f ? 8u : 0u);
+__device__ inline BlockScale block_scale(float amax, float global, float ginv) {
+  BlockScale r;
+  const float y = fminf(fmaxf(quotient(amax, 6.f, 1.f / 6.f), amax > 0.f ? 0.001953125f : 0.f), 448.f);
+  r.code = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false)) & 0xffu;
+  const float s = __builtin_amdgcn_cvt_f32_fp8(int(r.code), 0);
+  const float i = __builtin_amdgcn_rcpf(s);
+  r.s = s * global;
+  r.inv = s > 0.f ? fmaf(fmaf(-s, i, 1.f), i, i) * ginv : 0.f;
+  return r;
 }
 
 }  // namespace xtg::hip
