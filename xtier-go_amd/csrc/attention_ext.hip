@@ -22,6 +22,7 @@
 // With the others a q-col whose sum of weights is finite and whose accumulator is not is computed again key by key, by
 // whichever kernel writes it (slow_col).
 #include <algorithm>
+#include <cstdlib>
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -54,6 +55,7 @@ struct ExtArgs {
   int slots_pad, tile_lo, tiles;
   int ring, splits, records, cols, own;   // splits of the cached keys (few) or of all keys; own keys: their number
   int n_q, pos0, heads, group, window, bf16;
+  uint32_t group_inv;            // ceil(2^16 / group): (col * group_inv) >> 16 is col / group for col < 256
   int cached_end;                // cached positions from here on are not seen
   float scale, kglobal, vglobal, softcap;
   const float* slopes;
@@ -81,6 +83,23 @@ __device__ inline bf16x8 row8(const void* p, size_t at, int bf16) {
   const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
   const float4 a = f[0], b = f[1];
   return bf16x8{(__bf16)a.x, (__bf16)a.y, (__bf16)a.z, (__bf16)a.w, (__bf16)b.x, (__bf16)b.y, (__bf16)b.z, (__bf16)b.w};
+}
+
+// N chunks of 8 elements of a row, chunk c at at(c); zeros where it is not live (then row 0 is read). The type is asked
+// once: a branch a chunk would put each load behind the last one's.
+template <int N, class A>
+__device__ inline void row_chunks(const void* p, int bf16, bool live, A at, bf16x8 (&x)[N]) {
+  if (bf16) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) x[c] = *reinterpret_cast<const bf16x8*>(static_cast<const __bf16*>(p) + at(c));
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; ++c) x[c] = row8(p, at(c), 0);
+  }
+  if (!live) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) x[c] = bf16x8{};
+  }
 }
 
 // The q-col's N operand chunks: to f16 times a power of two that brings the largest magnitude over the q-col's lanes
@@ -383,26 +402,26 @@ struct OwnTile {
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const int j = 32 * t + 16 * b + i;
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c)
-        kw[b][c] = j < a.own ? row8(a.k, (size_t(j) * size_t(kv_heads) + size_t(h)) * D + size_t(32 * c + 8 * g), a.bf16)
-                             : bf16x8{};
+      const size_t at = (size_t(j < a.own ? j : 0) * size_t(kv_heads) + size_t(h)) * D + size_t(8 * g);
+      row_chunks(a.k, a.bf16, j < a.own, [&](int c) { return at + size_t(32 * c); }, kw[b]);
     }
   }
   __device__ bf16x8 k(int b, int st) const { return kw[b][st]; }
   __device__ void begin_v() {
     const int g = lane >> 4, i = lane & 15;
+    auto take = [&](auto* p) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int j = 32 * t + (e < 4 ? 4 * g + e : 12 + 4 * g + e);
+      for (int e = 0; e < 8; ++e) {
+        const int j = 32 * t + (e < 4 ? 4 * g + e : 12 + 4 * g + e);
+        const size_t at = (size_t(j < a.own ? j : 0) * size_t(kv_heads) + size_t(h)) * D;
 #pragma unroll
-      for (int dd = 0; dd < D / 16; ++dd) {
-        const size_t at = (size_t(j) * size_t(kv_heads) + size_t(h)) * D + size_t(Tile<D, T>::dim(dd, i));
-        vw[dd][e] = j >= a.own ? (__bf16)0.f
-                    : a.bf16   ? static_cast<const __bf16*>(a.v)[at]
-                               : (__bf16) static_cast<const float*>(a.v)[at];
+        for (int dd = 0; dd < D / 16; ++dd) vw[dd][e] = j < a.own ? (__bf16)p[at + size_t(Tile<D, T>::dim(dd, i))] : (__bf16)0.f;
       }
-    }
+    };
+    if (a.bf16)
+      take(static_cast<const __bf16*>(a.v));
+    else
+      take(static_cast<const float*>(a.v));
   }
   __device__ bf16x8 v(int dd) const { return vw[dd]; }
 };
@@ -483,40 +502,53 @@ __device__ inline void few_tile(const ExtArgs& a, TILE& T, const X8 (&q)[QB][D /
   next_v();
 }
 
-// The q-cols' operand chunks, spans and score factors of a work-group, for operands of T's type and dims.
-template <int D, int QB, class TILE, class X8>
-__device__ inline void few_queries(const ExtArgs& a, int h, int lane, float global, X8 (&q)[QB][D / 32],
-                                   Span (&span)[QB], Score (&sc)[QB]) {
+// The row of a q-col (below 32).
+__device__ inline int few_row(const ExtArgs& a, int col) { return int(uint32_t(col) * a.group_inv >> 16); }
+
+// The q-cols' rows, spans and score factors of a work-group; then their operands of T's type. The rows' loads go out
+// before the first tile's, and are waited for behind them.
+template <int D, int QB, class TILE>
+struct FewQueries {
+  bf16x8 x[QB][D / 32];
+  Span span[QB];
+  Score sc[QB];
+  __device__ void load(const ExtArgs& a, int h, int col0, int lane) {
 #pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    const int col = qb * 16 + (lane & 15), row = col / a.group, head = h * a.group + col % a.group;
-    const bool live = row < a.n_q;
-    bf16x8 x[D / 32];
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-      x[c] = live ? row8(a.q, (size_t(row) * size_t(a.heads) + size_t(head)) * D + size_t(TILE::q_dim(c, lane >> 4)), a.bf16)
-                  : bf16x8{};
-      if (a.scale < 0.f) x[c] = -x[c];
+    for (int qb = 0; qb < QB; ++qb) {
+      const int col = col0 + qb * 16 + (lane & 15), row = few_row(a, col), head = h * a.group + col - row * a.group;
+      const bool live = row < a.n_q;
+      const size_t at = live ? (size_t(row) * size_t(a.heads) + size_t(head)) * D : 0;
+      row_chunks(a.q, a.bf16, live, [&](int c) { return at + size_t(TILE::q_dim(c, lane >> 4)); }, x[qb]);
+      span[qb] = live ? row_span(a, row) : Span{0, 0u, 0};
+      sc[qb] = score_of(a, live ? head : 0, 1.f);
     }
-    const float f = to_operand(x, q[qb], [](float v) { return xor32_max(xor16_max(v)); });
-    span[qb] = live ? row_span(a, row) : Span{0, 0u, 0};
-    sc[qb] = score_of(a, live ? head : 0, f * global);
   }
-}
+  template <class X8>
+  __device__ void operand(const ExtArgs& a, float global, X8 (&q)[QB][D / 32]) {
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+      if (a.scale < 0.f) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) x[qb][c] = -x[qb][c];
+      }
+      sc[qb].f *= global * to_operand(x[qb], q[qb], [](float v) { return xor32_max(xor16_max(v)); });
+    }
+  }
+};
 
 template <int D, int QB>
-constexpr int few_passes() { return QB * D > 128 ? QB * D / 128 : 1; }
-template <int D, int QB>
-constexpr int few_lds_floats() { return kExtWaves * QB * 2 * 16 + kExtWaves * QB * D * 16 / few_passes<D, QB>(); }
+constexpr size_t few_lds() { return size_t(kExtWaves) * QB * (2 * 16 + D * 16) * sizeof(float); }
 
 template <int D, int QB, int T, bool MOD>
-__global__ void __launch_bounds__(kExtWaves * 64) ext_few_kernel(ExtArgs a) {
-  __shared__ float lds[few_lds_floats<D, QB>()];
+__global__ void __launch_bounds__(kExtWaves * 64, QB * D > 256 ? 1 : 2) ext_few_kernel(ExtArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  float* lds = reinterpret_cast<float*>(smem);
   __shared__ uint32_t again;   // q-cols to be computed again
   constexpr int ND = D / 16;
   const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) >> 6, g = lane >> 4, i = lane & 15;
-  const int h = int(blockIdx.x), kv_heads = int(gridDim.x), split = int(blockIdx.y);
-  const bool own = split == a.splits;   // the last work-group of a KV head: the call's own keys
+  const int h = int(blockIdx.x), kv_heads = int(gridDim.x), split = int(gridDim.y) - 1 - int(blockIdx.y);
+  const int col0 = int(blockIdx.z) * QB * 16;   // the work-group's first q-col
+  const bool own = split == a.splits;   // one more work-group, queued first: the call's own keys
   FewState<D, QB> st;
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
@@ -526,14 +558,14 @@ __global__ void __launch_bounds__(kExtWaves * 64) ext_few_kernel(ExtArgs a) {
   }
   if (own) {
     bf16x8 q[QB][D / 32];
-    Span span[QB];
-    Score sc[QB];
-    few_queries<D, QB, OwnTile<D, T>>(a, h, lane, 1.f, q, span, sc);
+    FewQueries<D, QB, OwnTile<D, T>> rows;
+    rows.load(a, h, col0, lane);
+    rows.operand(a, 1.f, q);
     for (int t = wave; 32 * t < a.own; t += kExtWaves) {
       OwnTile<D, T> tile(a, h, kv_heads, t, lane);
       const int p = a.pos0 + 32 * t + 4 * g, past = a.pos0 + a.own;
       auto at = [&](int e) { return p + e < past ? p + e : -1; };
-      few_tile<D, QB, MOD>(a, tile, q, span, sc, st, make_int4(at(0), at(1), at(2), at(3)),
+      few_tile<D, QB, MOD>(a, tile, q, rows.span, rows.sc, st, make_int4(at(0), at(1), at(2), at(3)),
                            make_int4(at(16), at(17), at(18), at(19)), [] {}, [] {});
     }
   } else {
@@ -541,23 +573,23 @@ __global__ void __launch_bounds__(kExtWaves * 64) ext_few_kernel(ExtArgs a) {
     const int t_begin = a.tile_lo + int((long long)a.tiles * split / a.splits);
     const int t_end = a.tile_lo + int((long long)a.tiles * (split + 1) / a.splits);
     X8 q[QB][D / 32];
-    Span span[QB];
-    Score sc[QB];
-    few_queries<D, QB, Tile<D, T>>(a, h, lane, T == kNvfp4 ? a.kglobal : 1.f, q, span, sc);
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb) span[qb] = cached_span(a, span[qb]);
+    FewQueries<D, QB, Tile<D, T>> rows;
+    rows.load(a, h, col0, lane);
     Tile<D, T> tile;
     int t = t_begin + wave;
+    const int4* sp = reinterpret_cast<const int4*>(a.slot_pos) + g;
     if (t < t_end) {
-      const int4* sp = reinterpret_cast<const int4*>(a.slot_pos) + g;
       tile.load_k(a, h, t, lane);
       int4 p0 = sp[t * 8], p1 = sp[t * 8 + 4];
       tile.load_v(a, h, t, lane);
+      rows.operand(a, T == kNvfp4 ? a.kglobal : 1.f, q);
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) rows.span[qb] = cached_span(a, rows.span[qb]);
       for (; t < t_end; t += kExtWaves) {
         const int n = min(t + kExtWaves, t_end - 1);   // past the end: loaded again, and not used
         const int4 c0 = p0, c1 = p1;
         few_tile<D, QB, MOD>(
-            a, tile, q, span, sc, st, c0, c1,
+            a, tile, q, rows.span, rows.sc, st, c0, c1,
             [&] {
               tile.load_k(a, h, n, lane);
               p0 = sp[n * 8], p1 = sp[n * 8 + 4];
@@ -575,9 +607,9 @@ __global__ void __launch_bounds__(kExtWaves * 64) ext_few_kernel(ExtArgs a) {
 
   if (threadIdx.x == 0) again = 0;
 
-  // the waves' states joined: the maxima and sums, then the accumulators in passes of what fits, each wave a part
+  // the waves' states joined: the maxima and sums, then the accumulators, each wave a part of the sums
   float* ml = lds;                                   // [wave][QB * 16][2]
-  float* part = lds + kExtWaves * QB * 2 * 16;       // [wave][QB][products of a pass][64 lanes][4]
+  float* part = lds + kExtWaves * QB * 2 * 16;       // [wave][QB][products][64 lanes][4]
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     const float l = xor32_sum(xor16_sum(st.l[qb]));
@@ -603,53 +635,48 @@ __global__ void __launch_bounds__(kExtWaves * 64) ext_few_kernel(ExtArgs a) {
 #pragma unroll
     for (int dd = 0; dd < ND; ++dd) st.acc[qb][dd] *= corr;
   }
-  constexpr int NP = few_passes<D, QB>(), PD = ND / NP;   // products of a pass
-  static_assert(PD % kExtWaves == 0 || kExtWaves % PD == 0, "a pass's products over the waves");
-  const size_t rec = (size_t(h) * size_t(a.records) + size_t(split)) * size_t(a.cols);
+  const size_t rec = ((size_t(blockIdx.z) * size_t(kv_heads) + size_t(h)) * size_t(a.records) + size_t(split)) * size_t(a.cols);
 #pragma unroll
-  for (int pass = 0; pass < NP; ++pass) {
-    if (pass) __syncthreads();
+  for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb)
+    for (int dd = 0; dd < ND; ++dd)
+      *reinterpret_cast<f32x4*>(part + (((wave * QB + qb) * ND + dd) * 64 + lane) * 4) = st.acc[qb][dd];
+  __syncthreads();
+  {
 #pragma unroll
-      for (int d = 0; d < PD; ++d)
-        *reinterpret_cast<f32x4*>(part + (((wave * QB + qb) * PD + d) * 64 + lane) * 4) = st.acc[qb][pass * PD + d];
-    __syncthreads();
-#pragma unroll
-    for (int x = 0; x < QB * PD; x += kExtWaves) {
-      const int qd = x + wave, qb = qd / PD, dd = pass * PD + qd % PD;
-      if (qd >= QB * PD) continue;
+    for (int x = 0; x < QB * ND; x += kExtWaves) {
+      const int qd = x + wave, qb = qd / ND, dd = qd % ND;
       f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < kExtWaves; ++w) y += *reinterpret_cast<const f32x4*>(part + ((w * QB * PD + qd) * 64 + lane) * 4);
-      const int col = qb * 16 + i, row = col / a.group;
+      for (int w = 0; w < kExtWaves; ++w) y += *reinterpret_cast<const f32x4*>(part + ((w * QB * ND + qd) * 64 + lane) * 4);
+      const int mine = qb * 16 + i, col = col0 + mine, row = few_row(a, col);
       if (row >= a.n_q) continue;
       float l = l_all[0];
       if constexpr (QB == 2) l = qb ? l_all[1] : l;
       if (a.records == 1) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (!not_finite(l) && not_finite(y[r])) atomicOr(&again, 1u << col);
+          if (!not_finite(l) && not_finite(y[r])) atomicOr(&again, 1u << mine);
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int dim = Tile<D, T>::dim(dd, 4 * g + r);
-          const size_t at = (size_t(row) * size_t(a.heads) + size_t(h * a.group + col % a.group)) * D + size_t(dim);
+          const size_t at = (size_t(row) * size_t(a.heads) + size_t(h * a.group + col - row * a.group)) * D + size_t(dim);
           if (a.bf16)
             static_cast<__bf16*>(a.out)[at] = (__bf16)(y[r] * inv);
           else
             static_cast<float*>(a.out)[at] = y[r] * inv;
         }
       } else {
-        *reinterpret_cast<f32x4*>(a.acc + (rec + size_t(col)) * D + size_t(16 * dd + 4 * g)) = y;
+        *reinterpret_cast<f32x4*>(a.acc + (rec + size_t(mine)) * D + size_t(16 * dd + 4 * g)) = y;
       }
     }
   }
   if (a.records == 1) {
     __syncthreads();
     for (uint32_t bits = again; bits; bits &= bits - 1) {
-      const int col = __builtin_ctz(bits);
-      slow_col<D, T>(a, h, kv_heads, col / a.group, h * a.group + col % a.group, lds);
+      const int col = col0 + __builtin_ctz(bits), row = few_row(a, col);
+      slow_col<D, T>(a, h, kv_heads, row, h * a.group + col - row * a.group, lds);
     }
     return;
   }
@@ -897,10 +924,10 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a) 
     if (f >= e) return;
     X8 q[R::NS];
     bf16x8 x[R::NS];
+    row_chunks(a.q, a.bf16, live, [&](int c) { return (live ? q_at : size_t(8 * half)) + size_t(16 * c); }, x);
+    if (a.scale < 0.f) {
 #pragma unroll
-    for (int c = 0; c < R::NS; ++c) {
-      x[c] = live ? row8(a.q, q_at + size_t(16 * c), a.bf16) : bf16x8{};
-      if (a.scale < 0.f) x[c] = -x[c];
+      for (int c = 0; c < R::NS; ++c) x[c] = -x[c];
     }
     const float factor = to_operand(x, q, [](float y) { return xor32_max(y); });
     const Score sc = score_of(a, live ? head : 0, factor * global);
@@ -1102,52 +1129,73 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a) 
 
 // ---------------------------------------------------------------------------------------------------- merge
 
-// A q-col's records in G groups of lanes, each the records s = group, group + G, .. in order, then the groups in order:
-// D / 4 lanes hold a record's accumulator, 4 rows each.
+// A q-col's records: their weights 2^(m - largest m) first, then the sums, D / 4 lanes to a record's accumulator and G
+// groups of lanes with the records s = group, group + G, .., whose sums are added in order. A batch of accumulators is
+// loaded before the weights are known: few q-cols' records are a matter of latency.
 template <int D, int T, int G>
 __global__ void __launch_bounds__(256) ext_merge_kernel(ExtArgs a, int kv_heads, int total) {
-  constexpr int L = D / 4, PER = 256 / (L * G);   // lanes a record; q-cols of a work-group
+  constexpr int L = D / 4, PER = 256 / (L * G), B = 8;   // lanes a record; q-cols of a work-group; records of a batch
   __shared__ float4 part[G > 1 ? PER * G * L : 1];
-  __shared__ float pm[G > 1 ? PER * G * 2 : 1], slow[264 + D];
+  __shared__ float slow[264 + D], all_m[4], all_l[4];
   __shared__ int again[PER];
   const int tid = int(threadIdx.x), x = tid % L, grp = tid / L % G, mine = tid / (L * G);
   const int id = int(blockIdx.x) * PER + mine;   // q-col of the call: row * heads + head
-  const int row = id / a.heads, head = id % a.heads, h = head / a.group, c = row * a.group + head % a.group;
   const bool live = id < total;
+  const int row = live ? id / a.heads : 0, head = live ? id % a.heads : 0, h = head / a.group, c = row * a.group + head % a.group;
   if (x == 0 && grp == 0) again[mine] = 0;
+  // record s's accumulator, maximum and sum
+  const size_t rec0 = (size_t(c / a.cols) * size_t(kv_heads) + size_t(h)) * size_t(a.records) * size_t(a.cols) + size_t(c % a.cols);
+  const float* acc = a.acc + rec0 * D + size_t(4 * x);
+  const float2* ml = reinterpret_cast<const float2*>(a.ml) + rec0;
+  float4 v[B];
+  float2 w[B];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int k = 0; k < B; ++k) {
+      const int s = s0 + k * G;
+      w[k] = s < a.records ? ml[size_t(s) * size_t(a.cols)] : make_float2(-INFINITY, 0.f);
+      v[k] = s < a.records ? *reinterpret_cast<const float4*>(acc + size_t(s) * size_t(a.cols) * D) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  };
+  load(grp);
+  // the largest maximum and the sum at it: a thread a record where a work-group has one q-col, else every thread all
   float m = -INFINITY, l = 0.f;
+  if constexpr (G > 1) {
+    for (int s = tid; s < a.records; s += 256) m = fmaxf(m, ml[size_t(s) * size_t(a.cols)].x);
+    m = wave_max(m);
+    if ((tid & 63) == 0) all_m[tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(all_m[0], all_m[1]), fmaxf(all_m[2], all_m[3]));
+  } else {
+#pragma unroll
+    for (int k = 0; k < B; ++k) m = fmaxf(m, w[k].x);   // (G = 1: all of them, at most B)
+  }
+  const float ref = m == -INFINITY ? 0.f : m;
   float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (live) {
-    const size_t rec0 = (size_t(c / a.cols) * size_t(kv_heads) + size_t(h)) * size_t(a.records);
-    for (int s = grp; s < a.records; s += G) {
-      const size_t rec = (rec0 + size_t(s)) * size_t(a.cols) + size_t(c % a.cols);
-      const float rm = a.ml[rec * 2], rl = a.ml[rec * 2 + 1];
-      const float4 v = *reinterpret_cast<const float4*>(a.acc + rec * D + size_t(4 * x));
-      const float to = fmaxf(m, rm), ref = to == -INFINITY ? 0.f : to;
-      const float c0 = __builtin_amdgcn_exp2f(m - ref), c1 = __builtin_amdgcn_exp2f(rm - ref);
-      m = to;
-      l = l * c0 + rl * c1;
-      if (c1 != 0.f) {   // (a record whose maximum is far below, or that saw nothing, adds nothing)
-        y.x = y.x * c0 + v.x * c1, y.y = y.y * c0 + v.y * c1, y.z = y.z * c0 + v.z * c1, y.w = y.w * c0 + v.w * c1;
-      }
+  for (int s0 = grp; s0 < a.records; s0 += B * G) {
+    if (s0 != grp) load(s0);
+#pragma unroll
+    for (int k = 0; k < B; ++k) {
+      const float f = __builtin_amdgcn_exp2f(w[k].x - ref);
+      l += w[k].y * f;
+      if (f != 0.f)   // (a record whose maximum is far below, or that saw nothing, adds nothing)
+        y.x += v[k].x * f, y.y += v[k].y * f, y.z += v[k].z * f, y.w += v[k].w * f;
     }
   }
   if constexpr (G > 1) {
     part[tid] = y;
-    if (x == 0) pm[(mine * G + grp) * 2] = m, pm[(mine * G + grp) * 2 + 1] = l;
+    l = x == 0 ? l : 0.f;   // a group's sum once; the groups' over the work-group
+    l = wave_sum(l);
+    if ((tid & 63) == 0) all_l[tid >> 6] = l;
     __syncthreads();
-    float to = -INFINITY;
-#pragma unroll
-    for (int s = 0; s < G; ++s) to = fmaxf(to, pm[(mine * G + s) * 2]);
-    const float ref = to == -INFINITY ? 0.f : to;
-    l = 0.f;
+    l = all_l[0] + all_l[1] + all_l[2] + all_l[3];
     y = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (grp == 0) {
 #pragma unroll
-    for (int s = 0; s < G; ++s) {
-      const float c1 = __builtin_amdgcn_exp2f(pm[(mine * G + s) * 2] - ref);
-      const float4 v = part[(mine * G + s) * L + x];
-      l += pm[(mine * G + s) * 2 + 1] * c1;
-      if (c1 != 0.f) y.x += v.x * c1, y.y += v.y * c1, y.z += v.z * c1, y.w += v.w * c1;
+      for (int s = 0; s < G; ++s) {
+        const float4 u = part[s * L + x];
+        y.x += u.x, y.y += u.y, y.z += u.z, y.w += u.w;
+      }
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -1156,8 +1204,8 @@ __global__ void __launch_bounds__(256) ext_merge_kernel(ExtArgs a, int kv_heads,
   if (live && grp == 0) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int v = 4 * x + r;
-      const size_t at = size_t(id) * D + size_t(Tile<D, T>::dim(v >> 4, v & 15));
+      const int u = 4 * x + r;
+      const size_t at = size_t(id) * D + size_t(Tile<D, T>::dim(u >> 4, u & 15));
       if (a.bf16)
         static_cast<__bf16*>(a.out)[at] = (__bf16)o[r];
       else
@@ -1167,10 +1215,10 @@ __global__ void __launch_bounds__(256) ext_merge_kernel(ExtArgs a, int kv_heads,
   if (!__syncthreads_or(bad && live)) return;
   if (bad && live) again[mine] = 1;
   __syncthreads();
-  for (int w = 0; w < PER; ++w)
-    if (again[w]) {
-      const int c = int(blockIdx.x) * PER + w;
-      slow_col<D, T>(a, c % a.heads / a.group, kv_heads, c / a.heads, c % a.heads, slow);
+  for (int k = 0; k < PER; ++k)
+    if (again[k]) {
+      const int q = int(blockIdx.x) * PER + k;
+      slow_col<D, T>(a, q % a.heads / a.group, kv_heads, q / a.heads, q % a.heads, slow);
     }
 }
 
@@ -1190,14 +1238,15 @@ ExtPlan ext_plan(const ExtCall& a, int cus) {
   }
   p.few = cols <= 32;
   if (p.few) {
-    p.cols = int((cols + 15) / 16 * 16);
     p.tile_lo = int(lo / 32);
     p.tiles = slots > lo ? int((slots + 31) / 32) - p.tile_lo : 0;
-    // two work-groups a CU, at least a tile for each wave
-    p.splits = std::min(std::max(1, 2 * cus / a.kv_heads), (p.tiles + kExtWaves - 1) / kExtWaves);
+    // a work-group a CU, at least a tile for each wave; where that leaves CUs idle, the second 16 q-cols apart
+    p.splits = std::min(std::max(1, cus / a.kv_heads), (p.tiles + kExtWaves - 1) / kExtWaves);
+    p.cols = cols > 16 && 2 * p.splits * a.kv_heads > cus ? 32 : 16;
+    p.blocks = int((cols + p.cols - 1) / p.cols);
     if (!a.k) p.splits = std::max(p.splits, 1);
     const size_t records = size_t(p.splits) + (a.k ? 1 : 0);
-    if (records > 1) p.record_bytes = records * size_t(a.kv_heads) * size_t(p.cols) * size_t(a.d + 2) * sizeof(float);
+    if (records > 1) p.record_bytes = records * size_t(a.kv_heads) * size_t(p.blocks * p.cols) * size_t(a.d + 2) * sizeof(float);
     return p;
   }
   p.blocks = int((cols + 127) / 128);
@@ -1219,11 +1268,15 @@ void launch(const ExtCall& c, const ExtPlan& p, const ExtArgs& a, hipStream_t st
   const char* mod = MOD ? "true" : "false";
   if (p.few) {
     timed([&] {
-      const dim3 grid{unsigned(c.kv_heads), unsigned(a.records)}, block{kExtWaves * 64};
+      const dim3 grid{unsigned(c.kv_heads), unsigned(a.records), unsigned(p.blocks)}, block{kExtWaves * 64};
+      auto go = [&](auto kernel, size_t lds) {
+        allow_lds(reinterpret_cast<const void*>(kernel), lds);
+        hipLaunchKernelGGL(kernel, grid, block, lds, stream, a);
+      };
       if (p.cols == 16)
-        hipLaunchKernelGGL((ext_few_kernel<D, 1, T, MOD>), grid, block, 0, stream, a);
+        go(&ext_few_kernel<D, 1, T, MOD>, few_lds<D, 1>());
       else
-        hipLaunchKernelGGL((ext_few_kernel<D, 2, T, MOD>), grid, block, 0, stream, a);
+        go(&ext_few_kernel<D, 2, T, MOD>, few_lds<D, 2>());
       HIP_CHECK(hipGetLastError());
       return strf("ext_few_kernel<%d, %d, %d, %s>", D, p.cols / 16, T, mod);
     });
@@ -1248,7 +1301,7 @@ void launch(const ExtCall& c, const ExtPlan& p, const ExtArgs& a, hipStream_t st
   }
   if (a.records > 1)
     timed([&] {
-      constexpr int G = 1024 / D;   // 256 threads of D / 4 a record: G records at once, or G q-cols
+      constexpr int G = 1024 / D;   // 256 threads, D / 4 a record: G records at once, or G q-cols of at most 8
       const int total = c.n_q * c.heads, groups = a.records > 8 ? G : 1;
       if (groups > 1)
         hipLaunchKernelGGL((ext_merge_kernel<D, T, G>), dim3(unsigned(total)), dim3(256), 0, stream, a, c.kv_heads, total);
@@ -1284,6 +1337,7 @@ void launch_attn_ext(const ExtCall& c, const ExtPlan& p, void* scratch, hipStrea
   a.own = c.k ? c.n_q : 0;
   a.records = p.few ? p.splits + (c.k ? 1 : 0) : p.splits;
   a.n_q = c.n_q, a.pos0 = int(c.pos0), a.heads = c.heads, a.group = c.heads / c.kv_heads, a.window = c.window;
+  a.group_inv = (65536u + uint32_t(a.group) - 1u) / uint32_t(a.group);
   a.bf16 = c.x_dtype == kXBF16;
   a.cached_end = c.k ? a.pos0 : INT_MAX;
   a.scale = c.scale, a.softcap = c.softcap, a.slopes = c.slopes, a.first = c.first, a.end = c.end;

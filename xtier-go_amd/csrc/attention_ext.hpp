@@ -28,7 +28,7 @@ struct ExtCall {
 
 // How a call is cut up. A q-col is a (row, q head of a KV head); a work-group takes `cols` of them for one KV head and
 // one of `splits` parts of the keys, and leaves a record (accumulator, maximum, sum) for each where there are more
-// than one. few: at most 32 q-cols, one block of them, whose work-groups' waves take cache tiles of their own; the last
+// than one. few: at most 32 q-cols, in one block or two, whose work-groups' waves take cache tiles of their own; the last
 // record is the call's own keys'. Otherwise blocks of 128 q-cols share tiles, the call's own keys packed as tiles too.
 struct ExtPlan {
   bool few = false;
