@@ -188,11 +188,15 @@ __device__ inline Score score_of(const ExtArgs& a, int head, float factor) {
   s.slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
   return s;
 }
+// What a call does to its scores, a bit each; kernels are made for each of the four.
+constexpr int kCap = 1, kBias = 2;
 // cap * tanh(x / cap) = cap * (1 - 2 / (e^(2 x / cap) + 1)), minus the bias.
-__device__ inline float changed(const ExtArgs& a, const Score& s, float qk, int dist) {
+template <int MOD>
+__device__ inline float changed(const Score& s, float qk, int dist) {
   float y = qk * s.f;
-  if (a.softcap > 0.f) y = s.top - 2.f * s.top * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y) + 1.f);
-  return y - s.slope * fabsf(float(dist));
+  if (MOD & kCap) y = fmaf(-2.f * s.top, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y) + 1.f), s.top);
+  if (MOD & kBias) y = fmaf(-s.slope, fabsf(float(dist)), y);
+  return y;
 }
 
 __device__ inline bool not_finite(float x) { return !(fabsf(x) <= FLT_MAX); }
@@ -222,11 +226,11 @@ __device__ inline float row_value(const void* p, size_t at, int bf16) {
   return bf16 ? (float)static_cast<const __bf16*>(p)[at] : (float)(__bf16) static_cast<const float*>(p)[at];
 }
 
-// One q-col by a work-group of 256 threads: 256 keys at a time, a score each thread, then a dim each thread; values of
-// keys that the row does not see are not read. lds: 264 + D floats.
-template <int D, int T>
+// One q-col by a work-group of NT threads: NT keys at a time, a score each thread, then a dim each thread; values of
+// keys that the row does not see are not read. lds: NT + 16 + D floats.
+template <int D, int T, int NT = 256>
 __device__ inline void slow_col(const ExtArgs& a, int h, int kv_heads, int row, int head, float* lds) {
-  float *q = lds, *w = lds + D, *red = lds + D + 256;
+  float *q = lds, *w = lds + D, *red = lds + D + NT;
   const int tid = int(threadIdx.x);
   const Span all = row_span(a, row), cached = cached_span(a, all);
   const Score sc = score_of(a, head, 1.f);
@@ -235,7 +239,7 @@ __device__ inline void slow_col(const ExtArgs& a, int h, int kv_heads, int row, 
   if (tid < D) q[tid] = row_value(a.q, at, a.bf16);
   __syncthreads();
   float m = -INFINITY, l = 0.f, acc = 0.f;
-  for (int k0 = 0; k0 < a.slots_pad + a.own; k0 += 256) {
+  for (int k0 = 0; k0 < a.slots_pad + a.own; k0 += NT) {
     const int key = k0 + tid, j = key - a.slots_pad;   // own key j
     int pos = -1;
     if (j < 0)
@@ -249,9 +253,10 @@ __device__ inline void slow_col(const ExtArgs& a, int h, int kv_heads, int row, 
       for (int x = 0; x < D; ++x)
         s += q[x] * (j < 0 ? cached_value<D, T>(a, false, h, key, x)
                            : row_value(a.k, (size_t(j) * size_t(kv_heads) + size_t(h)) * D + size_t(x), a.bf16));
-      s = changed(a, sc, a.scale < 0.f ? -s : s, all.t - pos);
+      if (a.scale < 0.f) s = -s;
+      s = a.softcap > 0.f ? changed<kCap | kBias>(sc, s, all.t - pos) : changed<kBias>(sc, s, all.t - pos);
     }
-    const float m_new = fmaxf(m, block_max<256>(s, red)), ref = m_new == -INFINITY ? 0.f : m_new;
+    const float m_new = fmaxf(m, block_max<NT>(s, red)), ref = m_new == -INFINITY ? 0.f : m_new;
     const float p = __builtin_amdgcn_exp2f(s - ref), corr = __builtin_amdgcn_exp2f(m - ref);
     w[tid] = seen ? p : -1.f;   // -1: not seen
     l = l * corr + block_sum<256>(p, red);
@@ -436,7 +441,7 @@ struct FewState {
 
 // One tile. next_k loads the next tile's keys once this one's are used, next_v its values: each load has about half a
 // tile's work to land behind.
-template <int D, int QB, bool MOD, class TILE, class X8, class NK, class NV>
+template <int D, int QB, int MOD, class TILE, class X8, class NK, class NV>
 __device__ inline void few_tile(const ExtArgs& a, TILE& T, const X8 (&q)[QB][D / 32], const Span (&span)[QB],
                                 const Score (&sc)[QB], FewState<D, QB>& st, int4 p0, int4 p1, NK&& next_k, NV&& next_v) {
   const int pos[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
@@ -470,7 +475,7 @@ __device__ inline void few_tile(const ExtArgs& a, TILE& T, const X8 (&q)[QB][D /
     for (int e = 0; e < 8; ++e) {
       float x = s[qb][e >> 2][e & 3];
       if constexpr (TILE::kScaled) x *= ks[e];
-      x = MOD ? changed(a, sc[qb], x, span[qb].t - pos[e]) : x * sc[qb].f;
+      x = changed<MOD>(sc[qb], x, span[qb].t - pos[e]);
       y[e] = uint32_t(pos[e] - span[qb].lo) < span[qb].len ? x : -INFINITY;
       mx = fmaxf(mx, y[e]);
     }
@@ -539,7 +544,7 @@ struct FewQueries {
 template <int D, int QB>
 constexpr size_t few_lds() { return size_t(kExtWaves) * QB * (2 * 16 + D * 16) * sizeof(float); }
 
-template <int D, int QB, int T, bool MOD>
+template <int D, int QB, int T, int MOD>
 __global__ void __launch_bounds__(kExtWaves * 64, QB * D > 256 ? 1 : 2) ext_few_kernel(ExtArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   float* lds = reinterpret_cast<float*>(smem);
@@ -732,13 +737,16 @@ __global__ void __launch_bounds__(256) ext_pack_kernel(const void* __restrict__ 
 // [64 lanes] entries of 8 keys: A operands of v_mfma_f32_32x32x16. Lane (half, i) of a K entry has key i and dims
 // 8 half .. +8 of the step, of a V entry row i and keys 8 a + 4 half + e, 16 + 8 a + 4 half + e (e = 0 .. 3) of step
 // a = 0, 1 of a 32-key block: what the lane's scores are of. A cache's entries are these too, in another order.
+// Two K and two V buffers; positions and FP8 scales of four tiles, with the first and last position.
 template <int D>
 struct Rows {
-  static constexpr int TK = D == 256 ? 32 : 64;         // two tiles' buffers leave room for two work-groups on a CU
+  static constexpr int TK = D == 256 ? 32 : 64;
   static constexpr int KB = TK / 32, NS = D / 16, NB = D / 32, KS = TK / 16;
   static constexpr int kEntries = TK * D / 8;           // of K, and of V
   static constexpr int PER = kEntries / 256;            // entries a thread stages
-  static constexpr size_t kBuffer = size_t(kEntries) * 32 + size_t(TK) * 12;   // K, V, positions, scales
+  static constexpr bool kAhead = D < 256;
+  static constexpr int kInfo = 3 * TK + 4;              // ints of a tile's positions, scales and extremes
+  static constexpr size_t kLds = size_t(kEntries) * 64 + size_t(kInfo) * 16;
 };
 
 // What a thread stages of a tile: loads in flight (raw), then entries written to LDS. A cache of an odd number of 32-slot
@@ -751,13 +759,13 @@ template <int D>
 struct Stage<D, kBf16> {
   using R = Rows<D>;
   uint4 k[R::PER], v[R::PER];
-  __device__ void load(const uint4* ck, const uint4* cv, int h, int pad, int tile, bool half) {
+  __device__ static void load(uint4 (&x)[R::PER], const uint4* c, int h, int pad, int tile, bool half) {
     const size_t at = (size_t(h) * size_t(pad) + size_t(tile) * R::TK) * (D / 8) + threadIdx.x;
 #pragma unroll
-    for (int u = 0; u < R::PER; ++u) k[u] = half && 2 * u >= R::PER ? make_uint4(0, 0, 0, 0) : ck[at + u * 256];
-#pragma unroll
-    for (int u = 0; u < R::PER; ++u) v[u] = half && 2 * u >= R::PER ? make_uint4(0, 0, 0, 0) : cv[at + u * 256];
+    for (int u = 0; u < R::PER; ++u) x[u] = half && 2 * u >= R::PER ? make_uint4(0, 0, 0, 0) : c[at + u * 256];
   }
+  __device__ void load_k(const uint4* ck, int h, int pad, int tile, bool half) { load(k, ck, h, pad, tile, half); }
+  __device__ void load_v(const uint4* cv, int h, int pad, int tile, bool half) { load(v, cv, h, pad, tile, half); }
   // entry x of a BF16 tile of TK keys to its place
   __device__ static int k_place(int x) {
     const int b = x / (2 * D), c = x / 64 % (D / 32), g = x >> 4 & 3, i = x & 15;
@@ -767,9 +775,11 @@ struct Stage<D, kBf16> {
     const int t = x / (4 * D), dd = x / 64 % (D / 16), g = x >> 4 & 3, i = x & 15;
     return ((dd >> 1) * R::KS + 2 * t + (g >> 1)) * 64 + (g & 1) * 32 + (dd & 1) * 16 + i;
   }
-  __device__ void store(uint4* lk, uint4* lv) const {
+  __device__ void store_k(uint4* lk) const {
 #pragma unroll
     for (int u = 0; u < R::PER; ++u) lk[k_place(int(threadIdx.x) + u * 256)] = k[u];
+  }
+  __device__ void store_v(uint4* lv) const {
 #pragma unroll
     for (int u = 0; u < R::PER; ++u) lv[v_place(int(threadIdx.x) + u * 256)] = v[u];
   }
@@ -781,23 +791,32 @@ struct Stage<D, kFp8> {
   using R = Rows<D>;
   using B = Stage<D, kBf16>;
   uint4 k[R::PER / 2], v[R::PER / 2];
-  __device__ void load(const uint4* ck, const uint4* cv, int h, int pad, int tile, bool half) {
+  __device__ static void load(uint4 (&x)[R::PER / 2], const uint4* c, int h, int pad, int tile, bool half) {
     const size_t at = (size_t(h) * size_t(pad) + size_t(tile) * R::TK) * (D / 16) + threadIdx.x;
 #pragma unroll
     for (int u = 0; u < R::PER / 2; ++u) {
       const bool past = half && int(threadIdx.x) + u * 256 >= R::kEntries / 4;
-      k[u] = past ? make_uint4(0, 0, 0, 0) : ck[at + u * 256];
-      v[u] = past ? make_uint4(0, 0, 0, 0) : cv[at + u * 256];
+      x[u] = past ? make_uint4(0, 0, 0, 0) : c[at + u * 256];
     }
   }
-  __device__ void store(uint4* lk, uint4* lv) const {
+  __device__ void load_k(const uint4* ck, int h, int pad, int tile, bool half) { load(k, ck, h, pad, tile, half); }
+  __device__ void load_v(const uint4* cv, int h, int pad, int tile, bool half) { load(v, cv, h, pad, tile, half); }
+  __device__ static int first(int u) {   // of BF16's entries
+    const int x = int(threadIdx.x) + u * 256;
+    return (x >> 6) * 128 + (x & 63);
+  }
+  __device__ void store_k(uint4* lk) const {
 #pragma unroll
     for (int u = 0; u < R::PER / 2; ++u) {
-      const int x = int(threadIdx.x) + u * 256, lane = x & 63, x0 = (x >> 6) * 128 + lane;   // of BF16's entries
-      lk[B::k_place(x0)] = __builtin_bit_cast(uint4, fp8_operand(k[u].x, k[u].y));
-      lk[B::k_place(x0 + 64)] = __builtin_bit_cast(uint4, fp8_operand(k[u].z, k[u].w));
-      lv[B::v_place(x0)] = __builtin_bit_cast(uint4, fp8_operand(v[u].x, v[u].y));
-      lv[B::v_place(x0 + 64)] = __builtin_bit_cast(uint4, fp8_operand(v[u].z, v[u].w));
+      lk[B::k_place(first(u))] = __builtin_bit_cast(uint4, fp8_operand(k[u].x, k[u].y));
+      lk[B::k_place(first(u) + 64)] = __builtin_bit_cast(uint4, fp8_operand(k[u].z, k[u].w));
+    }
+  }
+  __device__ void store_v(uint4* lv) const {
+#pragma unroll
+    for (int u = 0; u < R::PER / 2; ++u) {
+      lv[B::v_place(first(u))] = __builtin_bit_cast(uint4, fp8_operand(v[u].x, v[u].y));
+      lv[B::v_place(first(u) + 64)] = __builtin_bit_cast(uint4, fp8_operand(v[u].z, v[u].w));
     }
   }
 };
@@ -808,22 +827,26 @@ struct Stage<D, kNvfp4> {
   using R = Rows<D>;
   uint32_t k[R::PER], v[R::PER], ks;
   uint2 vs;
-  __device__ void load(const ExtArgs& a, int h, int tile, bool half) {
+  __device__ void load_k(const ExtArgs& a, int h, int tile, bool half) {
     const size_t at = size_t(h) * size_t(a.slots_pad) + size_t(tile) * R::TK;
-    const int tid = int(threadIdx.x), lane = tid & 63;
-    if (half && tid >= 128) {
+    const int tid = int(threadIdx.x);
 #pragma unroll
-      for (int u = 0; u < R::PER; ++u) k[u] = v[u] = 0;
-      ks = 0, vs = make_uint2(0, 0);
-      return;
-    }
+    for (int u = 0; u < R::PER; ++u) k[u] = 0;
+    ks = 0;
+    if (half && tid >= 128) return;
     take(k, a.ck + at * (D / 2), tid);
     const uint8_t* s = static_cast<const uint8_t*>(a.ks) + at * (D / 16);
     ks = D == 64 ? s[tid] : reinterpret_cast<const uint16_t*>(s)[tid];
-    // V: a wave has half a 32-slot tile's words (256 dims: a quarter)
-    const int part = tid >> 6;
+  }
+  // V: a wave has half a 32-slot tile's words (256 dims: a quarter)
+  __device__ void load_v(const ExtArgs& a, int h, int tile, bool half) {
+    const size_t at = size_t(h) * size_t(a.slots_pad) + size_t(tile) * R::TK;
+    const int tid = int(threadIdx.x), lane = tid & 63, part = tid >> 6, t = D == 256 ? 0 : part >> 1;
+#pragma unroll
+    for (int u = 0; u < R::PER; ++u) v[u] = 0;
+    vs = make_uint2(0, 0);
+    if (half && tid >= 128) return;
     take_v(a.cv + at * (D / 2), part, lane);
-    const int t = D == 256 ? 0 : part >> 1;
     const uint2* sv = reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.vs) + at * (D / 16));
     vs = sv[t * (D / 4) + (lane >> 4) * (D / 16) + (lane & 15) * (D / 16) / 16];
   }
@@ -846,9 +869,9 @@ struct Stage<D, kNvfp4> {
       v[0] = x.x, v[1] = x.y;
     }
   }
-  __device__ void store(uint4* lk, uint4* lv) const {
+  __device__ void store_k(uint4* lk) const {
     const int tid = int(threadIdx.x), lane = tid & 63, part = tid >> 6, g = lane >> 4, i = lane & 15;
-    // K: D = 64, 128: 16-slot block `part`; 256: block part / 2, chunk part % 2
+    // D = 64, 128: 16-slot block `part`; 256: block part / 2, chunk part % 2
     const int b = D == 256 ? part >> 1 : part, chunk = D == 256 ? part & 1 : 0;
 #pragma unroll
     for (int c = 0; c < R::PER; ++c) {
@@ -856,6 +879,9 @@ struct Stage<D, kNvfp4> {
       lk[((b >> 1) * R::NS + (dim8 >> 1)) * 64 + (dim8 & 1) * 32 + (b & 1) * 16 + i] =
           __builtin_bit_cast(uint4, dequant8(k[c], scale_pair(ks, c >> 1)));
     }
+  }
+  __device__ void store_v(uint4* lv) const {
+    const int tid = int(threadIdx.x), lane = tid & 63, part = tid >> 6, g = lane >> 4, i = lane & 15;
     f16x2 s[4];
     v_scales(vs, s);
     const int t = D == 256 ? 0 : part >> 1, dd0 = (D == 256 ? part : part & 1) * R::PER;
@@ -868,7 +894,56 @@ struct Stage<D, kNvfp4> {
   }
 };
 
-template <int D, int T, bool MOD>
+// The largest and smallest of a wave's values (every lane gets them).
+__device__ inline void wave_extremes(int& top, int& least) {
+  auto step = [&](int a, int b) { top = max(top, a), least = min(least, b); };
+  step(__builtin_amdgcn_update_dpp(0, top, kDppXor1, 0xF, 0xF, false), __builtin_amdgcn_update_dpp(0, least, kDppXor1, 0xF, 0xF, false));
+  step(__builtin_amdgcn_update_dpp(0, top, kDppXor2, 0xF, 0xF, false), __builtin_amdgcn_update_dpp(0, least, kDppXor2, 0xF, 0xF, false));
+  step(__builtin_amdgcn_update_dpp(0, top, kDppHalfMirror, 0xF, 0xF, false), __builtin_amdgcn_update_dpp(0, least, kDppHalfMirror, 0xF, 0xF, false));
+  step(__builtin_amdgcn_update_dpp(0, top, kDppMirror, 0xF, 0xF, false), __builtin_amdgcn_update_dpp(0, least, kDppMirror, 0xF, 0xF, false));
+  auto a = __builtin_amdgcn_permlane16_swap(uint32_t(top), uint32_t(top), false, false);
+  auto b = __builtin_amdgcn_permlane16_swap(uint32_t(least), uint32_t(least), false, false);
+  top = max(int(a[0]), int(a[1])), least = min(int(b[0]), int(b[1]));
+  a = __builtin_amdgcn_permlane32_swap(uint32_t(top), uint32_t(top), false, false);
+  b = __builtin_amdgcn_permlane32_swap(uint32_t(least), uint32_t(least), false, false);
+  top = max(int(a[0]), int(a[1])), least = min(int(b[0]), int(b[1]));
+}
+
+// The tiles of TK keys that a work-group goes over (its split's part): of the cache (a linear one's slots are positions),
+// then of the call's own keys, from the first to the last that one of its q-cols sees. lo_top, hi_low: positions from
+// the one to below the other are seen by all of the wave's q-cols.
+struct KeyTiles {
+  int c_first, c_end, o_first, o_end, lo_top, hi_low;
+};
+template <int TK, int WAVES, int COLS>
+__device__ inline KeyTiles key_tiles(const ExtArgs& a, Span all, int (&bounds)[WAVES][2], int wave, int lane, int split) {
+  int lo = all.len ? all.lo : INT_MAX, hi = all.len ? all.lo + int(all.len) : 0;
+  int lo_top = all.len ? all.lo : INT_MAX, hi_low = hi;
+#pragma unroll
+  for (int x = 1; x < COLS; x <<= 1) {
+    lo = min(lo, __shfl_xor(lo, x));
+    hi = max(hi, __shfl_xor(hi, x));
+    lo_top = max(lo_top, __shfl_xor(lo_top, x));
+    hi_low = min(hi_low, __shfl_xor(hi_low, x));
+  }
+  if (lane == 0) bounds[wave][0] = lo, bounds[wave][1] = hi;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) lo = min(lo, bounds[w][0]), hi = max(hi, bounds[w][1]);
+  int c_lo = 0, c_n = 0, o_lo = 0, o_n = 0;
+  if (hi > lo) {
+    const int s_lo = a.ring ? 0 : min(lo, a.tiles), s_hi = a.ring ? a.tiles : min(min(hi, a.cached_end), a.tiles);
+    if (s_hi > s_lo && lo < a.cached_end) c_lo = s_lo / TK, c_n = (s_hi + TK - 1) / TK - c_lo;
+    const int j_lo = max(0, lo - a.pos0), j_hi = min(a.own, hi - a.pos0);
+    if (j_hi > j_lo) o_lo = j_lo / TK, o_n = (j_hi + TK - 1) / TK - o_lo;
+  }
+  const int n = c_n + o_n, first = int((long long)n * split / a.splits), last = int((long long)n * (split + 1) / a.splits);
+  auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  return {uniform(c_lo + min(first, c_n)), uniform(c_lo + min(last, c_n)), uniform(o_lo + max(first, c_n) - c_n),
+          uniform(o_lo + max(last, c_n) - c_n), uniform(lo_top), uniform(hi_low)};
+}
+
+template <int D, int T, int MOD>
 __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a) {
   using R = Rows<D>;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -880,33 +955,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a) 
   const bool live = row < a.n_q;
 
   const Span all = live ? row_span(a, row) : Span{0, 0u, 0};
-  // what the wave's q-cols see, and the work-group's: from the first to past the last position
-  int lo = all.len ? all.lo : INT_MAX, hi = all.len ? all.lo + int(all.len) : 0;
-  int lo_top = all.len ? all.lo : live ? INT_MAX : 0, hi_low = live ? (all.len ? all.lo + int(all.len) : 0) : INT_MAX;
-#pragma unroll
-  for (int x = 1; x < 32; x <<= 1) {
-    lo = min(lo, __shfl_xor(lo, x));
-    hi = max(hi, __shfl_xor(hi, x));
-    lo_top = max(lo_top, __shfl_xor(lo_top, x));
-    hi_low = min(hi_low, __shfl_xor(hi_low, x));
-  }
-  lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
-  lo_top = __builtin_amdgcn_readfirstlane(lo_top), hi_low = __builtin_amdgcn_readfirstlane(hi_low);
-  if (lane == 0) bounds[wave][0] = lo, bounds[wave][1] = hi;
-  __syncthreads();
-  int wg_lo = bounds[0][0], wg_hi = bounds[0][1];
-#pragma unroll
-  for (int w = 1; w < kExtWaves; ++w) wg_lo = min(wg_lo, bounds[w][0]), wg_hi = max(wg_hi, bounds[w][1]);
-
-  // the tiles: of the cache (a linear one's slots are positions), then of the call's own keys
-  int c_lo = 0, c_n = 0, o_lo = 0, o_n = 0;
-  if (wg_hi > wg_lo) {
-    const int s_lo = a.ring ? 0 : min(wg_lo, a.tiles), s_hi = a.ring ? a.tiles : min(min(wg_hi, a.cached_end), a.tiles);
-    if (s_hi > s_lo && wg_lo < a.cached_end) c_lo = s_lo / R::TK, c_n = (s_hi + R::TK - 1) / R::TK - c_lo;
-    const int j_lo = max(0, wg_lo - a.pos0), j_hi = min(a.own, wg_hi - a.pos0);
-    if (j_hi > j_lo) o_lo = j_lo / R::TK, o_n = (j_hi + R::TK - 1) / R::TK - o_lo;
-  }
-  const int n = c_n + o_n, first = int((long long)n * split / a.splits), last = int((long long)n * (split + 1) / a.splits);
+  const KeyTiles n = key_tiles<R::TK, kExtWaves, 32>(a, all, bounds, wave, lane, split);
 
   float m = -INFINITY, l = 0.f;
   f32x16 acc[R::NB];
@@ -916,174 +965,233 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a) 
     for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
   const size_t q_at = (size_t(row) * size_t(a.heads) + size_t(head)) * D + size_t(8 * half);
 
-  // the tiles f .. e - 1 of one kind: SRC's stages, a q operand of its type
+  uint4* const kbuf = reinterpret_cast<uint4*>(smem);             // two buffers each
+  uint4* const vbuf = kbuf + 2 * R::kEntries;
+  int* const info = reinterpret_cast<int*>(smem + size_t(R::kEntries) * 64);
+
+  // The tiles f .. e - 1 of one kind (S: the type of its stages). Where registers allow (kAhead), a wave's matrix ops and
+  // its vector ALUs work on different tiles at a time: while it turns tile t's scores into weights, first the products of
+  // tile t - 1 with V and then tile t + 1's scores are made. So K is in LDS two tiles ahead of V, and a barrier ends each
+  // step.
   auto run = [&](auto src, auto operand, int f, int e, Span span, int span_hi_low, float global) {
     constexpr int S = decltype(src)::value;
     constexpr bool OWN = decltype(operand)::value;
     using X8 = typename OperandOf<S>::type;
     if (f >= e) return;
     X8 q[R::NS];
+    Score sc;
     bf16x8 x[R::NS];
     row_chunks(a.q, a.bf16, live, [&](int c) { return (live ? q_at : size_t(8 * half)) + size_t(16 * c); }, x);
-    if (a.scale < 0.f) {
-#pragma unroll
-      for (int c = 0; c < R::NS; ++c) x[c] = -x[c];
-    }
-    const float factor = to_operand(x, q, [](float y) { return xor32_max(y); });
-    const Score sc = score_of(a, live ? head : 0, factor * global);
     Stage<D, S> stage;
     int pos = -1;
     float ks = 0.f, vs = 0.f;
-    auto load = [&](int t) {
+    auto half_tile = [&](int t) { return !OWN && R::TK == 64 && t * 64 + 32 == a.slots_pad; };
+    auto load_k = [&](int t) {
+      t = min(t, e - 1);   // past the last: loaded again, and not used
+      pos = -1;
       if constexpr (OWN) {
-        stage.load(a.pk, a.pv, h, (a.own + 63) / 64 * 64, t, false);
-        if (tid < R::TK) pos = t * R::TK + tid < a.own ? a.pos0 + t * R::TK + tid : -1;
+        stage.load_k(a.pk, h, (a.own + 63) / 64 * 64, t, false);
+        if (tid < R::TK && t * R::TK + tid < a.own) pos = a.pos0 + t * R::TK + tid;
       } else {
-        const bool half_tile = R::TK == 64 && t * 64 + 32 == a.slots_pad;
         if constexpr (S == kNvfp4)
-          stage.load(a, h, t, half_tile);
+          stage.load_k(a, h, t, half_tile(t));
         else
-          stage.load(reinterpret_cast<const uint4*>(a.ck), reinterpret_cast<const uint4*>(a.cv), h, a.slots_pad, t, half_tile);
-        pos = -1;
-        if (tid < (half_tile ? 32 : R::TK)) {
+          stage.load_k(reinterpret_cast<const uint4*>(a.ck), h, a.slots_pad, t, half_tile(t));
+        if (tid < (half_tile(t) ? 32 : R::TK)) {
           pos = a.slot_pos[t * R::TK + tid];
           if constexpr (S == kFp8) {
             const size_t at = size_t(h) * size_t(a.slots_pad) + size_t(t * R::TK + tid);
             ks = static_cast<const float*>(a.ks)[at];
             vs = static_cast<const float*>(a.vs)[at];
-            if (not_finite(vs)) ks = NAN, vs = 0.f;
           }
         }
       }
     };
-    auto store = [&](int buf) {
-      uint8_t* base = smem + size_t(buf) * R::kBuffer;
-      stage.store(reinterpret_cast<uint4*>(base), reinterpret_cast<uint4*>(base) + R::kEntries);
-      int* lp = reinterpret_cast<int*>(base + R::kEntries * 32);
-      if (tid < R::TK) {
-        lp[tid] = pos;
-        if constexpr (S == kFp8) {
-          reinterpret_cast<float*>(lp)[R::TK + tid] = ks;
-          reinterpret_cast<float*>(lp)[2 * R::TK + tid] = vs;
+    auto load_v = [&](int t) {
+      t = min(t, e - 1);
+      if constexpr (OWN)
+        stage.load_v(a.pv, h, (a.own + 63) / 64 * 64, t, false);
+      else if constexpr (S == kNvfp4)
+        stage.load_v(a, h, t, half_tile(t));
+      else
+        stage.load_v(reinterpret_cast<const uint4*>(a.cv), h, a.slots_pad, t, half_tile(t));
+    };
+    auto store_k = [&](int t) {
+      stage.store_k(kbuf + ((t - f) & 1) * R::kEntries);
+      int* lp = info + ((t - f) & 3) * R::kInfo;
+      if (wave == 0) {   // the tile's last and first positions, -1 with a slot that has none
+        int top = pos, least = tid < R::TK ? pos : INT_MAX;
+        wave_extremes(top, least);
+        if (tid == 0) lp[3 * R::TK] = top, lp[3 * R::TK + 1] = least;
+        if (tid < R::TK) {
+          lp[tid] = pos;
+          if constexpr (S == kFp8) {   // a key whose V scale is not finite is NaN itself, and the scale zero
+            reinterpret_cast<float*>(lp)[R::TK + tid] = not_finite(vs) ? NAN : ks;
+            reinterpret_cast<float*>(lp)[2 * R::TK + tid] = not_finite(vs) ? 0.f : vs;
+          }
         }
       }
     };
-    load(f);
-    __syncthreads();   // a buffer may still be read by what ran before
-    store(0);
-    __syncthreads();
-    for (int t = f; t < e; ++t) {
-      const int buf = (t - f) & 1;
-      if (t + 1 < e) load(t + 1);
-      const uint8_t* base = smem + size_t(buf) * R::kBuffer;
-      const X8* lk = reinterpret_cast<const X8*>(base);
-      const X8* lv = lk + R::kEntries;
-      const int* lp = reinterpret_cast<const int*>(base + R::kEntries * 32);
-      // the tile's positions against what the wave's q-cols see: none, all, or a mask
-      const int mine = lp[lane & (R::TK - 1)];
-      int top = mine, low = mine < 0 ? INT_MAX : mine, least = mine;
+    auto store_v = [&](int t) { stage.store_v(vbuf + ((t - f) & 1) * R::kEntries); };
+    auto scores = [&](int t, f32x16 (&s)[R::KB]) {
+      const X8* lk = reinterpret_cast<const X8*>(kbuf + ((t - f) & 1) * R::kEntries);
 #pragma unroll
-      for (int y = 1; y < 64; y <<= 1) {
-        top = max(top, __shfl_xor(top, y));
-        low = min(low, __shfl_xor(low, y));
-        least = min(least, __shfl_xor(least, y));
+      for (int b = 0; b < R::KB; ++b) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
+#pragma unroll
+        for (int c = 0; c < R::NS; ++c) s[b] = mfma32(lk[(b * R::NS + c) * 64 + lane], q[c], s[b]);
       }
-      if (top >= lo && low < hi) {
-        const bool mask = least < lo_top || top >= span_hi_low;
-        f32x16 s[R::KB];
+    };
+    X8 w[R::KS];
 #pragma unroll
-        for (int b = 0; b < R::KB; ++b)
+    for (int k = 0; k < R::KS; ++k) w[k] = X8{};
+    auto products = [&](int t) {
+      const X8* lv = reinterpret_cast<const X8*>(vbuf + ((t - f) & 1) * R::kEntries);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
+      for (int k = 0; k < R::KS; ++k)
 #pragma unroll
-        for (int b = 0; b < R::KB; ++b)
+        for (int d = 0; d < R::NB; ++d) acc[d] = mfma32(lv[(d * R::KS + k) * 64 + lane], w[k], acc[d]);
+    };
+
+    // scores to y (scaled, changed, masked), m moved if they pass it; then their weights
+    auto softmax_begin = [&](int t, const f32x16 (&s)[R::KB], float (&y)[R::KB][16]) {
+      const int* lp = info + ((t - f) & 3) * R::kInfo;
+      // row 8 j + r' of block b (r = 4 j + r') is key 32 b + 8 j + 4 half + r'
+      const int4* lp4 = reinterpret_cast<const int4*>(lp) + half;
+      const float4* lf4 = reinterpret_cast<const float4*>(lp) + half;
 #pragma unroll
-          for (int c = 0; c < R::NS; ++c) s[b] = mfma32(lk[(b * R::NS + c) * 64 + lane], q[c], s[b]);
-        // scores; row 8 j + r' of block b (r = 4 j + r') is key 32 b + 8 j + 4 half + r'
-        const int4* lp4 = reinterpret_cast<const int4*>(lp) + half;
-        const float4* lf4 = reinterpret_cast<const float4*>(lp) + half;
-        float mx = -INFINITY;
-        if (mask || MOD || S == kFp8) {
+      for (int b = 0; b < R::KB; ++b)
 #pragma unroll
-          for (int b = 0; b < R::KB; ++b)
+        for (int j = 0; j < 4; ++j) {
+          int p[4] = {0, 0, 0, 0};
+          float k4[4] = {1.f, 1.f, 1.f, 1.f};
+          if constexpr ((MOD & kBias) != 0) {
+            const int4 p4 = lp4[b * 8 + j * 2];
+            p[0] = p4.x, p[1] = p4.y, p[2] = p4.z, p[3] = p4.w;
+          }
+          if constexpr (S == kFp8) {
+            const float4 z = lf4[R::TK / 4 + b * 8 + j * 2];
+            k4[0] = z.x, k4[1] = z.y, k4[2] = z.z, k4[3] = z.w;
+          }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int4 p4 = lp4[b * 8 + j * 2];
-              const int p[4] = {p4.x, p4.y, p4.z, p4.w};
-              float k4[4] = {1.f, 1.f, 1.f, 1.f};
-              if constexpr (S == kFp8) {
-                const float4 y = lf4[R::TK / 4 + b * 8 + j * 2];
-                k4[0] = y.x, k4[1] = y.y, k4[2] = y.z, k4[3] = y.w;
-              }
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                float y = s[b][4 * j + r];
-                if constexpr (S == kFp8) y *= k4[r];
-                y = MOD ? changed(a, sc, y, span.t - p[r]) : y * sc.f;
-                s[b][4 * j + r] = uint32_t(p[r] - span.lo) < span.len ? y : -INFINITY;
-              }
-            }
-        } else {
-#pragma unroll
-          for (int b = 0; b < R::KB; ++b)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[b][r] *= sc.f;
+          for (int r = 0; r < 4; ++r)
+            y[b][4 * j + r] = changed<MOD>(sc, S == kFp8 ? s[b][4 * j + r] * k4[r] : s[b][4 * j + r], span.t - p[r]);
         }
-#pragma unroll
-        for (int b = 0; b < R::KB; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
-        mx = xor32_max(mx);
-        if (__ballot(mx > m + kSlack)) {
-          const float to = mx > m + kSlack ? mx : m;
-          const float corr = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.f : to));
-          m = to;
-          l *= corr;
-#pragma unroll
-          for (int d = 0; d < R::NB; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[d][r] *= corr;
-        }
-        const float ref = (m == -INFINITY ? 0.f : m) - kUp;
-        float sum = 0.f;
-        X8 w[R::KS];
+      // the tile's positions against what the wave's q-cols see: all, or a mask
+      const int top = __builtin_amdgcn_readfirstlane(lp[3 * R::TK]), least = __builtin_amdgcn_readfirstlane(lp[3 * R::TK + 1]);
+      if (least < n.lo_top || top >= span_hi_low) {
 #pragma unroll
         for (int b = 0; b < R::KB; ++b)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            float v4[4] = {1.f, 1.f, 1.f, 1.f};
-            if constexpr (S == kFp8) {
-              const float4 y = lf4[2 * R::TK / 4 + b * 8 + j * 2];
-              v4[0] = y.x, v4[1] = y.y, v4[2] = y.z, v4[3] = y.w;
-            }
+            const int4 p4 = lp4[b * 8 + j * 2];
+            const int p[4] = {p4.x, p4.y, p4.z, p4.w};
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              float p = __builtin_amdgcn_exp2f(s[b][4 * j + r] - ref);
-              sum += p;
-              if constexpr (S == kFp8) p *= v4[r];
-              w[2 * b + (j & 1)][(j >> 1) * 4 + r] = p;
-            }
+            for (int r = 0; r < 4; ++r)
+              if (uint32_t(p[r] - span.lo) >= span.len) y[b][4 * j + r] = -INFINITY;
           }
-        l += sum;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < R::KB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, y[b][r]);
+      mx = xor32_max(mx);
+      if (__ballot(mx > m + kSlack)) {
+        const float to = mx > m + kSlack ? mx : m;
+        const float corr = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.f : to));
+        m = to;
+        l *= corr;
 #pragma unroll
         for (int d = 0; d < R::NB; ++d)
 #pragma unroll
-          for (int k = 0; k < R::KS; ++k) acc[d] = mfma32(lv[(d * R::KS + k) * 64 + lane], w[k], acc[d]);
+          for (int r = 0; r < 16; ++r) acc[d][r] *= corr;
       }
-      if (t + 1 < e) store(buf ^ 1);
+    };
+    auto softmax_end = [&](int t, const float (&y)[R::KB][16]) {
+      const float4* lf4 = reinterpret_cast<const float4*>(info + ((t - f) & 3) * R::kInfo) + half;
+      const float ref = (m == -INFINITY ? 0.f : m) - kUp;
+      float sum = 0.f;
+#pragma unroll
+      for (int b = 0; b < R::KB; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float v4[4] = {1.f, 1.f, 1.f, 1.f};
+          if constexpr (S == kFp8) {
+            const float4 z = lf4[2 * R::TK / 4 + b * 8 + j * 2];
+            v4[0] = z.x, v4[1] = z.y, v4[2] = z.z, v4[3] = z.w;
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float p = __builtin_amdgcn_exp2f(y[b][4 * j + r] - ref);
+            sum += p;
+            if constexpr (S == kFp8) p *= v4[r];
+            w[2 * b + (j & 1)][(j >> 1) * 4 + r] = p;
+          }
+        }
+      l += sum;
+    };
+
+    load_k(f);
+    __syncthreads();   // the buffers may still be read by what ran before
+    store_k(f);
+    if (a.scale < 0.f) {
+#pragma unroll
+      for (int c = 0; c < R::NS; ++c) x[c] = -x[c];
+    }
+    const float factor = to_operand(x, q, [](float y) { return xor32_max(y); });
+    sc = score_of(a, live ? head : 0, factor * global);
+    f32x16 s[R::KB];
+    float y[R::KB][16];
+    if constexpr (R::kAhead) {
+      load_k(f + 1);
+#pragma unroll
+      for (int u = 0; u < R::PER; ++u) vbuf[R::kEntries + tid + u * 256] = make_uint4(0, 0, 0, 0);   // "tile f - 1"
       __syncthreads();
+      scores(f, s);
+      store_k(f + 1);
+      load_k(f + 2);
+      load_v(f);
+      __syncthreads();
+      for (int t = f; t < e; ++t) {
+        products(t - 1);
+        store_k(t + 2);
+        store_v(t);
+        load_k(t + 3);
+        load_v(t + 1);
+        softmax_begin(t, s, y);
+        scores(t + 1, s);   // (past the last tile: of the one before it, and not used)
+        softmax_end(t, y);
+        __syncthreads();
+      }
+      products(e - 1);
+    } else {
+      load_v(f);
+      store_v(f);
+      __syncthreads();
+      for (int t = f; t < e; ++t) {
+        load_k(t + 1);
+        load_v(t + 1);
+        scores(t, s);
+        softmax_begin(t, s, y);
+        softmax_end(t, y);
+        products(t);
+        store_k(t + 1);
+        store_v(t + 1);
+        __syncthreads();
+      }
     }
   };
-  run(std::integral_constant<int, T>{}, std::false_type{}, c_lo + min(first, c_n), c_lo + min(last, c_n), cached_span(a, all),
-      min(hi_low, a.cached_end), T == kNvfp4 ? a.kglobal : 1.f);
+  run(std::integral_constant<int, T>{}, std::false_type{}, n.c_first, n.c_end, cached_span(a, all),
+      min(n.hi_low, a.cached_end), T == kNvfp4 ? a.kglobal : 1.f);
   if (T == kNvfp4 && a.vglobal != 1.f) {
 #pragma unroll
     for (int d = 0; d < R::NB; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[d][r] *= a.vglobal;
   }
-  run(std::integral_constant<int, kBf16>{}, std::true_type{}, o_lo + max(first, c_n) - c_n, o_lo + max(last, c_n) - c_n, all,
-      hi_low, 1.f);
+  run(std::integral_constant<int, kBf16>{}, std::true_type{}, n.o_first, n.o_end, all, n.hi_low, 1.f);
 
   l = xor32_sum(l);
   if (a.splits == 1) {
@@ -1136,7 +1244,7 @@ template <int D, int T, int G>
 __global__ void __launch_bounds__(256) ext_merge_kernel(ExtArgs a, int kv_heads, int total) {
   constexpr int L = D / 4, PER = 256 / (L * G), B = 8;   // lanes a record; q-cols of a work-group; records of a batch
   __shared__ float4 part[G > 1 ? PER * G * L : 1];
-  __shared__ float slow[264 + D], all_m[4], all_l[4];
+  __shared__ float slow[272 + D], all_m[4], all_l[4];
   __shared__ int again[PER];
   const int tid = int(threadIdx.x), x = tid % L, grp = tid / L % G, mine = tid / (L * G);
   const int id = int(blockIdx.x) * PER + mine;   // q-col of the call: row * heads + head
@@ -1254,7 +1362,7 @@ ExtPlan ext_plan(const ExtCall& a, int cus) {
   const int tk = a.d == 256 ? 32 : 64;
   const long long keys = slots - lo + (a.k ? a.n_q : 0), tiles = (keys + tk - 1) / tk;
   const long long groups = (long long)p.blocks * a.kv_heads;
-  p.splits = int(std::max(1LL, std::min((2LL * cus + groups - 1) / groups, tiles / 8)));
+  p.splits = int(std::max(1LL, std::min((2LL * cus + groups - 1) / groups, getenv("XTG_TPS") ? tiles / atoi(getenv("XTG_TPS")) : tiles / 8)));
   if (p.splits > 1)
     p.record_bytes = size_t(p.splits) * size_t(groups) * 128 * size_t(a.d + 2) * sizeof(float);
   if (a.k) p.pack_bytes = 2 * size_t(a.kv_heads) * size_t((a.n_q + 63) / 64 * 64) * size_t(a.d) * 2;
@@ -1263,9 +1371,8 @@ ExtPlan ext_plan(const ExtCall& a, int cus) {
 
 namespace {
 
-template <int D, int T, bool MOD>
+template <int D, int T, int MOD>
 void launch(const ExtCall& c, const ExtPlan& p, const ExtArgs& a, hipStream_t stream, const Timed& timed) {
-  const char* mod = MOD ? "true" : "false";
   if (p.few) {
     timed([&] {
       const dim3 grid{unsigned(c.kv_heads), unsigned(a.records), unsigned(p.blocks)}, block{kExtWaves * 64};
@@ -1278,7 +1385,7 @@ void launch(const ExtCall& c, const ExtPlan& p, const ExtArgs& a, hipStream_t st
       else
         go(&ext_few_kernel<D, 2, T, MOD>, few_lds<D, 2>());
       HIP_CHECK(hipGetLastError());
-      return strf("ext_few_kernel<%d, %d, %d, %s>", D, p.cols / 16, T, mod);
+      return strf("ext_few_kernel<%d, %d, %d, %d>", D, p.cols / 16, T, MOD);
     });
   } else {
     if (c.k)
@@ -1291,12 +1398,12 @@ void launch(const ExtCall& c, const ExtPlan& p, const ExtArgs& a, hipStream_t st
         return strf("ext_pack_kernel<%d, %d>", D, T);
       });
     timed([&] {
-      const size_t lds = 2 * Rows<D>::kBuffer;
+      const dim3 grid{unsigned(c.kv_heads), unsigned(p.blocks), unsigned(p.splits)};
+      const size_t lds = Rows<D>::kLds;
       allow_lds(reinterpret_cast<const void*>(&ext_rows_kernel<D, T, MOD>), lds);
-      hipLaunchKernelGGL((ext_rows_kernel<D, T, MOD>), dim3(unsigned(c.kv_heads), unsigned(p.blocks), unsigned(p.splits)),
-                         dim3(kExtWaves * 64), lds, stream, a);
+      hipLaunchKernelGGL((ext_rows_kernel<D, T, MOD>), grid, dim3(kExtWaves * 64), lds, stream, a);
       HIP_CHECK(hipGetLastError());
-      return strf("ext_rows_kernel<%d, %d, %s>", D, T, mod);
+      return strf("ext_rows_kernel<%d, %d, %d>", D, T, MOD);
     });
   }
   if (a.records > 1)
@@ -1315,10 +1422,14 @@ void launch(const ExtCall& c, const ExtPlan& p, const ExtArgs& a, hipStream_t st
 
 template <int D, int T>
 void launch(const ExtCall& c, const ExtPlan& p, const ExtArgs& a, hipStream_t stream, const Timed& timed) {
-  if (c.softcap > 0.f || c.slopes)
-    launch<D, T, true>(c, p, a, stream, timed);
+  if (c.softcap > 0.f && c.slopes)
+    launch<D, T, kCap | kBias>(c, p, a, stream, timed);
+  else if (c.softcap > 0.f)
+    launch<D, T, kCap>(c, p, a, stream, timed);
+  else if (c.slopes)
+    launch<D, T, kBias>(c, p, a, stream, timed);
   else
-    launch<D, T, false>(c, p, a, stream, timed);
+    launch<D, T, 0>(c, p, a, stream, timed);
 }
 
 }  // namespace
