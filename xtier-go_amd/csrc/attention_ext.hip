@@ -22,7 +22,6 @@
 // With the others a q-col whose sum of weights is finite and whose accumulator is not is computed again key by key, by
 // whichever kernel writes it (slow_col).
 #include <algorithm>
-#include <cstdlib>
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -279,6 +278,21 @@ __device__ inline void slow_col(const ExtArgs& a, int h, int kv_heads, int row, 
     else
       static_cast<float*>(a.out)[at] = y;
   }
+}
+
+// The largest and smallest of a wave's values (every lane gets them).
+__device__ inline void wave_extremes(int& top, int& least) {
+  auto step = [&](int a, int b) { top = max(top, a), least = min(least, b); };
+  step(__builtin_amdgcn_update_dpp(0, top, kDppXor1, 0xF, 0xF, false), __builtin_amdgcn_update_dpp(0, least, kDppXor1, 0xF, 0xF, false));
+  step(__builtin_amdgcn_update_dpp(0, top, kDppXor2, 0xF, 0xF, false), __builtin_amdgcn_update_dpp(0, least, kDppXor2, 0xF, 0xF, false));
+  step(__builtin_amdgcn_update_dpp(0, top, kDppHalfMirror, 0xF, 0xF, false), __builtin_amdgcn_update_dpp(0, least, kDppHalfMirror, 0xF, 0xF, false));
+  step(__builtin_amdgcn_update_dpp(0, top, kDppMirror, 0xF, 0xF, false), __builtin_amdgcn_update_dpp(0, least, kDppMirror, 0xF, 0xF, false));
+  auto a = __builtin_amdgcn_permlane16_swap(uint32_t(top), uint32_t(top), false, false);
+  auto b = __builtin_amdgcn_permlane16_swap(uint32_t(least), uint32_t(least), false, false);
+  top = max(int(a[0]), int(a[1])), least = min(int(b[0]), int(b[1]));
+  a = __builtin_amdgcn_permlane32_swap(uint32_t(top), uint32_t(top), false, false);
+  b = __builtin_amdgcn_permlane32_swap(uint32_t(least), uint32_t(least), false, false);
+  top = max(int(a[0]), int(a[1])), least = min(int(b[0]), int(b[1]));
 }
 
 // ------------------------------------------------------------------------------------------------- few q-cols
@@ -553,7 +567,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, QB * D > 256 ? 1 : 2) ext_few_
   const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) >> 6, g = lane >> 4, i = lane & 15;
   const int h = int(blockIdx.x), kv_heads = int(gridDim.x), split = int(gridDim.y) - 1 - int(blockIdx.y);
   const int col0 = int(blockIdx.z) * QB * 16;   // the work-group's first q-col
-  const bool own = split == a.splits;   // one more work-group, queued first: the call's own keys
+  const bool own = split >= a.splits;   // the work-groups past the cache's, queued first: the call's own keys
   FewState<D, QB> st;
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
@@ -566,10 +580,14 @@ __global__ void __launch_bounds__(kExtWaves * 64, QB * D > 256 ? 1 : 2) ext_few_
     FewQueries<D, QB, OwnTile<D, T>> rows;
     rows.load(a, h, col0, lane);
     rows.operand(a, 1.f, q);
-    for (int t = wave; 32 * t < a.own; t += kExtWaves) {
+    const int t = (split - a.splits) * kExtWaves + wave, p = a.pos0 + 32 * t, past = a.pos0 + a.own;
+    bool any = false;   // a q-col that sees one of the tile's keys
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb)
+      any |= rows.span[qb].len > 0 && rows.span[qb].lo < p + 32 && int(rows.span[qb].len) > p - rows.span[qb].lo;
+    if (32 * t < a.own && __ballot(any)) {
       OwnTile<D, T> tile(a, h, kv_heads, t, lane);
-      const int p = a.pos0 + 32 * t + 4 * g, past = a.pos0 + a.own;
-      auto at = [&](int e) { return p + e < past ? p + e : -1; };
+      auto at = [&](int e) { return p + 4 * g + e < past ? p + 4 * g + e : -1; };
       few_tile<D, QB, MOD>(a, tile, q, rows.span, rows.sc, st, make_int4(at(0), at(1), at(2), at(3)),
                            make_int4(at(16), at(17), at(18), at(19)), [] {}, [] {});
     }
@@ -582,6 +600,14 @@ __global__ void __launch_bounds__(kExtWaves * 64, QB * D > 256 ? 1 : 2) ext_few_
     rows.load(a, h, col0, lane);
     Tile<D, T> tile;
     int t = t_begin + wave;
+    if (!a.ring && (a.first || a.window > 0)) {   // tiles before the first position that a q-col sees
+      int lo = INT_MAX, none = 0;
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) lo = rows.span[qb].len ? min(lo, rows.span[qb].lo) : lo;
+      wave_extremes(none, lo);
+      const int skip = (min(__builtin_amdgcn_readfirstlane(lo) / 32, t_end) - t + kExtWaves - 1) / kExtWaves;
+      if (skip > 0) t += skip * kExtWaves;
+    }
     const int4* sp = reinterpret_cast<const int4*>(a.slot_pos) + g;
     if (t < t_end) {
       tile.load_k(a, h, t, lane);
@@ -893,21 +919,6 @@ struct Stage<D, kNvfp4> {
     }
   }
 };
-
-// The largest and smallest of a wave's values (every lane gets them).
-__device__ inline void wave_extremes(int& top, int& least) {
-  auto step = [&](int a, int b) { top = max(top, a), least = min(least, b); };
-  step(__builtin_amdgcn_update_dpp(0, top, kDppXor1, 0xF, 0xF, false), __builtin_amdgcn_update_dpp(0, least, kDppXor1, 0xF, 0xF, false));
-  step(__builtin_amdgcn_update_dpp(0, top, kDppXor2, 0xF, 0xF, false), __builtin_amdgcn_update_dpp(0, least, kDppXor2, 0xF, 0xF, false));
-  step(__builtin_amdgcn_update_dpp(0, top, kDppHalfMirror, 0xF, 0xF, false), __builtin_amdgcn_update_dpp(0, least, kDppHalfMirror, 0xF, 0xF, false));
-  step(__builtin_amdgcn_update_dpp(0, top, kDppMirror, 0xF, 0xF, false), __builtin_amdgcn_update_dpp(0, least, kDppMirror, 0xF, 0xF, false));
-  auto a = __builtin_amdgcn_permlane16_swap(uint32_t(top), uint32_t(top), false, false);
-  auto b = __builtin_amdgcn_permlane16_swap(uint32_t(least), uint32_t(least), false, false);
-  top = max(int(a[0]), int(a[1])), least = min(int(b[0]), int(b[1]));
-  a = __builtin_amdgcn_permlane32_swap(uint32_t(top), uint32_t(top), false, false);
-  b = __builtin_amdgcn_permlane32_swap(uint32_t(least), uint32_t(least), false, false);
-  top = max(int(a[0]), int(a[1])), least = min(int(b[0]), int(b[1]));
-}
 
 // The tiles of TK keys that a work-group goes over (its split's part): of the cache (a linear one's slots are positions),
 // then of the call's own keys, from the first to the last that one of its q-cols sees. lo_top, hi_low: positions from
@@ -1332,6 +1343,11 @@ __global__ void __launch_bounds__(256) ext_merge_kernel(ExtArgs a, int kv_heads,
 
 // ---------------------------------------------------------------------------------------------------- launches
 
+// Calls of up to this many q-cols take ext_few_kernel, which starts sooner (one launch less, no barriers) and dequantises
+// a tile again for every 32 of them: over 4000 NVFP4 keys of 128 dims, 32 / 8 heads, 384 q-cols took 27.6 us (many: 44.1),
+// 768 51.6 (63.6), 1024 64.4 (53.9).
+constexpr int kFewCols = 768;
+
 ExtPlan ext_plan(const ExtCall& a, int cus) {
   ExtPlan p;
   const int group = a.heads / a.kv_heads;
@@ -1344,17 +1360,22 @@ ExtPlan ext_plan(const ExtCall& a, int cus) {
     if (!a.cache->ring || a.k) slots = std::min(slots, past);   // (a ring fills from its first slot on)
     if (!a.cache->ring && a.window > 0) lo = std::max(0LL, std::min(slots, a.pos0 - a.window + 1));
   }
-  p.few = cols <= 32;
+  const int own_tiles = a.k ? (a.n_q + 31) / 32 : 0;
+  p.few = cols <= kFewCols && cols * group <= 65536;
   if (p.few) {
     p.tile_lo = int(lo / 32);
     p.tiles = slots > lo ? int((slots + 31) / 32) - p.tile_lo : 0;
-    // a work-group a CU, at least a tile for each wave; where that leaves CUs idle, the second 16 q-cols apart
-    p.splits = std::min(std::max(1, cus / a.kv_heads), (p.tiles + kExtWaves - 1) / kExtWaves);
-    p.cols = cols > 16 && 2 * p.splits * a.kv_heads > cus ? 32 : 16;
+    // at least a tile for each wave; a work-group a CU (one and a half where blocks of q-cols share what they read); where
+    // that leaves CUs idle, blocks of 16 q-cols instead of 32
+    const int most = (p.tiles + kExtWaves - 1) / kExtWaves;
+    p.cols = cols <= 16 || (cols <= 32 && 2 * most * a.kv_heads <= cus) ? 16 : 32;
     p.blocks = int((cols + p.cols - 1) / p.cols);
+    p.splits = std::min(std::max(1, (p.blocks > 2 ? cus * 3 / 2 : cus) / (a.kv_heads * p.blocks)), most);
     if (!a.k) p.splits = std::max(p.splits, 1);
-    const size_t records = size_t(p.splits) + (a.k ? 1 : 0);
-    if (records > 1) p.record_bytes = records * size_t(a.kv_heads) * size_t(p.blocks * p.cols) * size_t(a.d + 2) * sizeof(float);
+    p.own = (own_tiles + kExtWaves - 1) / kExtWaves;
+    const size_t records = size_t(p.splits) + size_t(p.own);
+    if (records > 1)
+      p.record_bytes = records * size_t(a.kv_heads) * size_t(p.blocks * p.cols) * size_t(a.d + 2) * sizeof(float);
     return p;
   }
   p.blocks = int((cols + 127) / 128);
@@ -1362,7 +1383,8 @@ ExtPlan ext_plan(const ExtCall& a, int cus) {
   const int tk = a.d == 256 ? 32 : 64;
   const long long keys = slots - lo + (a.k ? a.n_q : 0), tiles = (keys + tk - 1) / tk;
   const long long groups = (long long)p.blocks * a.kv_heads;
-  p.splits = int(std::max(1LL, std::min((2LL * cus + groups - 1) / groups, getenv("XTG_TPS") ? tiles / atoi(getenv("XTG_TPS")) : tiles / 8)));
+  // as many as leave every work-group resident at once (two a CU), four tiles each at least
+  p.splits = int(std::max(1LL, std::min(2LL * cus / groups, tiles / 4)));
   if (p.splits > 1)
     p.record_bytes = size_t(p.splits) * size_t(groups) * 128 * size_t(a.d + 2) * sizeof(float);
   if (a.k) p.pack_bytes = 2 * size_t(a.kv_heads) * size_t((a.n_q + 63) / 64 * 64) * size_t(a.d) * 2;
@@ -1446,7 +1468,7 @@ void launch_attn_ext(const ExtCall& c, const ExtPlan& p, void* scratch, hipStrea
   }
   a.tile_lo = p.tile_lo, a.tiles = p.tiles, a.splits = p.splits, a.cols = p.cols;
   a.own = c.k ? c.n_q : 0;
-  a.records = p.few ? p.splits + (c.k ? 1 : 0) : p.splits;
+  a.records = p.splits + p.own;
   a.n_q = c.n_q, a.pos0 = int(c.pos0), a.heads = c.heads, a.group = c.heads / c.kv_heads, a.window = c.window;
   a.group_inv = (65536u + uint32_t(a.group) - 1u) / uint32_t(a.group);
   a.bf16 = c.x_dtype == kXBF16;

@@ -28,11 +28,11 @@ struct ExtCall {
 
 // How a call is cut up. A q-col is a (row, q head of a KV head); a work-group takes `cols` of them for one KV head and
 // one of `splits` parts of the keys, and leaves a record (accumulator, maximum, sum) for each where there are more
-// than one. few: at most 32 q-cols, in one block or two, whose work-groups' waves take cache tiles of their own; the last
-// record is the call's own keys'. Otherwise blocks of 128 q-cols share tiles, the call's own keys packed as tiles too.
+// than one. few: the work-groups' waves take cache tiles of their own, and `own` work-groups more the call's own keys.
+// Otherwise blocks of 128 q-cols share tiles, the call's own keys packed as tiles too.
 struct ExtPlan {
   bool few = false;
-  int cols = 128, blocks = 1, splits = 1;
+  int cols = 128, blocks = 1, splits = 1, own = 0;
   int tile_lo = 0, tiles = 0;    // few: the cache's 32-slot tiles to scan; else tile_lo = 0 and the slots to scan
   size_t pack_bytes = 0;         // own keys and values as BF16 tiles
   size_t record_bytes = 0;
