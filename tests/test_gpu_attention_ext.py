@@ -73,7 +73,7 @@ class Call:
         bits = 11 if self.dtype == "nvfp4" and not self.own else 8
         finite = np.isfinite(out)
         np.testing.assert_array_equal(got[~finite], out[~finite].astype(np.float32))
-        off = np.abs(got.astype(np.float64) - out)[finite]
+        off = np.abs(got.astype(np.float64)[finite] - out[finite])
         tol = o.tolerance(out, size, most, self.d, bits, self.x)[finite]
         assert (off <= tol).all(), "off by %.3g of %.3g" % (off[off > tol].max(), tol[off > tol].max())
         return got
@@ -86,6 +86,8 @@ class Call:
 
 
 HEADS = {64: (16, 8), 128: (8, 2), 256: (4, 2)}
+# over 768 (row, q head of a KV head) pairs the call's work-groups share tiles; these groups of heads bring few rows there
+MANY = {64: (32, 1), 128: (64, 2), 256: (32, 1)}
 
 
 @pytest.mark.parametrize("d", [64, 128, 256])
@@ -95,6 +97,38 @@ HEADS = {64: (16, 8), 128: (8, 2), 256: (4, 2)}
 def test_plain_scores(hip, d, dtype, n, ctx):
     c = Call(hip, np.random.default_rng(n * 1000 + ctx + d), dtype, n, ctx if dtype != "none" else 0, *HEADS[d], d)
     c.check()
+    c.free()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", ["nvfp4", "bf16", "fp8", "none"])
+@pytest.mark.parametrize("n,ctx", [(25, 1), (26, 64), (33, 80), (40, 321), (130, 33)])
+def test_plain_scores_of_many(hip, d, dtype, n, ctx):
+    """The cache ends with the context: for 64 and 128 dims also in the middle of a tile of 64 keys."""
+    c = Call(hip, np.random.default_rng(n * 1000 + ctx + d), dtype, n, ctx if dtype != "none" else 0, *MANY[d], d,
+             slots=ctx)
+    c.check()
+    c.free()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", ["nvfp4", "bf16", "fp8", "none"])
+@pytest.mark.parametrize("kw", [dict(softcap=20.0), dict(slopes=True), dict(slopes=True, softcap=30.0, window=70)])
+def test_changed_scores_of_many(hip, d, dtype, kw):
+    kw = dict(kw)
+    if kw.get("slopes"):
+        kw["slopes"] = np.linspace(0.01, 0.5, MANY[d][0])
+    c = Call(hip, np.random.default_rng(d), dtype, 30, 200 if dtype != "none" else 0, *MANY[d], d, spread=5.0)
+    c.check(**kw)
+    c.free()
+
+
+def test_key_splits_of_many(hip):
+    """Enough tiles to be split over work-groups, with a window and documents that leave some of them without keys."""
+    c = Call(hip, np.random.default_rng(5), "nvfp4", 32, 3000, 64, 2, 128)
+    c.check()
+    c.check(window=500)
+    c.check(first=np.full(32, 2990), softcap=5.0)
     c.free()
 
 
@@ -122,13 +156,13 @@ def test_changed_scores_other_heads(hip, dtype, d, n):
 
 
 @pytest.mark.parametrize("dtype", ["nvfp4", "bf16", "none"])
-@pytest.mark.parametrize("n", [3, 90, 300])
-def test_documents_prefixes_and_padding(hip, dtype, n):
+@pytest.mark.parametrize("n,heads", [(3, 8), (90, 8), (300, 8), (26, 64), (150, 64)])
+def test_documents_prefixes_and_padding(hip, dtype, n, heads):
     """first / end as packed documents, prefixes seen both ways, padding rows (nothing), ends before the row, and
     values outside of every position."""
     rng = np.random.default_rng(n)
     ctx = 150 if dtype != "none" else 0
-    c = Call(hip, rng, dtype, n, ctx, 8, 2, 128)
+    c = Call(hip, rng, dtype, n, ctx, heads, 2, 128)
     cuts = np.sort(rng.integers(0, n, 4))
     start = np.array([max([0] + [ctx + x for x in cuts if x <= i and x > 0]) for i in range(n)])
     c.check(first=start)
@@ -147,19 +181,20 @@ def test_documents_prefixes_and_padding(hip, dtype, n):
 
 
 @pytest.mark.parametrize("dtype", ["nvfp4", "bf16", "fp8"])
+@pytest.mark.parametrize("heads", [8, 64])
 @pytest.mark.parametrize("n,ctx,ring,window", [(1, 500, 96, 90), (8, 77, 96, 64), (8, 1000, 103, 0), (60, 400, 160, 100),
-                                               (1, 95, 96, 0)])
-def test_rings(hip, dtype, n, ctx, ring, window):
-    c = Call(hip, np.random.default_rng(ctx), dtype, n, ctx, 8, 2, 128, ring=ring)
+                                               (1, 95, 96, 0), (26, 150, 90, 70)])
+def test_rings(hip, dtype, heads, n, ctx, ring, window):
+    c = Call(hip, np.random.default_rng(ctx), dtype, n, ctx, heads, 2, 128, ring=ring)
     c.check(window=window)
     c.free()
 
 
 @pytest.mark.parametrize("dtype", ["nvfp4", "bf16", "fp8"])
-@pytest.mark.parametrize("n", [1, 7, 50])
-def test_rows_already_stored(hip, dtype, n):
+@pytest.mark.parametrize("n,heads", [(1, 8), (7, 8), (50, 8), (50, 64)])
+def test_rows_already_stored(hip, dtype, n, heads):
     """k and v NULL: the call's rows are among the cached ones, also at positions from pos0 on."""
-    c = Call(hip, np.random.default_rng(n), dtype, n, 200, 8, 2, 128, own=False)
+    c = Call(hip, np.random.default_rng(n), dtype, n, 200, heads, 2, 128, own=False)
     c.check(pos0=200 - n)
     c.check(pos0=100)   # rows in the middle: later positions are masked
     c.check(pos0=100, end=np.full(n, 150), softcap=5.0)
@@ -177,9 +212,9 @@ def test_stale_slots_are_not_seen(hip):
 
 
 @pytest.mark.parametrize("dtype", ["nvfp4", "bf16"])
-@pytest.mark.parametrize("n", [2, 33])
-def test_fp32_rows(hip, dtype, n):
-    c = Call(hip, np.random.default_rng(n), dtype, n, 210, 8, 2, 128, x_dtype=o.F32)
+@pytest.mark.parametrize("n,heads", [(2, 8), (33, 8), (33, 64)])
+def test_fp32_rows(hip, dtype, n, heads):
+    c = Call(hip, np.random.default_rng(n), dtype, n, 210, heads, 2, 128, x_dtype=o.F32)
     c.check()
     c.check(softcap=4.0, window=60)
     c.free()
@@ -194,24 +229,24 @@ def test_head_groups(hip, heads, kvh, n):
 
 
 @pytest.mark.parametrize("scale", [4.0, -0.3, 0.0])
-@pytest.mark.parametrize("n", [1, 40])
-def test_scales_and_sharp_softmaxes(hip, scale, n):
-    c = Call(hip, np.random.default_rng(8), "nvfp4", n, 300, 8, 2, 128)
+@pytest.mark.parametrize("n,heads", [(1, 8), (40, 8), (40, 64)])
+def test_scales_and_sharp_softmaxes(hip, scale, n, heads):
+    c = Call(hip, np.random.default_rng(8), "nvfp4", n, 300, heads, 2, 128)
     c.check(scale=scale)
     c.check(scale=scale, softcap=50.0)
     c.free()
 
 
 @pytest.mark.parametrize("dtype", ["nvfp4", "bf16", "fp8"])
-@pytest.mark.parametrize("n", [1, 6, 70])
-def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(hip, dtype, n):
+@pytest.mark.parametrize("n,heads", [(1, 8), (6, 8), (70, 8), (26, 64)])
+def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(hip, dtype, n, heads):
     """NaN and infinities in cached keys and values outside of the rows' windows, inside of some, and in the call's own
     rows, seen by later rows only."""
     rng = np.random.default_rng(n)
     ctx, kvh, d = 120, 2, 128
-    c = Call(hip, rng, dtype, n, ctx, 8, kvh, d)
+    c = Call(hip, rng, dtype, n, ctx, heads, kvh, d)
     kc, vc = c.unit(rng, (ctx, kvh, d)), rng.standard_normal((ctx, kvh, d)).astype(np.float32)
-    q = c.unit(rng, (n, 8, d)) * d
+    q = c.unit(rng, (n, heads, d)) * d
     k, v = c.unit(rng, (n, kvh, d)), rng.standard_normal((n, kvh, d)).astype(np.float32)
     vc[20, 0, 3], kc[21, 1, 4], vc[22, 1, 9] = np.nan, np.nan, np.inf if dtype != "fp8" else np.nan
     if dtype != "fp8":   # its scale would be infinite, and the whole row NaN
@@ -232,16 +267,16 @@ def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(hip, dtype
     c.free()
 
 
-@pytest.mark.parametrize("n", [1, 5, 66])
-def test_captured_and_replayed(hip, n):
+@pytest.mark.parametrize("n,heads", [(1, 8), (5, 8), (66, 8), (26, 64)])
+def test_captured_and_replayed(hip, n, heads):
     """A graph of a write, an attention and a read, replayed with eager work between the replays."""
     rng = np.random.default_rng(n)
-    c = Call(hip, rng, "nvfp4", n, 900, 8, 2, 128, slots=1100)
+    c = Call(hip, rng, "nvfp4", n, 900, heads, 2, 128, slots=1100)
     k2, v2 = hip.array(shape=(n, 2, 128), dtype=np.uint16), hip.array(shape=(n, 2, 128), dtype=np.uint16)
-    slopes = np.linspace(0.1, 0.2, 8)
+    slopes = np.linspace(0.1, 0.2, heads)
     want = c.check(softcap=10.0, slopes=slopes)
     hip.graph_begin()
-    c.hip.attention_ext(c.cache, *c.dev, c.out, n, 900, 8, 2, 128, o.BF16, 0, None, 10.0, c.extra[0])
+    c.hip.attention_ext(c.cache, *c.dev, c.out, n, 900, heads, 2, 128, o.BF16, 0, None, 10.0, c.extra[0])
     c.cache.write(900, n, c.dev[1], c.dev[2], o.BF16)
     c.cache.read(900, n, k2, v2, o.BF16)
     g = hip.graph_end("ext")
@@ -263,7 +298,7 @@ def test_captured_and_replayed(hip, n):
 
 
 def test_the_same_call_twice_is_the_same(hip):
-    for n, ctx, kw in ((1, 3000, {}), (33, 2000, dict(softcap=8.0)), (200, 1000, {})):
+    for n, ctx, kw in ((1, 3000, {}), (33, 2000, dict(softcap=8.0)), (200, 1000, {}), (700, 900, dict(window=100))):
         c = Call(hip, np.random.default_rng(n), "nvfp4", n, ctx, 16, 4, 128)
         a = c.run(**kw)
         for _ in range(3):
