@@ -763,16 +763,15 @@ __global__ void __launch_bounds__(256) ext_pack_kernel(const void* __restrict__ 
 // [64 lanes] entries of 8 keys: A operands of v_mfma_f32_32x32x16. Lane (half, i) of a K entry has key i and dims
 // 8 half .. +8 of the step, of a V entry row i and keys 8 a + 4 half + e, 16 + 8 a + 4 half + e (e = 0 .. 3) of step
 // a = 0, 1 of a 32-key block: what the lane's scores are of. A cache's entries are these too, in another order.
-// Two K and two V buffers; positions and FP8 scales of four tiles, with the first and last position.
+// Two buffers of each, with the tiles' positions, FP8 scales and first and last position.
 template <int D>
 struct Rows {
   static constexpr int TK = D == 256 ? 32 : 64;
   static constexpr int KB = TK / 32, NS = D / 16, NB = D / 32, KS = TK / 16;
   static constexpr int kEntries = TK * D / 8;           // of K, and of V
   static constexpr int PER = kEntries / 256;            // entries a thread stages
-  static constexpr bool kAhead = D < 256;
   static constexpr int kInfo = 3 * TK + 4;              // ints of a tile's positions, scales and extremes
-  static constexpr size_t kLds = size_t(kEntries) * 64 + size_t(kInfo) * 16;
+  static constexpr size_t kLds = size_t(kEntries) * 64 + size_t(kInfo) * 8 + 2048;   // (and room to turn the output)
 };
 
 // What a thread stages of a tile: loads in flight (raw), then entries written to LDS. A cache of an odd number of 32-slot
@@ -980,10 +979,9 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a) 
   uint4* const vbuf = kbuf + 2 * R::kEntries;
   int* const info = reinterpret_cast<int*>(smem + size_t(R::kEntries) * 64);
 
-  // The tiles f .. e - 1 of one kind (S: the type of its stages). Where registers allow (kAhead), a wave's matrix ops and
-  // its vector ALUs work on different tiles at a time: while it turns tile t's scores into weights, first the products of
-  // tile t - 1 with V and then tile t + 1's scores are made. So K is in LDS two tiles ahead of V, and a barrier ends each
-  // step.
+  // The tiles f .. e - 1 of one kind (S: the type of its stages), the next one's loads in flight behind each. (Making the
+  // scores of one tile and the products of another while a third's weights are computed was no faster: what bounds a
+  // step is the reading of its tile from LDS by every wave, 128 bytes a cycle.)
   auto run = [&](auto src, auto operand, int f, int e, Span span, int span_hi_low, float global) {
     constexpr int S = decltype(src)::value;
     constexpr bool OWN = decltype(operand)::value;
@@ -1029,7 +1027,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a) 
     };
     auto store_k = [&](int t) {
       stage.store_k(kbuf + ((t - f) & 1) * R::kEntries);
-      int* lp = info + ((t - f) & 3) * R::kInfo;
+      int* lp = info + ((t - f) & 1) * R::kInfo;
       if (wave == 0) {   // the tile's last and first positions, -1 with a slot that has none
         int top = pos, least = tid < R::TK ? pos : INT_MAX;
         wave_extremes(top, least);
@@ -1047,16 +1045,15 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a) 
     auto scores = [&](int t, f32x16 (&s)[R::KB]) {
       const X8* lk = reinterpret_cast<const X8*>(kbuf + ((t - f) & 1) * R::kEntries);
 #pragma unroll
-      for (int b = 0; b < R::KB; ++b) {
+      for (int b = 0; b < R::KB; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
 #pragma unroll
-        for (int c = 0; c < R::NS; ++c) s[b] = mfma32(lk[(b * R::NS + c) * 64 + lane], q[c], s[b]);
-      }
+      for (int c = 0; c < R::NS; ++c)
+#pragma unroll
+        for (int b = 0; b < R::KB; ++b) s[b] = mfma32(lk[(b * R::NS + c) * 64 + lane], q[c], s[b]);
     };
     X8 w[R::KS];
-#pragma unroll
-    for (int k = 0; k < R::KS; ++k) w[k] = X8{};
     auto products = [&](int t) {
       const X8* lv = reinterpret_cast<const X8*>(vbuf + ((t - f) & 1) * R::kEntries);
 #pragma unroll
@@ -1067,7 +1064,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a) 
 
     // scores to y (scaled, changed, masked), m moved if they pass it; then their weights
     auto softmax_begin = [&](int t, const f32x16 (&s)[R::KB], float (&y)[R::KB][16]) {
-      const int* lp = info + ((t - f) & 3) * R::kInfo;
+      const int* lp = info + ((t - f) & 1) * R::kInfo;
       // row 8 j + r' of block b (r = 4 j + r') is key 32 b + 8 j + 4 half + r'
       const int4* lp4 = reinterpret_cast<const int4*>(lp) + half;
       const float4* lf4 = reinterpret_cast<const float4*>(lp) + half;
@@ -1121,7 +1118,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a) 
       }
     };
     auto softmax_end = [&](int t, const float (&y)[R::KB][16]) {
-      const float4* lf4 = reinterpret_cast<const float4*>(info + ((t - f) & 3) * R::kInfo) + half;
+      const float4* lf4 = reinterpret_cast<const float4*>(info + ((t - f) & 1) * R::kInfo) + half;
       const float ref = (m == -INFINITY ? 0.f : m) - kUp;
       float sum = 0.f;
 #pragma unroll
@@ -1145,6 +1142,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a) 
     };
 
     load_k(f);
+    load_v(f);
     __syncthreads();   // the buffers may still be read by what ran before
     store_k(f);
     if (a.scale < 0.f) {
@@ -1155,43 +1153,18 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a) 
     sc = score_of(a, live ? head : 0, factor * global);
     f32x16 s[R::KB];
     float y[R::KB][16];
-    if constexpr (R::kAhead) {
-      load_k(f + 1);
-#pragma unroll
-      for (int u = 0; u < R::PER; ++u) vbuf[R::kEntries + tid + u * 256] = make_uint4(0, 0, 0, 0);   // "tile f - 1"
+    store_v(f);
+    __syncthreads();
+    for (int t = f; t < e; ++t) {
+      load_k(t + 1);
+      load_v(t + 1);
+      scores(t, s);
+      softmax_begin(t, s, y);
+      softmax_end(t, y);
+      products(t);
+      store_k(t + 1);
+      store_v(t + 1);
       __syncthreads();
-      scores(f, s);
-      store_k(f + 1);
-      load_k(f + 2);
-      load_v(f);
-      __syncthreads();
-      for (int t = f; t < e; ++t) {
-        products(t - 1);
-        store_k(t + 2);
-        store_v(t);
-        load_k(t + 3);
-        load_v(t + 1);
-        softmax_begin(t, s, y);
-        scores(t + 1, s);   // (past the last tile: of the one before it, and not used)
-        softmax_end(t, y);
-        __syncthreads();
-      }
-      products(e - 1);
-    } else {
-      load_v(f);
-      store_v(f);
-      __syncthreads();
-      for (int t = f; t < e; ++t) {
-        load_k(t + 1);
-        load_v(t + 1);
-        scores(t, s);
-        softmax_begin(t, s, y);
-        softmax_end(t, y);
-        products(t);
-        store_k(t + 1);
-        store_v(t + 1);
-        __syncthreads();
-      }
     }
   };
   run(std::integral_constant<int, T>{}, std::false_type{}, n.c_first, n.c_end, cached_span(a, all),
@@ -1207,24 +1180,48 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a) 
   l = xor32_sum(l);
   if (a.splits == 1) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const size_t out = (size_t(row) * size_t(a.heads) + size_t(head)) * D;
     bool bad = false;
-    if (live) {
 #pragma unroll
-      for (int d = 0; d < R::NB; ++d)
+    for (int d = 0; d < R::NB; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int v = 32 * d + 8 * (r >> 2) + 4 * half + (r & 3);
-          const size_t at = out + size_t(Tile<D, T>::dim(v >> 4, v & 15));
-          bad |= not_finite(acc[d][r]);
-          if (a.bf16)
-            static_cast<__bf16*>(a.out)[at] = (__bf16)(acc[d][r] * inv);
-          else
-            static_cast<float*>(a.out)[at] = acc[d][r] * inv;
-        }
-    }
-    const uint64_t any = __ballot(bad && !not_finite(l));
+      for (int r = 0; r < 16; ++r) bad |= live && not_finite(acc[d][r]);
+    const long long out = live ? (long long)((size_t(row) * size_t(a.heads) + size_t(head)) * D) : -1;
     __syncthreads();   // the last tile's buffer, and bounds
+    // a lane has a q-col's values 512 bytes or more from its neighbour's: they are turned in LDS, a wave its own 32 rows
+    auto write = [&](auto* to) {
+      using X = std::remove_pointer_t<decltype(to)>;
+      constexpr int DP = sizeof(X) == 4 && D > 128 ? 128 : D, PITCH = DP + 16 / int(sizeof(X));   // dims of a pass
+      static_assert(kExtWaves * 32 * PITCH * sizeof(X) <= R::kLds, "the tiles' buffers hold the rows");
+      X* mine = reinterpret_cast<X*>(smem) + wave * 32 * PITCH;
+#pragma unroll
+      for (int p = 0; p < D; p += DP) {
+        if (p) __syncthreads();
+#pragma unroll
+        for (int d = 0; d < R::NB; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int v = 32 * d + 8 * (r >> 2) + (r & 3);   // and 4 half
+            const int low = Tile<D, T>::dim(v >> 4, v & 15), step = Tile<D, T>::dim(0, 4) - Tile<D, T>::dim(0, 0);
+            if (low < p || low >= p + DP) continue;   // (with half = 1 on the same side)
+            mine[(lane & 31) * PITCH + low - p + half * step] = X(acc[d][r] * inv);
+          }
+        __syncthreads();
+        constexpr int CH = DP * int(sizeof(X)) / 16, PER = 64 / CH;   // 16-byte pieces of a row; rows at a time
+#pragma unroll
+        for (int c = 0; c < 32; c += PER) {
+          const int of = c + lane / CH, piece = lane % CH;
+          const int lo32 = __shfl(int(uint32_t(out)), of), hi32 = __shfl(int(out >> 32), of);
+          if (hi32 < 0) continue;
+          const size_t at = (size_t(uint32_t(hi32)) << 32 | size_t(uint32_t(lo32))) + size_t(p);
+          reinterpret_cast<uint4*>(to + at)[piece] = reinterpret_cast<const uint4*>(mine + of * PITCH)[piece];
+        }
+      }
+    };
+    if (a.bf16)
+      write(static_cast<__bf16*>(a.out));
+    else
+      write(static_cast<float*>(a.out));
+    const uint64_t any = __ballot(bad && !not_finite(l));
     if (lane == 0) bounds[wave][0] = int(uint32_t(any) | uint32_t(any >> 32));
     __syncthreads();
     for (int w = 0; w < kExtWaves; ++w)
