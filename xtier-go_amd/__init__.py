@@ -246,6 +246,7 @@ class HipBackend:
         self.h = lib().xtg_hip_open(json.dumps({"device": device}).encode(), err, len(err))
         if not self.h:
             raise XtgError(err.value.decode(errors="replace"))
+        self._err = _errbuf()   # of the calls that a decode step makes for every layer (one thread at a time)
         # Prepared weights are keyed by the address of their codes (as in the reference); every Weight passed in
         # is kept alive here so that no later array can reuse an address that still names a prepared copy.
         self._weights = {}
@@ -467,7 +468,7 @@ class HipBackend:
         a = AttnExt(n_q, pos0, heads, kv_heads, head_dim, window, sc, _ptr(q), _ptr(k), _ptr(v),
                     cache.h if cache is not None else None, _ptr(out), x_dtype, softcap, _ptr(slopes), _ptr(first),
                     _ptr(end))
-        err = _errbuf()
+        err = self._err
         _check(lib().xtg_hip_attention_ext(self.h, ctypes.byref(a), err, len(err)), err)
 
     # ---- the Dory decode step
@@ -615,13 +616,13 @@ class KvCache:
 
     def write(self, pos, n, k, v, x_dtype=X_F32):
         """store for device rows of x_dtype (queued)."""
-        err = _errbuf()
+        err = self.b._err
         _check(lib().xtg_hip_kv_write(self.b.h, self.h, pos, n, _ptr(k), _ptr(v), x_dtype, err, len(err)), err)
 
     def read(self, pos, n, k, v, x_dtype=X_F32):
         """The rows of positions pos .. pos + n - 1 as the cache holds them into device k, v [n][kv_heads][head_dim] of
         x_dtype, zeros where it holds none (queued)."""
-        err = _errbuf()
+        err = self.b._err
         _check(lib().xtg_hip_kv_read(self.b.h, self.h, pos, n, _ptr(k), _ptr(v), x_dtype, err, len(err)), err)
 
     def store_host(self, pos, k, v):

@@ -40,8 +40,35 @@ struct ExtPlan {
 };
 ExtPlan ext_plan(const ExtCall& a, int cus);
 
+constexpr int kBf16 = 0, kFp8 = 1, kNvfp4 = 2;   // XTG_KV_*
+constexpr int kExtWaves = 4;                     // waves of a work-group
+
+// What the kernels take.
+struct ExtArgs {
+  const void *q, *k, *v;
+  void* out;
+  const uint8_t *ck, *cv;
+  const void *ks, *vs;
+  const int* slot_pos;
+  const uint4 *pk, *pv;          // packed own keys and values
+  float *acc, *ml;               // records [block][KV head][split][cols][d], [..][2]; row r of product dd at 16 dd + r
+  int slots_pad, tile_lo, tiles;
+  int ring, splits, records, cols, own;   // splits of the cached keys (few) or of all keys; own keys: their number
+  int n_q, pos0, heads, group, window, bf16;
+  uint32_t group_inv;            // ceil(2^16 / group): (col * group_inv) >> 16 is col / group for col < 256
+  int cached_end;                // cached positions from here on are not seen
+  float scale, kglobal, vglobal, softcap;
+  const float* slopes;
+  const int* first;
+  const int* end;
+};
+
 // Queues the call's launches on scratch of the plan's size, each a callable that returns its name, given to `timed`.
 using Timed = std::function<void(const std::function<std::string()>&)>;
 void launch_attn_ext(const ExtCall& a, const ExtPlan& p, void* scratch, hipStream_t stream, const Timed& timed);
+
+// The launches for heads of D dims (64, 128, 256) over a cache of `dtype`.
+template <int D>
+void ext_launch(const ExtCall& c, const ExtPlan& p, const ExtArgs& a, int dtype, hipStream_t stream, const Timed& timed);
 
 }  // namespace xtg::hip

@@ -7,7 +7,7 @@
 // stay.
 #include <algorithm>
 
-#include "attention.hpp"
+#include "attention_ext.hpp"
 #include "common.hpp"
 #include "kv4.hpp"
 
@@ -324,8 +324,6 @@ struct ReadArgs {
   int t0, tiles, total_tiles;   // first tile, tiles to visit (laps of a ring counted again), the cache's tiles
   float kglobal, vglobal;
 };
-
-constexpr int kBf16 = 0, kFp8 = 1, kNvfp4 = 2;   // XTG_KV_*
 
 // Every row of the call is one work-group's to write, zeros included: a tile is visited once for every lap of the ring
 // that the rows take. NVFP4 is dealt as the store deals it; BF16 and FP8 by 16-byte words, a wave a tile.
