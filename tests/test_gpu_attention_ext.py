@@ -297,6 +297,44 @@ def test_captured_and_replayed(hip, n, heads):
     other.free()
 
 
+@pytest.mark.parametrize("n,heads", [(1, 8), (20, 8), (45, 64)])
+def test_the_last_positions(hip, n, heads):
+    """Rows up to position 2^31 - 2, over a ring and over their own keys alone."""
+    rng, pos0, ring = np.random.default_rng(n), 2 ** 31 - 1 - n, 96
+    c = Call(hip, rng, "nvfp4", n, 0, heads, 2, 128, ring)
+    kc, vc = Call.unit(rng, (ring, 2, 128)), rng.standard_normal((ring, 2, 128)).astype(np.float32)
+    c.fill(pos0 - ring, kc, vc)
+    own = c.keys
+    c.keys = [np.concatenate([a, b]) for a, b in zip(o.stored_pair(kc, vc, "nvfp4"), own)]
+    c.ctx, c.at = pos0, pos0 - ring + np.arange(ring + n)
+    c.check(window=90)
+    c.check(end=np.full(n, 2 ** 31 - 1), softcap=5.0)
+    c.cache.destroy()
+    c.cache, c.keys, c.at = None, own, pos0 + np.arange(n)
+    c.check()
+    c.free()
+
+
+def test_a_chunk_of_many_blocks(hip):
+    """More blocks of rows than the second axis of a grid has (65535): the rows' keys repeat, so that each full window
+    gives what a short call gives."""
+    n, heads, d, w = 131100, 64, 64, 7
+    rng = np.random.default_rng(1)
+    k, v = (np.tile(rng.standard_normal((w, 1, d)).astype(np.float32), (n // w + 1, 1, 1))[:n] for _ in range(2))
+    q = Call.unit(rng, (1, heads, d)) * np.float32(d)
+    dev = [hip.array(o.rows(x, o.BF16)[0]) for x in (np.repeat(q, n, 0), k, v)]
+    out = hip.array(shape=(n, heads, d), dtype=np.uint16)
+    hip.attention_ext(None, *dev, out, n, 0, heads, 1, d, o.BF16, w)
+    got = out.numpy()
+    ref, size, most = o.attend(o.bf16(q), o.bf16(k[:w]), o.bf16(v[:w]), np.arange(w), w - 1, d ** -0.5, w)
+    tol = o.tolerance(ref, size, most, d, 8, o.BF16)
+    for at in range(w - 1, n, 8192):
+        rows = o.bf16_values(got[at:at + 8192])
+        assert (np.abs(rows - ref) <= tol).all(), at
+    for x in dev + [out]:
+        x.free()
+
+
 def test_the_same_call_twice_is_the_same(hip):
     for n, ctx, kw in ((1, 3000, {}), (33, 2000, dict(softcap=8.0)), (200, 1000, {}), (700, 900, dict(window=100))):
         c = Call(hip, np.random.default_rng(n), "nvfp4", n, ctx, 16, 4, 128)
@@ -361,7 +399,7 @@ def test_refusals(hip, pkg):
                          (dict(out=None), "NULL"), (dict(k=None), "both, or neither"), (dict(v=None), "both, or neither"),
                          (dict(cache=None, k=None, v=None), "neither"), (dict(kv_heads=4), "cache of"),
                          (dict(head_dim=64), "cache of"), (dict(q=a.ptr + 8), "16-byte"), (dict(out=a.ptr + 4), "16-byte"),
-                         (dict(first=a.ptr + 2), "4-byte")]:
+                         (dict(first=a.ptr + 2), "4-byte"), (dict(n_q=2 ** 27 + 1), "rows of")]:
         with pytest.raises(pkg.XtgError, match=what):
             hip.attention_ext(**dict(good, **change))
     other = hip.kv_cache(2, 128, 64, 0, 2)

@@ -563,14 +563,14 @@ __global__ void __launch_bounds__(kExtWaves * 64, QB * D > 256 ? 1 : 2) ext_few_
     FewQueries<D, QB, OwnTile<D, T>> rows;
     rows.load(a, h, col0, lane);
     rows.operand(a, 1.f, q);
-    const int t = (split - a.splits) * kExtWaves + wave, p = a.pos0 + 32 * t, past = a.pos0 + a.own;
+    const int t = (split - a.splits) * kExtWaves + wave, p = a.pos0 + 32 * t;   // (p + 32 can pass 2^31)
     bool any = false;   // a q-col that sees one of the tile's keys
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb)
-      any |= rows.span[qb].len > 0 && rows.span[qb].lo < p + 32 && int(rows.span[qb].len) > p - rows.span[qb].lo;
+      any |= rows.span[qb].len > 0 && rows.span[qb].lo - 32 < p && int(rows.span[qb].len) > p - rows.span[qb].lo;
     if (32 * t < a.own && __ballot(any)) {
       OwnTile<D, T> tile(a, h, kv_heads, t, lane);
-      auto at = [&](int e) { return p + 4 * g + e < past ? p + 4 * g + e : -1; };
+      auto at = [&](int e) { return 32 * t + 4 * g + e < a.own ? p + 4 * g + e : -1; };
       few_tile<D, QB, MOD>(a, tile, q, rows.span, rows.sc, st, make_int4(at(0), at(1), at(2), at(3)),
                            make_int4(at(16), at(17), at(18), at(19)), [] {}, [] {});
     }
@@ -937,13 +937,13 @@ __device__ inline KeyTiles key_tiles(const ExtArgs& a, Span all, int (&bounds)[W
 }
 
 template <int D, int T, int MOD>
-__global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a) {
+__global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, int kv_heads) {
   using R = Rows<D>;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   __shared__ int bounds[kExtWaves][2];
   const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6, half = lane >> 5;
-  const int h = int(blockIdx.x), kv_heads = int(gridDim.x), block = int(gridDim.y) - 1 - int(blockIdx.y);
-  const int split = int(blockIdx.z);   // later rows, which see most, first
+  const int h = int(blockIdx.x) % kv_heads, block = (int(gridDim.x) - 1 - int(blockIdx.x)) / kv_heads;   // later rows,
+  const int split = int(blockIdx.y);                                                                  // which see most, first
   const int col = block * 128 + wave * 32 + (lane & 31), row = col / a.group, head = h * a.group + col % a.group;
   const bool live = row < a.n_q;
 
@@ -1350,10 +1350,10 @@ void launch(const ExtCall& c, const ExtPlan& p, const ExtArgs& a, hipStream_t st
         return strf("ext_pack_kernel<%d, %d>", D, T);
       });
     timed([&] {
-      const dim3 grid{unsigned(c.kv_heads), unsigned(p.blocks), unsigned(p.splits)};
+      const dim3 grid{unsigned(c.kv_heads) * unsigned(p.blocks), unsigned(p.splits)};
       const size_t lds = Rows<D>::kLds;
       allow_lds(reinterpret_cast<const void*>(&ext_rows_kernel<D, T, MOD>), lds);
-      hipLaunchKernelGGL((ext_rows_kernel<D, T, MOD>), grid, dim3(kExtWaves * 64), lds, stream, a);
+      hipLaunchKernelGGL((ext_rows_kernel<D, T, MOD>), grid, dim3(kExtWaves * 64), lds, stream, a, c.kv_heads);
       HIP_CHECK(hipGetLastError());
       return strf("ext_rows_kernel<%d, %d, %d>", D, T, MOD);
     });

@@ -66,7 +66,12 @@ void Backend::ensure(void*& buf, size_t& size, size_t need) {
     buf = nullptr;
     size = 0;
   }
-  HIP_CHECK(hipMalloc(&buf, need));
+  int current = device_;
+  HIP_CHECK(hipGetDevice(&current));
+  if (current != device_) HIP_CHECK(hipSetDevice(device_));
+  const hipError_t got = hipMalloc(&buf, need);
+  if (current != device_) HIP_CHECK(hipSetDevice(current));
+  HIP_CHECK(got);
   size = need;
 }
 
@@ -680,7 +685,7 @@ void Backend::attention_ext(const ExtCall& a) {
   XTG_CHECK(a.d == 64 || a.d == 128 || a.d == 256, "attention_ext: head_dim %d (64, 128 or 256)", a.d);
   XTG_CHECK(a.kv_heads >= 1 && a.heads >= 1 && a.heads % a.kv_heads == 0 && a.kv_heads < 65536,
             "attention_ext: %d heads over %d KV heads", a.heads, a.kv_heads);
-  XTG_CHECK((long long)a.n_q * (a.heads / a.kv_heads) < (1LL << 31), "attention_ext: %d rows of %d heads", a.n_q, a.heads);
+  XTG_CHECK((long long)a.n_q * a.heads <= (1LL << 30), "attention_ext: %d rows of %d heads (2^30 at most)", a.n_q, a.heads);
   XTG_CHECK(a.x_dtype == kXF32 || a.x_dtype == kXBF16, "attention_ext: unknown row type %d", a.x_dtype);
   XTG_CHECK(std::isfinite(a.scale), "attention_ext: scale %g", double(a.scale));
   XTG_CHECK(std::isfinite(a.softcap) && a.softcap >= 0.f, "attention_ext: softcap %g", double(a.softcap));

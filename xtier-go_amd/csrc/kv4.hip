@@ -2,9 +2,10 @@
 //
 // Both are bound by HBM for many rows, and by latency for few: 64 to 256 threads take a (KV head, 32-slot tile), so that
 // a decoded token's rows are one step of a few loads in each. Of K a thread takes a few dims of a key, rows read as they
-// lie; of V a few dims of 8 keys, so that it reads and writes whole words of codes. Of a call's rows a tile's slots hold the ones at their positions; a ring's last rows and first rows can share a tile,
-// which is still one work-group's in a store, since a V word holds the codes of 8 slots and the nibbles of other rows
-// stay.
+// lie; of V a few dims of 8 keys, so that it reads and writes whole words of codes. A ring's last rows and first rows can
+// share a tile, which is still one work-group's in a store, since a V word holds the codes of 8 slots and the nibbles of
+// other rows stay. 32749 BF16 rows of 8 heads of 128 dims written and then read: 81 us for 344 MB, 4.2 TB/s (a copy of
+// 4 GB reaches 4.7); one row 9.3, which is the two calls' queueing.
 #include <algorithm>
 
 #include "attention_ext.hpp"
@@ -254,7 +255,7 @@ template <int D, class X>
 __global__ void __launch_bounds__(256) kv_store4_kernel(Store4Args a) {
   constexpr int NT = Deal4<D, true>::NT;
   __shared__ uint32_t not_finite[256 / NT];   // a tile's slots
-  const int w = (int(blockIdx.x) * 256 + int(threadIdx.x)) / NT;
+  const int w = int(blockIdx.x) * (256 / NT) + int(threadIdx.x) / NT;
   const bool in = w < a.tiles * a.kv_heads;   // (threads past the end wait for the others)
   const int h = w % a.kv_heads, t = in ? (a.t0 + w / a.kv_heads) % a.total_tiles : 0;
   if (threadIdx.x < 256 / NT) not_finite[threadIdx.x] = 0;
@@ -330,7 +331,7 @@ struct ReadArgs {
 template <int D, int T, class X>
 __global__ void __launch_bounds__(256) kv_read_kernel(ReadArgs a) {
   constexpr int NT = T == kNvfp4 ? Deal4<D, false>::NT : 64;
-  const int w = (int(blockIdx.x) * 256 + int(threadIdx.x)) / NT;
+  const int w = int(blockIdx.x) * (256 / NT) + int(threadIdx.x) / NT;
   if (w >= a.tiles * a.kv_heads) return;
   const int h = w % a.kv_heads, u = a.t0 + w / a.kv_heads, lap = u / a.total_tiles, t = u % a.total_tiles;
   const long long p0 = a.base + (long long)lap * a.slots;   // slot s holds position p0 + s in this lap
