@@ -15,9 +15,10 @@
 //     and more of them take the call's own keys. One row is bound by the cache's bytes (32768 NVFP4 keys of 8 heads of 128
 //     dims: 9 us for 38 MB, 4.2 TB/s), more rows by the vector ALUs (a tile is dequantised for every 32 q-cols).
 //   ext_rows_kernel: more q-cols (a prompt chunk). Four waves of 32 q-cols share tiles through LDS: each is dequantised
-//     once per work-group. The call's own keys are packed as BF16 tiles first (ext_pack_kernel). Bound by LDS: every wave
-//     reads every tile, 128 bytes a cycle and CU (512 rows over 16384 keys, 32 / 8 heads of 128 dims: 156 us, 0.89 PFLOP/s;
-//     heads of 256 dims, whose q does not stay in registers, 0.43).
+//     once per work-group. The call's own keys are packed as BF16 tiles first (ext_pack_kernel). Bound by what a SIMD issues:
+//     the matrix ops of its two waves (36 % of the time at 2.1 GHz) and their vector ALU work (50 %: exponentials, masks,
+//     dequantisation) hardly overlap, while LDS is busy for 28 %. 512 rows over 16384 NVFP4 keys, 32 / 8 heads of 128 dims:
+//     154 us, 0.9 PFLOP/s; 1500 capped rows over 2500 keys, 16 / 4 heads of 256 dims: 93 us, 0.52.
 //   ext_merge_kernel: joins the records of a q-col in their order.
 //
 // Values that are not finite: a score that is masked is replaced, so a key's only reach the q-cols that see it. Not so a
@@ -165,8 +166,8 @@ struct Score {
 };
 __device__ inline Score score_of(const ExtArgs& a, int head, float factor) {
   Score s;
-  s.f = fabsf(a.scale) * factor * (a.softcap > 0.f ? 2.f * kLog2e / a.softcap : kLog2e);
-  s.top = a.softcap * kLog2e;
+  s.f = fmaxf(fabsf(a.scale) * factor * (a.softcap > 0.f ? 2.f * kLog2e / a.softcap : kLog2e), FLT_MIN);
+  s.top = fmaxf(a.softcap * kLog2e, FLT_MIN);   // (not zero: times an infinity they are one)
   s.slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
   return s;
 }
@@ -179,6 +180,22 @@ __device__ inline float changed(const Score& s, float qk, int dist) {
   if (MOD & kCap) y = fmaf(-2.f * s.top, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y) + 1.f), s.top);
   if (MOD & kBias) y = fmaf(-s.slope, fabsf(float(dist)), y);
   return y;
+}
+
+// A score in two steps: begun for every key (masked(): where it is not seen), and from the best of them for the maximum
+// (best: the score is monotone in it) or inside the exponential, finish(x, minus) = score - minus in one operation.
+template <int MOD>
+__device__ inline float begin(const Score& s, float qk, int dist) {
+  if (MOD == kCap) return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(qk * s.f) + 1.f);
+  return MOD ? changed<MOD>(s, qk, dist) : qk;
+}
+template <int MOD>
+__device__ inline float masked() { return MOD == kCap ? INFINITY : -INFINITY; }
+template <int MOD>
+__device__ inline float best(float a, float b) { return MOD == kCap ? fminf(a, b) : fmaxf(a, b); }
+template <int MOD>
+__device__ inline float finish(const Score& s, float x, float minus) {
+  return MOD == kCap ? fmaf(-2.f * s.top, x, s.top - minus) : MOD ? x - minus : fmaf(x, s.f, -minus);
 }
 
 __device__ inline bool not_finite(float x) { return !(fabsf(x) <= FLT_MAX); }
@@ -754,7 +771,8 @@ struct Rows {
   static constexpr int kEntries = TK * D / 8;           // of K, and of V
   static constexpr int PER = kEntries / 256;            // entries a thread stages
   static constexpr int kInfo = 3 * TK + 4;              // ints of a tile's positions, scales and extremes
-  static constexpr size_t kLds = size_t(kEntries) * 64 + size_t(kInfo) * 8 + 2048;   // (and room to turn the output)
+  static constexpr size_t kLds = size_t(kEntries) * 64 + size_t(kInfo) * 8 + 2048 + (D == 256 ? 2 * 4096 : 0);
+  // (and room to turn the output; for heads of 256 dims, for two chunks of q)
 };
 
 // What a thread stages of a tile: loads in flight (raw), then entries written to LDS. A cache of an odd number of 32-slot
@@ -774,6 +792,26 @@ struct Stage<D, kBf16> {
   }
   __device__ void load_k(const uint4* ck, int h, int pad, int tile, bool half) { load(k, ck, h, pad, tile, half); }
   __device__ void load_v(const uint4* cv, int h, int pad, int tile, bool half) { load(v, cv, h, pad, tile, half); }
+  // The tile straight into its place in LDS: 64 entries a wave's load, a lane's the one that comes to its part of them.
+  __device__ static void direct(const uint4* c, int h, int pad, int tile, uint4* to, bool v) {
+    const uint4* from = c + (size_t(h) * size_t(pad) + size_t(tile) * R::TK) * (D / 8);
+    const int lane = int(threadIdx.x) & 63, half = lane >> 5, i = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+#pragma unroll
+    for (int u = 0; u < R::PER; ++u) {
+      const int row = u * 4 + wave;   // of 64 entries
+      int x;
+      if (v) {
+        const int dd = row / R::KS * 2 + (i >> 4), ks = row % R::KS;
+        x = (ks >> 1) * 4 * D + dd * 64 + ((ks & 1) * 2 + half) * 16 + (i & 15);
+      } else {
+        const int b = row / R::NS * 2 + (i >> 4), st = row % R::NS;
+        x = b * 2 * D + (st >> 1) * 64 + ((st & 1) * 2 + half) * 16 + (i & 15);
+      }
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + x),
+                                       (__attribute__((address_space(3))) void*)(to + row * 64), 16, 0, 0);
+    }
+  }
   // entry x of a BF16 tile of TK keys to its place
   __device__ static int k_place(int x) {
     const int b = x / (2 * D), c = x / 64 % (D / 32), g = x >> 4 & 3, i = x & 15;
@@ -963,14 +1001,16 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
   int* const info = reinterpret_cast<int*>(smem + size_t(R::kEntries) * 64);
 
   // The tiles f .. e - 1 of one kind (S: the type of its stages), the next one's loads in flight behind each. (Making the
-  // scores of one tile and the products of another while a third's weights are computed was no faster: what bounds a
-  // step is the reading of its tile from LDS by every wave, 128 bytes a cycle.)
+  // scores of one tile and the products of another while a third's weights are computed was no faster, nor reading LDS
+  // further ahead, nor priorities or a delay between the two work-groups of a CU.)
   auto run = [&](auto src, auto operand, int f, int e, Span span, int span_hi_low, float global) {
     constexpr int S = decltype(src)::value;
     constexpr bool OWN = decltype(operand)::value;
     using X8 = typename OperandOf<S>::type;
     if (f >= e) return;
     X8 q[R::NS];
+    constexpr int QL = D == 256 && S != kBf16 ? 2 : 0;   // chunks of q in LDS, for the same reason
+    X8* const ql = reinterpret_cast<X8*>(smem + R::kLds - 4096 * QL) + wave * 64 + lane;
     Score sc;
     bf16x8 x[R::NS];
     row_chunks(a.q, a.bf16, live, [&](int c) { return (live ? q_at : size_t(8 * half)) + size_t(16 * c); }, x);
@@ -978,16 +1018,25 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
     int pos = -1;
     float ks = 0.f, vs = 0.f;
     auto half_tile = [&](int t) { return !OWN && R::TK == 64 && t * 64 + 32 == a.slots_pad; };
+    // BF16 tiles of 256 dims, whose stages do not fit beside q and the accumulators, go from memory to LDS directly (with
+    // registers spilled, each of their reloads waited for the tile's loads: 115 us, now 93, of the case above; heads of 128
+    // dims, whose stages fit, took 39.5 us so and 40.7 directly)
+    constexpr bool kDirect = D == 256 && S == kBf16;
+    const int rows_pad = OWN ? (a.own + 63) / 64 * 64 : a.slots_pad;
     auto load_k = [&](int t) {
+      if constexpr (kDirect) {   // (past the last: nothing)
+        if (t < e)
+          stage.direct(OWN ? a.pk : reinterpret_cast<const uint4*>(a.ck), h, rows_pad, t, kbuf + ((t - f) & 1) * R::kEntries, false);
+      }
       t = min(t, e - 1);   // past the last: loaded again, and not used
       pos = -1;
       if constexpr (OWN) {
-        stage.load_k(a.pk, h, (a.own + 63) / 64 * 64, t, false);
+        if constexpr (!kDirect) stage.load_k(a.pk, h, rows_pad, t, false);
         if (tid < R::TK && t * R::TK + tid < a.own) pos = a.pos0 + t * R::TK + tid;
       } else {
         if constexpr (S == kNvfp4)
           stage.load_k(a, h, t, half_tile(t));
-        else
+        else if constexpr (!kDirect)
           stage.load_k(reinterpret_cast<const uint4*>(a.ck), h, a.slots_pad, t, half_tile(t));
         if (tid < (half_tile(t) ? 32 : R::TK)) {
           pos = a.slot_pos[t * R::TK + tid];
@@ -1000,16 +1049,21 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
       }
     };
     auto load_v = [&](int t) {
+      if constexpr (kDirect) {
+        if (t < e)
+          stage.direct(OWN ? a.pv : reinterpret_cast<const uint4*>(a.cv), h, rows_pad, t, vbuf + ((t - f) & 1) * R::kEntries, true);
+        return;
+      }
       t = min(t, e - 1);
       if constexpr (OWN)
-        stage.load_v(a.pv, h, (a.own + 63) / 64 * 64, t, false);
+        stage.load_v(a.pv, h, rows_pad, t, false);
       else if constexpr (S == kNvfp4)
         stage.load_v(a, h, t, half_tile(t));
       else
         stage.load_v(reinterpret_cast<const uint4*>(a.cv), h, a.slots_pad, t, half_tile(t));
     };
     auto store_k = [&](int t) {
-      stage.store_k(kbuf + ((t - f) & 1) * R::kEntries);
+      if constexpr (!kDirect) stage.store_k(kbuf + ((t - f) & 1) * R::kEntries);
       int* lp = info + ((t - f) & 1) * R::kInfo;
       if (wave == 0) {   // the tile's last and first positions, -1 with a slot that has none
         int top = pos, least = tid < R::TK ? pos : INT_MAX;
@@ -1024,7 +1078,12 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
         }
       }
     };
-    auto store_v = [&](int t) { stage.store_v(vbuf + ((t - f) & 1) * R::kEntries); };
+    auto store_v = [&](int t) {
+      if constexpr (kDirect)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the tile's loads into LDS, before the barrier behind
+      else
+        stage.store_v(vbuf + ((t - f) & 1) * R::kEntries);
+    };
     auto scores = [&](int t, f32x16 (&s)[R::KB]) {
       const X8* lk = reinterpret_cast<const X8*>(kbuf + ((t - f) & 1) * R::kEntries);
 #pragma unroll
@@ -1034,7 +1093,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
 #pragma unroll
       for (int c = 0; c < R::NS; ++c)
 #pragma unroll
-        for (int b = 0; b < R::KB; ++b) s[b] = mfma32(lk[(b * R::NS + c) * 64 + lane], q[c], s[b]);
+        for (int b = 0; b < R::KB; ++b) s[b] = mfma32(lk[(b * R::NS + c) * 64 + lane], c < R::NS - QL ? q[c] : ql[(c - R::NS + QL) * 256], s[b]);
     };
     X8 w[R::KS];
     auto products = [&](int t) {
@@ -1045,7 +1104,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
         for (int d = 0; d < R::NB; ++d) acc[d] = mfma32(lv[(d * R::KS + k) * 64 + lane], w[k], acc[d]);
     };
 
-    // scores to y (scaled, changed, masked), m moved if they pass it; then their weights
+    // scores begun (masked) in y, m moved if they pass it; then their weights
     auto softmax_begin = [&](int t, const f32x16 (&s)[R::KB], float (&y)[R::KB][16]) {
       const int* lp = info + ((t - f) & 1) * R::kInfo;
       // row 8 j + r' of block b (r = 4 j + r') is key 32 b + 8 j + 4 half + r'
@@ -1067,7 +1126,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            y[b][4 * j + r] = changed<MOD>(sc, S == kFp8 ? s[b][4 * j + r] * k4[r] : s[b][4 * j + r], span.t - p[r]);
+            y[b][4 * j + r] = begin<MOD>(sc, S == kFp8 ? s[b][4 * j + r] * k4[r] : s[b][4 * j + r], span.t - p[r]);
         }
       // the tile's positions against what the wave's q-cols see: all, or a mask
       const int top = __builtin_amdgcn_readfirstlane(lp[3 * R::TK]), least = __builtin_amdgcn_readfirstlane(lp[3 * R::TK + 1]);
@@ -1080,15 +1139,15 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
             const int p[4] = {p4.x, p4.y, p4.z, p4.w};
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (uint32_t(p[r] - span.lo) >= span.len) y[b][4 * j + r] = -INFINITY;
+              if (uint32_t(p[r] - span.lo) >= span.len) y[b][4 * j + r] = masked<MOD>();
           }
       }
-      float mx = -INFINITY;
+      float mx = masked<MOD>();
 #pragma unroll
       for (int b = 0; b < R::KB; ++b)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, y[b][r]);
-      mx = xor32_max(mx);
+        for (int r = 0; r < 16; ++r) mx = best<MOD>(mx, y[b][r]);
+      mx = xor32_max(finish<MOD>(sc, mx, 0.f));
       if (__ballot(mx > m + kSlack)) {
         const float to = mx > m + kSlack ? mx : m;
         const float corr = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.f : to));
@@ -1115,7 +1174,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            float p = __builtin_amdgcn_exp2f(y[b][4 * j + r] - ref);
+            float p = __builtin_amdgcn_exp2f(finish<MOD>(sc, y[b][4 * j + r], ref));
             sum += p;
             if constexpr (S == kFp8) p *= v4[r];
             w[2 * b + (j & 1)][(j >> 1) * 4 + r] = p;
@@ -1124,9 +1183,10 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
       l += sum;
     };
 
+    if constexpr (kDirect) __syncthreads();
     load_k(f);
     load_v(f);
-    __syncthreads();   // the buffers may still be read by what ran before
+    if constexpr (!kDirect) __syncthreads();   // the buffers may still be read by what ran before
     store_k(f);
     if (a.scale < 0.f) {
 #pragma unroll
@@ -1134,6 +1194,8 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
     }
     const float factor = to_operand(x, q, [](float y) { return xor32_max(y); });
     sc = score_of(a, live ? head : 0, factor * global);
+#pragma unroll
+    for (int c = 0; c < QL; ++c) ql[c * 256] = q[R::NS - QL + c];
     f32x16 s[R::KB];
     float y[R::KB][16];
     store_v(f);
