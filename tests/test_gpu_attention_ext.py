@@ -237,6 +237,15 @@ def test_scales_and_sharp_softmaxes(hip, scale, n, heads):
     c.free()
 
 
+@pytest.mark.parametrize("size", [2.0 ** -127, 2.0 ** -100, 2.0 ** 40])
+@pytest.mark.parametrize("n,heads", [(2, 8), (26, 64)])
+def test_tiny_and_huge_queries(hip, size, n, heads):
+    """Queries near both ends of BF16's exponents: scores that vanish, and scores of one at a scale that undoes them."""
+    c = Call(hip, np.random.default_rng(n), "nvfp4", n, 300, heads, 2, 128, spread=size)
+    c.check(scale=128 ** -0.5 if size < 1 else 2.0 ** -46)
+    c.free()
+
+
 @pytest.mark.parametrize("dtype", ["nvfp4", "bf16", "fp8"])
 @pytest.mark.parametrize("n,heads", [(1, 8), (6, 8), (70, 8), (26, 64)])
 def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(hip, dtype, n, heads):

@@ -95,7 +95,7 @@ __device__ inline float to_operand(const bf16x8 (&x)[N], f16x8 (&q)[N], J join) 
 #pragma unroll
     for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint((float)x[c][e]) & 0x7fffffffu);
   m = __float_as_uint(join(__uint_as_float(m & 0xff800000u)));   // powers of two, or infinity: ordered as floats
-  const int ex = m == 0u || m >= 0x7f800000u ? 0 : int(m >> 23) - 127 - 8;
+  const int ex = m == 0u || m >= 0x7f800000u ? 0 : max(int(m >> 23) - 127 - 8, -126);   // (2^-ex is finite)
   const float down = ldexpf(1.f, -ex);
 #pragma unroll
   for (int c = 0; c < N; ++c)
