@@ -230,7 +230,7 @@ typedef struct xtg_attn_ext {
   const xtg_hip_kv* cache;
   void* out;              /* device [n_q][heads][head_dim] */
   int x_dtype;            /* XTG_X_F32 or XTG_X_BF16, of q, k, v and out */
-  float softcap;          /* 0: none */
+  float softcap;          /* 0: none; up to 1024 */
   const float* slopes;    /* device [heads], or NULL */
   const int32_t* first;   /* device [n_q], or NULL */
   const int32_t* end;     /* device [n_q], or NULL */

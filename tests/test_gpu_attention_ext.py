@@ -237,6 +237,14 @@ def test_scales_and_sharp_softmaxes(hip, scale, n, heads):
     c.free()
 
 
+@pytest.mark.parametrize("cap", [1e-38, 1e-3, 1024.0])
+@pytest.mark.parametrize("n,heads", [(2, 8), (26, 64)])
+def test_tiny_and_large_caps(hip, cap, n, heads):
+    c = Call(hip, np.random.default_rng(n), "nvfp4", n, 300, heads, 2, 128)
+    c.check(softcap=cap)
+    c.free()
+
+
 @pytest.mark.parametrize("size", [2.0 ** -127, 2.0 ** -100, 2.0 ** 40])
 @pytest.mark.parametrize("n,heads", [(2, 8), (26, 64)])
 def test_tiny_and_huge_queries(hip, size, n, heads):
@@ -404,7 +412,7 @@ def test_refusals(hip, pkg):
     for change, what in [(dict(n_q=0), "rows at"), (dict(pos0=-1), "rows at"), (dict(pos0=2 ** 31 - 2), "rows at"),
                          (dict(head_dim=96), "head_dim"), (dict(kv_heads=3), "heads over"), (dict(kv_heads=0), "heads over"),
                          (dict(heads=0), "heads over"), (dict(x_dtype=2), "row type"), (dict(scale=float("inf")), "scale"),
-                         (dict(softcap=-1.0), "softcap"), (dict(softcap=float("nan")), "softcap"), (dict(q=None), "NULL"),
+                         (dict(softcap=-1.0), "softcap"), (dict(softcap=float("nan")), "softcap"), (dict(softcap=1025.0), "softcap"), (dict(q=None), "NULL"),
                          (dict(out=None), "NULL"), (dict(k=None), "both, or neither"), (dict(v=None), "both, or neither"),
                          (dict(cache=None, k=None, v=None), "neither"), (dict(kv_heads=4), "cache of"),
                          (dict(head_dim=64), "cache of"), (dict(q=a.ptr + 8), "16-byte"), (dict(out=a.ptr + 4), "16-byte"),

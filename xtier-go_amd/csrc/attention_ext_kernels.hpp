@@ -166,8 +166,9 @@ struct Score {
 };
 __device__ inline Score score_of(const ExtArgs& a, int head, float factor) {
   Score s;
-  s.f = fmaxf(fabsf(a.scale) * factor * (a.softcap > 0.f ? 2.f * kLog2e / a.softcap : kLog2e), FLT_MIN);
-  s.top = fmaxf(a.softcap * kLog2e, FLT_MIN);   // (not zero: times an infinity they are one)
+  s.f = fabsf(a.scale) * factor * (a.softcap > 0.f ? 2.f * kLog2e / a.softcap : kLog2e);
+  s.f = fminf(fmaxf(s.f, FLT_MIN), FLT_MAX);    // (times an infinity one, times zero none)
+  s.top = fmaxf(a.softcap * kLog2e, FLT_MIN);
   s.slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
   return s;
 }

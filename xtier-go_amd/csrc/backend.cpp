@@ -688,7 +688,8 @@ void Backend::attention_ext(const ExtCall& a) {
   XTG_CHECK((long long)a.n_q * a.heads <= (1LL << 30), "attention_ext: %d rows of %d heads (2^30 at most)", a.n_q, a.heads);
   XTG_CHECK(a.x_dtype == kXF32 || a.x_dtype == kXBF16, "attention_ext: unknown row type %d", a.x_dtype);
   XTG_CHECK(std::isfinite(a.scale), "attention_ext: scale %g", double(a.scale));
-  XTG_CHECK(std::isfinite(a.softcap) && a.softcap >= 0.f, "attention_ext: softcap %g", double(a.softcap));
+  // cap * (1 - 2 / (e^(2 s / cap) + 1)) in FP32 is off by up to cap * 2^-23 or so
+  XTG_CHECK(a.softcap >= 0.f && a.softcap <= 1024.f, "attention_ext: softcap %g (0 to 1024)", double(a.softcap));
   XTG_CHECK(a.q && a.out, "attention_ext: NULL argument");
   XTG_CHECK(!a.k == !a.v, "attention_ext: one of k and v is NULL (both, or neither)");
   XTG_CHECK(a.k || a.cache, "attention_ext: neither a cache nor keys of the call");
