@@ -1,4 +1,5 @@
-// Attention with capped, biased and masked scores over a cache of any dtype (attention_ext.hip).
+// Attention with capped, biased and masked scores over a cache of any dtype (plan: attention_ext.hip; kernels:
+// attention_ext_kernels.hpp).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -55,7 +56,7 @@ struct ExtArgs {
   int slots_pad, tile_lo, tiles;
   int ring, splits, records, cols, own;   // splits of the cached keys (few) or of all keys; own keys: their number
   int n_q, pos0, heads, group, window, bf16;
-  uint32_t group_inv;            // ceil(2^16 / group): (col * group_inv) >> 16 is col / group for col < 256
+  uint32_t group_inv;            // ceil(2^16 / group): (col * group_inv) >> 16 is col / group for col * group <= 2^16
   int cached_end;                // cached positions from here on are not seen
   float scale, kglobal, vglobal, softcap;
   const float* slopes;

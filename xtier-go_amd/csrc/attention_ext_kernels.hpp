@@ -1294,7 +1294,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
 // A q-col's records: their weights 2^(m - largest m) first, then the sums, D / 4 lanes to a record's accumulator and G
 // groups of lanes with the records s = group, group + G, .., whose sums are added in order. A batch of B accumulators is
 // loaded before the weights are known: few q-cols' records are a matter of latency. G = 1 (up to 16 records): a work-group
-// has several q-cols; 1440 of 9 records of 128 dims took 2.4 us so and 4.8 with a work-group each.
+// has several q-cols; 1440 of 9 records of 128 dims took 3.9 us so and 6.5 with a work-group each.
 template <int D, int T, int G, int B>
 __global__ void __launch_bounds__(256) ext_merge_kernel(ExtArgs a, int kv_heads, int total) {
   constexpr int L = D / 4, PER = 256 / (L * G);   // lanes a record; q-cols of a work-group
