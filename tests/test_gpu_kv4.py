@@ -163,6 +163,29 @@ def test_rows_that_are_not_finite(hip, d):
 
 
 @gpu
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("x_dtype", [o.F32, o.BF16])
+@pytest.mark.parametrize("glob", [2.0 ** -60, 0.5, 1.0])
+def test_values_beyond_what_a_global_holds_saturate(hip, d, x_dtype, glob):
+    """Finite values up to FP32's largest, whose quotients by the global and by a scale pass FP32, among ordinary ones:
+    the largest scale and codes of 6, as the format says, and blocks beside them as ever."""
+    rng = np.random.default_rng(d + x_dtype)
+    n, kvh = 40, 2
+    k, v = some_rows(rng, n, kvh, d) * np.float32(glob), some_rows(rng, n, kvh, d) * np.float32(glob)
+    for x in (k, v):
+        big = np.float32(10.0 ** rng.uniform(20, 38.5, x.shape)) * np.where(rng.random(x.shape) < 0.5, -1, 1)
+        x[...] = np.where(rng.random(x.shape) < 0.1, big, x)
+        x[5, 0, :16], x[37, 1, -1] = np.float32(3.38e38), np.float32(-3.38e38)
+        x[7] = big[7]
+    cache = hip.kv_cache(kvh, d, n, 0, 2)
+    cache.globals(glob, glob)
+    write(hip, cache, 0, k, v, x_dtype)
+    for g, x in zip(read(hip, cache, 0, n), (k, v)):
+        np.testing.assert_array_equal(g, o.stored_nvfp4(o.rows(x, x_dtype)[1], glob).astype(np.float32))
+    cache.destroy()
+
+
+@gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp8"])
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_other_caches_write_bf16_rows_and_read_back(hip, dtype, d):

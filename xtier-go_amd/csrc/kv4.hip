@@ -190,7 +190,7 @@ __device__ inline void store4_tile(const Store4Args& a, uint32_t* not_finite, in
     const BlockScale s = block_scale(__uint_as_float(m) * a.kinv, a.kglobal, a.kinv);
     float y[KD];
 #pragma unroll
-    for (int c = 0; c < KD; ++c) y[c] = quotient(k[u][c], s.s, s.inv);
+    for (int c = 0; c < KD; ++c) y[c] = over_scale(k[u][c], s);
     uint32_t code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, y[0], y[1], 1.f, 0);
     code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[2], y[3], 1.f, 1);
     code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, y[4], y[5], 1.f, 2);
@@ -217,7 +217,7 @@ __device__ inline void store4_tile(const Store4Args& a, uint32_t* not_finite, in
     }
 #pragma unroll
     for (int c = 0; c < P; ++c) {
-      const float y0 = quotient(v[e][c], s[0].s, s[0].inv), y1 = quotient(v[e + 1][c], s[1].s, s[1].inv);
+      const float y0 = over_scale(v[e][c], s[0]), y1 = over_scale(v[e + 1][c], s[1]);
       if (e == 0) code[c] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code[c], y0, y1, 1.f, 0);
       if (e == 2) code[c] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code[c], y0, y1, 1.f, 1);
       if (e == 4) code[c] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code[c], y0, y1, 1.f, 2);

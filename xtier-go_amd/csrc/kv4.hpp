@@ -73,9 +73,10 @@ __host__ __device__ inline float e4m3_scale_value(uint8_t s) {
 
 // The quantisation of a block of 16 whose largest magnitude over the global (a power of two, ginv its inverse) is amax: the scale is the
 // E4M3 value nearest to amax / 6, ties to even, at most 448, at least 2^-9 where amax > 0; a code is the E2M1 value
-// nearest to x / scale. Both quotients are rounded to FP32 first, which the second rounding does not see: a quotient by
-// b 2^q (1 <= b < 2) that is not a midpoint m of the second grid is off it by an ulp of its numerator over b 2^q or more,
-// which is over half an ulp of m, so it never rounds onto m.
+// nearest to x / scale, at most 6. Both quotients are rounded to FP32 first, which the second rounding does not see: a
+// quotient by b 2^q (1 <= b < 2) that is not a midpoint m of the second grid is off it by an ulp of its numerator over
+// b 2^q or more, which is over half an ulp of m, so it never rounds onto m. Numerators are held to 6 * 448 and 6 * scale
+// first, exact products: a quotient that passes FP32 would be an infinity, whose correction is NaN.
 struct BlockScale {
   uint32_t code;     // E4M3
   float s, inv;      // its value with the global, and the inverse (0 for a block of zeros)
@@ -87,9 +88,14 @@ __device__ inline float quotient(float x, float s, float inv) {
   return fmaf(fmaf(-y, s, x), inv, y);
 }
 
+// A value over its block's scale, held to what the codes hold.
+__device__ inline float over_scale(float x, const BlockScale& s) {
+  return quotient(__builtin_amdgcn_fmed3f(x, -6.f * s.s, 6.f * s.s), s.s, s.inv);
+}
+
 __device__ inline BlockScale block_scale(float amax, float global, float ginv) {
   BlockScale r;
-  const float y = fminf(fmaxf(quotient(amax, 6.f, 1.f / 6.f), amax > 0.f ? 0.001953125f : 0.f), 448.f);
+  const float y = fmaxf(quotient(fminf(amax, 2688.f), 6.f, 1.f / 6.f), amax > 0.f ? 0.001953125f : 0.f);
   r.code = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false)) & 0xffu;
   const float s = __builtin_amdgcn_cvt_f32_fp8(int(r.code), 0);
   const float i = __builtin_amdgcn_rcpf(s);
