@@ -245,6 +245,49 @@ def test_tiny_and_large_caps(hip, cap, n, heads):
     c.free()
 
 
+@pytest.mark.parametrize("dtype", ["nvfp4", "bf16", "fp8", "none"])
+@pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 40])
+@pytest.mark.parametrize("n,heads", [(2, 8), (45, 8), (26, 64)])
+def test_a_tiny_cap_with_large_queries_and_keys_of_zeros(hip, dtype, size, n, heads):
+    """What a product is multiplied by passes FP32 and has to stay finite: a key of zeros has a score of zero. All scores
+    are within 1e-38 of it, so the weights are equal (tolerances count no error of a score)."""
+    rng = np.random.default_rng(n)
+    ctx, kvh, d = 0 if dtype == "none" else 120, 2, 128
+    c = Call(hip, rng, dtype, n, ctx, heads, kvh, d)
+    kc, vc = c.unit(rng, (ctx, kvh, d)), rng.standard_normal((ctx, kvh, d)).astype(np.float32)
+    q = c.unit(rng, (n, heads, d)) * np.float32(d * size)
+    k, v = c.unit(rng, (n, kvh, d)), rng.standard_normal((n, kvh, d)).astype(np.float32)
+    kc[::3], k[::2] = 0.0, 0.0
+    if ctx:
+        c.fill(0, kc, vc)
+    for x in c.dev + [c.out]:
+        x.free()
+    c.set(0, kc, vc, q, k, v)
+    got = c.run(softcap=1e-38)
+    out, weight, _ = o.attend(c.q, *c.keys, c.at, ctx, d ** -0.5, softcap=1e-38)
+    off = np.abs(got.astype(np.float64) - out)
+    assert (off <= o.tolerance(out, weight, 0.0, d, 8, c.x)).all()
+    c.free()
+
+
+@pytest.mark.parametrize("x_dtype", [o.F32, o.BF16])
+@pytest.mark.parametrize("globs", [(2.0 ** 60, 2.0 ** -60), (2.0 ** -60, 2.0 ** 60), (0.25, 8.0)])
+@pytest.mark.parametrize("n,heads", [(2, 8), (40, 8), (50, 64)])
+def test_globals(hip, x_dtype, globs, n, heads):
+    """Keys and values at an NVFP4 cache's globals, the call's rows among them; the scale undoes the keys'."""
+    rng = np.random.default_rng(n)
+    ctx, kvh, d = 300, 2, 128
+    c = Call(hip, rng, "nvfp4", n, 0, heads, kvh, d, own=False, slots=ctx, x_dtype=x_dtype)
+    kc, vc = (x.astype(np.float32) for x in (c.unit(rng, (ctx, kvh, d)) * globs[0],
+                                              rng.standard_normal((ctx, kvh, d)) * globs[1]))
+    c.cache.globals(*globs)
+    c.fill(0, kc, vc)
+    c.keys, c.at = o.stored_pair(kc, vc, "nvfp4", globs), np.arange(ctx)
+    c.check(pos0=ctx - n, scale=d ** -0.5 / globs[0])
+    c.check(pos0=100, scale=-0.5 / globs[0], softcap=5.0, window=80)
+    c.free()
+
+
 @pytest.mark.parametrize("size", [2.0 ** -127, 2.0 ** -100, 2.0 ** 40])
 @pytest.mark.parametrize("n,heads", [(2, 8), (26, 64)])
 def test_tiny_and_huge_queries(hip, size, n, heads):

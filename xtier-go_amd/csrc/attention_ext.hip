@@ -2,6 +2,7 @@
 // compiled for each head size in attention_ext_d64.hip, _d128.hip and _d256.hip).
 #include <algorithm>
 #include <climits>
+#include <cmath>
 
 #include "attention_ext.hpp"
 #include "common.hpp"
@@ -74,6 +75,8 @@ void launch_attn_ext(const ExtCall& c, const ExtPlan& p, void* scratch, hipStrea
   a.group_inv = (65536u + uint32_t(a.group) - 1u) / uint32_t(a.group);
   a.bf16 = c.x_dtype == kXBF16;
   a.cached_end = c.k ? a.pos0 : INT_MAX;
+  const double log2e = kLog2e;
+  a.factor = std::fabs(double(c.scale)) * (c.softcap > 0.f ? 2 * log2e / c.softcap : log2e);
   a.scale = c.scale, a.softcap = c.softcap, a.slopes = c.slopes, a.first = c.first, a.end = c.end;
   char* at = static_cast<char*>(scratch);
   a.pk = reinterpret_cast<const uint4*>(at);

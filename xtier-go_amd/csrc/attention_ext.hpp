@@ -43,6 +43,7 @@ ExtPlan ext_plan(const ExtCall& a, int cus);
 
 constexpr int kBf16 = 0, kFp8 = 1, kNvfp4 = 2;   // XTG_KV_*
 constexpr int kExtWaves = 4;                     // waves of a work-group
+constexpr float kLog2e = 1.44269504088896341f;
 
 // What the kernels take.
 struct ExtArgs {
@@ -58,6 +59,7 @@ struct ExtArgs {
   int n_q, pos0, heads, group, window, bf16;
   uint32_t group_inv;            // ceil(2^16 / group): (col * group_inv) >> 16 is col / group for col * group <= 2^16
   int cached_end;                // cached positions from here on are not seen
+  double factor;                 // what a product q.k is multiplied by, in base-2 units (score_of)
   float scale, kglobal, vglobal, softcap;
   const float* slopes;
   const int* first;

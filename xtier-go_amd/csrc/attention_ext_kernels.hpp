@@ -41,7 +41,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr float kLog2e = 1.44269504088896341f;
 // Weights are 2^(s - m + 7), and m moves only when a score passes it by more than 8: weights stay below f16's 2^16,
 // and those of 2^-21 of the largest still have all their bits.
 constexpr float kUp = 7.f, kSlack = 8.f;
@@ -164,10 +163,14 @@ struct Score {
   float f;             // times this (the scale, or with a cap what the exponential takes)
   float top, slope;    // cap * log2(e); the head's slope * log2(e)
 };
-__device__ inline Score score_of(const ExtArgs& a, int head, float factor) {
+// Score::f for operands whose product times `factor`, a power of two, is q.k. In 64 bits: a small cap, a global and a
+// q-col's power of two pass FP32 together. (It stays finite and above zero: times an infinity one, times zero none.)
+__device__ inline float score_factor(const ExtArgs& a, double factor) {
+  return fminf(fmaxf(float(a.factor * factor), FLT_MIN), FLT_MAX);
+}
+__device__ inline Score score_of(const ExtArgs& a, int head, double factor) {
   Score s;
-  s.f = fabsf(a.scale) * factor * (a.softcap > 0.f ? 2.f * kLog2e / a.softcap : kLog2e);
-  s.f = fminf(fmaxf(s.f, FLT_MIN), FLT_MAX);    // (times an infinity one, times zero none)
+  s.f = score_factor(a, factor);
   s.top = fmaxf(a.softcap * kLog2e, FLT_MIN);
   s.slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
   return s;
@@ -233,7 +236,7 @@ __device__ inline void slow_col(const ExtArgs& a, int h, int kv_heads, int row, 
   float *q = lds, *w = lds + D, *red = lds + D + 256;
   const int tid = int(threadIdx.x);
   const Span all = row_span(a, row), cached = cached_span(a, all);
-  const Score sc = score_of(a, head, 1.f);
+  const Score sc = score_of(a, head, 1.);
   const size_t at = (size_t(row) * size_t(a.heads) + size_t(head)) * D + size_t(tid);
   __syncthreads();
   if (tid < D) q[tid] = row_value(a.q, at, a.bf16);
@@ -540,7 +543,7 @@ struct FewQueries {
       const size_t at = live ? (size_t(row) * size_t(a.heads) + size_t(head)) * D : 0;
       row_chunks(a.q, a.bf16, live, [&](int c) { return at + size_t(TILE::q_dim(c, lane >> 4)); }, x[qb]);
       span[qb] = live ? row_span(a, row) : Span{0, 0u, 0};
-      sc[qb] = score_of(a, live ? head : 0, 1.f);
+      sc[qb] = score_of(a, live ? head : 0, 1.);
     }
   }
   template <class X8>
@@ -551,7 +554,7 @@ struct FewQueries {
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) x[qb][c] = -x[qb][c];
       }
-      sc[qb].f *= global * to_operand(x[qb], q[qb], [](float v) { return xor32_max(xor16_max(v)); });
+      sc[qb].f = score_factor(a, double(global) * to_operand(x[qb], q[qb], [](float v) { return xor32_max(xor16_max(v)); }));
     }
   }
 };
@@ -1194,7 +1197,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
       for (int c = 0; c < R::NS; ++c) x[c] = -x[c];
     }
     const float factor = to_operand(x, q, [](float y) { return xor32_max(y); });
-    sc = score_of(a, live ? head : 0, factor * global);
+    sc = score_of(a, live ? head : 0, double(factor) * global);
 #pragma unroll
     for (int c = 0; c < QL; ++c) ql[c * 256] = q[R::NS - QL + c];
     f32x16 s[R::KB];
