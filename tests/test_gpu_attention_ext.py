@@ -358,6 +358,27 @@ def test_captured_and_replayed(hip, n, heads):
 
 
 @pytest.mark.parametrize("n,heads", [(1, 8), (20, 8), (45, 64)])
+def test_captured_at_a_later_position_than_the_first_call(pkg, n, heads):
+    """The first call of a shape sizes the scratch for every position of the cache: a session that was warmed up at its
+    beginning captures its steps far into it."""
+    b = pkg.HipBackend(0)
+    c = Call(b, np.random.default_rng(n), "nvfp4", n, 4000, heads, 2, 128, slots=5000)
+    c.queue(pos0=3)
+    b.finish()
+    b.graph_begin()
+    c.queue()
+    g = b.graph_end("late")
+    for _ in range(3):
+        c.out.upload(np.full(c.out.shape, 0x7fc1, np.uint16))
+        b.graph_launch(g)
+        got = c.result()
+        np.testing.assert_array_equal(c.check(), got)
+    b.graph_destroy(g)
+    c.free()
+    b.close()
+
+
+@pytest.mark.parametrize("n,heads", [(1, 8), (20, 8), (45, 64)])
 def test_the_last_positions(hip, n, heads):
     """Rows up to position 2^31 - 2, over a ring and over their own keys alone."""
     rng, pos0, ring = np.random.default_rng(n), 2 ** 31 - 1 - n, 96

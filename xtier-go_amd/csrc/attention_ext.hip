@@ -15,18 +15,11 @@ namespace xtg::hip {
 // 768 51.6 (63.6), 1024 64.4 (53.9).
 constexpr int kFewCols = 768;
 
-ExtPlan ext_plan(const ExtCall& a, int cus) {
+// The plan for the cache's slots lo .. slots - 1.
+static ExtPlan plan_of(const ExtCall& a, int cus, long long lo, long long slots) {
   ExtPlan p;
   const int group = a.heads / a.kv_heads;
   const long long cols = (long long)a.n_q * group;
-  // the slots that can hold a position which a row sees: a linear cache's are positions
-  long long slots = 0, lo = 0;
-  if (a.cache) {
-    slots = a.cache->slots;
-    const long long past = a.k ? a.pos0 : a.end ? slots : a.pos0 + a.n_q;
-    if (!a.cache->ring || a.k) slots = std::min(slots, past);   // (a ring fills from its first slot on)
-    if (!a.cache->ring && a.window > 0) lo = std::max(0LL, std::min(slots, a.pos0 - a.window + 1));
-  }
   const int own_tiles = a.k ? (a.n_q + 31) / 32 : 0;
   p.few = cols <= kFewCols && cols * group <= 65536;
   if (p.few) {
@@ -55,6 +48,22 @@ ExtPlan ext_plan(const ExtCall& a, int cus) {
   if (p.splits > 1)
     p.record_bytes = size_t(p.splits) * size_t(groups) * 128 * size_t(a.d + 2) * sizeof(float);
   if (a.k) p.pack_bytes = 2 * size_t(a.kv_heads) * size_t((a.n_q + 63) / 64 * 64) * size_t(a.d) * 2;
+  return p;
+}
+
+ExtPlan ext_plan(const ExtCall& a, int cus) {
+  // the slots that can hold a position which a row sees: a linear cache's are positions
+  const long long all = a.cache ? a.cache->slots : 0;
+  long long slots = all, lo = 0;
+  if (a.cache) {
+    const long long past = a.k ? a.pos0 : a.end ? slots : a.pos0 + a.n_q;
+    if (!a.cache->ring || a.k) slots = std::min(slots, past);   // (a ring fills from its first slot on)
+    if (!a.cache->ring && a.window > 0) lo = std::max(0LL, std::min(slots, a.pos0 - a.window + 1));
+  }
+  ExtPlan p = plan_of(a, cus, lo, slots);
+  // Records grow with the slots until the splits fill the CUs. Scratch is what the whole cache takes, so that later
+  // positions of a decode loop, or of a graph captured after an early call, never ask for more.
+  p.scratch = plan_of(a, cus, 0, all).used_bytes();
   return p;
 }
 

@@ -37,7 +37,8 @@ struct ExtPlan {
   int tile_lo = 0, tiles = 0;    // few: the cache's 32-slot tiles to scan; else tile_lo = 0 and the slots to scan
   size_t pack_bytes = 0;         // own keys and values as BF16 tiles
   size_t record_bytes = 0;
-  size_t scratch_bytes() const { return pack_bytes + record_bytes; }
+  size_t used_bytes() const { return pack_bytes + record_bytes; }
+  size_t scratch = 0;            // used_bytes() at most, whatever the call's positions and window
 };
 ExtPlan ext_plan(const ExtCall& a, int cus);
 

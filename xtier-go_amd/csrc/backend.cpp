@@ -704,7 +704,7 @@ void Backend::attention_ext(const ExtCall& a) {
               a.cache->head_dim, a.kv_heads, a.d);
   }
   const ExtPlan p = ext_plan(a, cus_);
-  ensure(ext_, ext_size_, p.scratch_bytes());
+  ensure(ext_, ext_size_, p.scratch);
   launch_attn_ext(a, p, ext_, stream_, [&](auto&& launch) { timed(launch); });
 }
 
