@@ -85,7 +85,7 @@ void launch_attn_ext(const ExtCall& c, const ExtPlan& p, void* scratch, hipStrea
   a.bf16 = c.x_dtype == kXBF16;
   a.cached_end = c.k ? a.pos0 : INT_MAX;
   const double log2e = kLog2e;
-  a.factor = std::fabs(double(c.scale)) * (c.softcap > 0.f ? 2 * log2e / c.softcap : log2e);
+  a.factor = float(std::frexp(std::fabs(double(c.scale)) * (c.softcap > 0.f ? 2 * log2e / c.softcap : log2e), &a.factor_exp));
   a.scale = c.scale, a.softcap = c.softcap, a.slopes = c.slopes, a.first = c.first, a.end = c.end;
   char* at = static_cast<char*>(scratch);
   a.pk = reinterpret_cast<const uint4*>(at);

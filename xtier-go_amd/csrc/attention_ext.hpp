@@ -60,7 +60,8 @@ struct ExtArgs {
   int n_q, pos0, heads, group, window, bf16;
   uint32_t group_inv;            // ceil(2^16 / group): (col * group_inv) >> 16 is col / group for col * group <= 2^16
   int cached_end;                // cached positions from here on are not seen
-  double factor;                 // what a product q.k is multiplied by, in base-2 units (score_of)
+  float factor;                  // what a product q.k is multiplied by in base-2 units (score_factor): factor * 2^factor_exp
+  int factor_exp;
   float scale, kglobal, vglobal, softcap;
   const float* slopes;
   const int* first;

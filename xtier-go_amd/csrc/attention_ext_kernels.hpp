@@ -85,9 +85,9 @@ __device__ inline void row_chunks(const void* p, int bf16, bool live, A at, bf16
 }
 
 // The q-col's N operand chunks: to f16 times a power of two that brings the largest magnitude over the q-col's lanes
-// (`join`) to 2^8 .. 2^9, or as they are. Returns what a product has to be multiplied by.
+// (`join`) to 2^8 .. 2^9, or as they are. Returns the power of two that a product has to be multiplied by.
 template <int N, class J>
-__device__ inline float to_operand(const bf16x8 (&x)[N], f16x8 (&q)[N], J join) {
+__device__ inline int to_operand(const bf16x8 (&x)[N], f16x8 (&q)[N], J join) {
   uint32_t m = 0;
 #pragma unroll
   for (int c = 0; c < N; ++c)
@@ -100,13 +100,13 @@ __device__ inline float to_operand(const bf16x8 (&x)[N], f16x8 (&q)[N], J join) 
   for (int c = 0; c < N; ++c)
 #pragma unroll
     for (int e = 0; e < 8; ++e) q[c][e] = (_Float16)((float)x[c][e] * down);
-  return ldexpf(1.f, ex);
+  return ex;
 }
 template <int N, class J>
-__device__ inline float to_operand(const bf16x8 (&x)[N], bf16x8 (&q)[N], J) {
+__device__ inline int to_operand(const bf16x8 (&x)[N], bf16x8 (&q)[N], J) {
 #pragma unroll
   for (int c = 0; c < N; ++c) q[c] = x[c];
-  return 1.f;
+  return 0;
 }
 
 // 8 E4M3 codes as BF16, exactly.
@@ -163,14 +163,15 @@ struct Score {
   float f;             // times this (the scale, or with a cap what the exponential takes)
   float top, slope;    // cap * log2(e); the head's slope * log2(e)
 };
-// Score::f for operands whose product times `factor`, a power of two, is q.k. In 64 bits: a small cap, a global and a
-// q-col's power of two pass FP32 together. (It stays finite and above zero: times an infinity one, times zero none.)
-__device__ inline float score_factor(const ExtArgs& a, double factor) {
-  return fminf(fmaxf(float(a.factor * factor), FLT_MIN), FLT_MAX);
+// Score::f for operands whose product times global * 2^ex is q.k (a power of two too). Exponents are added as integers: those of
+// a small cap, a global and a q-col pass FP32 together. (It stays finite and above zero: times an infinity one, times zero
+// none.)
+__device__ inline float score_factor(const ExtArgs& a, float global, int ex) {
+  return fminf(fmaxf(ldexpf(a.factor * global, a.factor_exp + ex), FLT_MIN), FLT_MAX);
 }
-__device__ inline Score score_of(const ExtArgs& a, int head, double factor) {
+__device__ inline Score score_of(const ExtArgs& a, int head, float global, int ex) {
   Score s;
-  s.f = score_factor(a, factor);
+  s.f = score_factor(a, global, ex);
   s.top = fmaxf(a.softcap * kLog2e, FLT_MIN);
   s.slope = a.slopes ? a.slopes[head] * kLog2e : 0.f;
   return s;
@@ -236,7 +237,7 @@ __device__ inline void slow_col(const ExtArgs& a, int h, int kv_heads, int row, 
   float *q = lds, *w = lds + D, *red = lds + D + 256;
   const int tid = int(threadIdx.x);
   const Span all = row_span(a, row), cached = cached_span(a, all);
-  const Score sc = score_of(a, head, 1.);
+  const Score sc = score_of(a, head, 1.f, 0);
   const size_t at = (size_t(row) * size_t(a.heads) + size_t(head)) * D + size_t(tid);
   __syncthreads();
   if (tid < D) q[tid] = row_value(a.q, at, a.bf16);
@@ -543,7 +544,7 @@ struct FewQueries {
       const size_t at = live ? (size_t(row) * size_t(a.heads) + size_t(head)) * D : 0;
       row_chunks(a.q, a.bf16, live, [&](int c) { return at + size_t(TILE::q_dim(c, lane >> 4)); }, x[qb]);
       span[qb] = live ? row_span(a, row) : Span{0, 0u, 0};
-      sc[qb] = score_of(a, live ? head : 0, 1.);
+      sc[qb] = score_of(a, live ? head : 0, 1.f, 0);
     }
   }
   template <class X8>
@@ -554,7 +555,7 @@ struct FewQueries {
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) x[qb][c] = -x[qb][c];
       }
-      sc[qb].f = score_factor(a, double(global) * to_operand(x[qb], q[qb], [](float v) { return xor32_max(xor16_max(v)); }));
+      sc[qb].f = score_factor(a, global, to_operand(x[qb], q[qb], [](float v) { return xor32_max(xor16_max(v)); }));
     }
   }
 };
@@ -1196,8 +1197,8 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
 #pragma unroll
       for (int c = 0; c < R::NS; ++c) x[c] = -x[c];
     }
-    const float factor = to_operand(x, q, [](float y) { return xor32_max(y); });
-    sc = score_of(a, live ? head : 0, double(factor) * global);
+    const int ex = to_operand(x, q, [](float y) { return xor32_max(y); });
+    sc = score_of(a, live ? head : 0, global, ex);
 #pragma unroll
     for (int c = 0; c < QL; ++c) ql[c * 256] = q[R::NS - QL + c];
     f32x16 s[R::KB];
