@@ -209,6 +209,26 @@ def test_other_caches_write_bf16_rows_and_read_back(hip, dtype, d):
 
 
 @gpu
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_fp8_rows_with_infinities_read_back_as_they_load(hip, d):
+    """A row with an infinity has an infinite scale: its codes of zero are NaN, in K and V, on the device as on the host;
+    a NaN is one by itself."""
+    rng = np.random.default_rng(d)
+    n, kvh = 40, 2
+    k, v = (rng.standard_normal((n, kvh, d)).astype(np.float32) for _ in "kv")
+    k[3, 0, 5], v[3, 1, 7], v[36, 0, 2], k[20, 1, 1], v[20, 1, 1] = np.inf, -np.inf, np.inf, np.nan, np.nan
+    cache = hip.kv_cache(kvh, d, n + 5, 0, o.KV["fp8"])
+    write(hip, cache, 0, k, v)
+    got = read(hip, cache, 0, n + 5)
+    for h in range(kvh):
+        for g, w in zip(got, cache.load(h, 0, n)):
+            np.testing.assert_array_equal(g[:n, h], w)
+    assert np.isnan(got[1][3, 1]).all() and np.isnan(got[1][20, 1, 1]) and np.isfinite(got[1][20, 1, 2:]).all()
+    assert not any(g[n:].any() for g in got)
+    cache.destroy()
+
+
+@gpu
 def test_save_restore_copy_release(hip):
     rng = np.random.default_rng(2)
     kvh, d, ring, n = 2, 128, 45, 60

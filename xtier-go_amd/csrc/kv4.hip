@@ -427,8 +427,9 @@ __global__ void __launch_bounds__(256) kv_read_kernel(ReadArgs a) {
       for (int e = 0; e < 8; ++e) {
         const int slot = 32 * t + (e < 4 ? 4 * g + e : 12 + 4 * g + e), r = row_of(slot);
         if (r < 0) continue;
-        float y = a.slot_pos[slot] == int(p0 + slot) ? x[e] : 0.f;
-        if (T == kFp8 && y != 0.f) y *= static_cast<const float*>(a.vs)[head + size_t(slot)];
+        const bool held = a.slot_pos[slot] == int(p0 + slot);
+        float y = held ? x[e] : 0.f;
+        if (T == kFp8 && held) y *= static_cast<const float*>(a.vs)[head + size_t(slot)];   // (infinite: zeros are NaN)
         dst(a.v, r)[16 * dd + i] = X(y);
       }
     }
