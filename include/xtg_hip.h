@@ -211,7 +211,7 @@ int xtg_hip_attention_noalloc(xtg_hip* h, const xtg_attn_args* a, char* err, int
  * first NULL: from 0; end NULL: to t (end[i] = t + 1). A document's start in `first` keeps packed documents apart; an
  * `end` past t lets the rows of a prefix see all of it; first[i] >= end[i] (a padding row) leaves nothing. Its score for
  * a key is s = (q . k) * scale, then softcap * tanh(s / softcap) where softcap > 0, then minus slopes[head] * |t - p|
- * where slopes is given. A row that sees nothing gets zeros.
+ * where slopes is given. A row that sees nothing gets zeros, one whose scores are all minus infinity NaN.
  * The keys are the cache's (NULL: none) at positions before pos0, as their slots say, and the call's own k, v at pos0 ..
  * pos0 + n_q - 1, not yet stored; with k and v NULL they are the cache's alone, the call's own rows among them.
  * Rows are x_dtype: BF16, or FP32, of which q, k and v are rounded to BF16 as they are read (as a cache rounds what it

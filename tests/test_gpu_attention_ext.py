@@ -327,6 +327,45 @@ def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(hip, dtype
     c.free()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "none"])
+@pytest.mark.parametrize("n,heads", [(1, 8), (6, 8), (70, 8), (26, 64), (40, 64)])
+def test_rows_whose_scores_are_all_minus_infinity(hip, dtype, n, heads):
+    """Such a row is NaN, as its formula is (only a row that sees nothing is zeros); with one other key it is that key's."""
+    rng = np.random.default_rng(n)
+    ctx, kvh, d = 0 if dtype == "none" else 700, 2, 128
+    c = Call(hip, rng, dtype, n, ctx, heads, kvh, d, slots=ctx + n)
+    kc, vc = c.unit(rng, (ctx, kvh, d)), rng.standard_normal((ctx, kvh, d)).astype(np.float32)
+    q = c.unit(rng, (n, heads, d)) * d
+    k, v = c.unit(rng, (n, kvh, d)), rng.standard_normal((n, kvh, d)).astype(np.float32)
+    q[..., 0], kc[..., 0] = 1.0, -np.inf
+    if dtype == "none":
+        k[0, :, 0] = -np.inf
+    else:
+        c.fill(0, kc, vc)
+    for x in c.dev + [c.out]:
+        x.free()
+    c.set(0, kc, vc, q, k, v)
+    got = c.check()
+    if dtype == "none":
+        assert np.isnan(got[0]).all() and np.isfinite(got[1:]).all()
+    else:
+        assert np.isfinite(got).all()
+        assert np.isnan(c.check(end=np.full(n, ctx))).all()
+        assert not c.check(first=np.full(n, ctx), end=np.full(n, ctx)).any()
+    c.free()
+
+
+@pytest.mark.parametrize("dtype", ["nvfp4", "bf16", "fp8"])
+@pytest.mark.parametrize("n,heads", [(1, 8), (45, 8), (26, 64)])
+def test_positions_that_the_cache_does_not_hold(hip, dtype, n, heads):
+    """Rows may see positions that were never written: they see nothing there."""
+    c = Call(hip, np.random.default_rng(n), dtype, n, 0, heads, 2, 128, slots=900)
+    c.at = 800 + np.arange(n)
+    assert not c.check(pos0=800, end=np.full(n, 800)).any()
+    c.check(pos0=800)
+    c.free()
+
+
 @pytest.mark.parametrize("n,heads", [(1, 8), (5, 8), (66, 8), (26, 64)])
 def test_captured_and_replayed(hip, n, heads):
     """A graph of a write, an attention and a read, replayed with eager work between the replays."""

@@ -24,7 +24,7 @@
 // Values that are not finite: a score that is masked is replaced, so a key's only reach the q-cols that see it. Not so a
 // value's, times a weight of zero. NVFP4 caches hold such rows as NaN keys (kv4.hip) and their V scales are taken as zero.
 // With the others a q-col whose sum of weights is finite and whose accumulator is not is computed again key by key, by
-// whichever kernel writes it (slow_col).
+// whichever kernel writes it (slow_col). So is one without a sum that may see a key: scores of minus infinity alone are NaN.
 #pragma once
 
 #include <cfloat>
@@ -205,6 +205,22 @@ __device__ inline float finish(const Score& s, float x, float minus) {
 
 __device__ inline bool not_finite(float x) { return !(fabsf(x) <= FLT_MAX); }
 
+// A kernel's ExtArgs, its first argument, read again: what of them only a rare path behind the loops needs does not stay in
+// registers through these.
+__device__ inline ExtArgs args_again() {
+  auto from = (const __attribute__((address_space(4))) uint32_t*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(from));
+  struct Words {
+    uint32_t w[sizeof(ExtArgs) / 4];
+  } words;
+#pragma unroll
+  for (size_t x = 0; x < sizeof(ExtArgs) / 4; ++x) words.w[x] = from[x];
+  return __builtin_bit_cast(ExtArgs, words);
+}
+
+// A sum of no weights in a row that sees some positions: nothing is there, or all of its scores are minus infinity.
+__device__ inline bool no_sum(float l, int row) { return l == 0.f && row_span(args_again(), row).len > 0; }
+
 // ------------------------------------------------------------------------------------------- a q-col key by key
 
 template <int D, int T>
@@ -231,7 +247,8 @@ __device__ inline float row_value(const void* p, size_t at, int bf16) {
 }
 
 // One q-col by a work-group of 256 threads: 256 keys at a time, a score each thread, then a dim each thread; values of
-// keys that the row does not see are not read. lds: 272 + D floats.
+// keys that the row does not see are not read. Scores of minus infinity alone leave no sum, and NaN; keys that the row does
+// not see, or that are not there, zeros. lds: 272 + D floats.
 template <int D, int T>
 __device__ inline void slow_col(const ExtArgs& a, int h, int kv_heads, int row, int head, float* lds) {
   float *q = lds, *w = lds + D, *red = lds + D + 256;
@@ -242,8 +259,10 @@ __device__ inline void slow_col(const ExtArgs& a, int h, int kv_heads, int row, 
   __syncthreads();
   if (tid < D) q[tid] = row_value(a.q, at, a.bf16);
   __syncthreads();
-  float m = -INFINITY, l = 0.f, acc = 0.f;
+  float m = -INFINITY, l = 0.f, acc = 0.f;   // (m: -inf until a key is seen, -FLT_MAX at least from then on)
   for (int k0 = 0; k0 < a.slots_pad + a.own; k0 += 256) {
+    // (a linear cache's slots are positions; the work-group's threads have one row)
+    if (!a.ring && k0 + 256 <= a.slots_pad && (k0 + 256 <= all.lo || k0 - all.lo >= int(cached.len))) continue;
     const int key = k0 + tid, j = key - a.slots_pad;   // own key j
     int pos = -1;
     if (j < 0)
@@ -260,8 +279,9 @@ __device__ inline void slow_col(const ExtArgs& a, int h, int kv_heads, int row, 
       if (a.scale < 0.f) s = -s;
       s = a.softcap > 0.f ? changed<kCap | kBias>(sc, s, all.t - pos) : changed<kBias>(sc, s, all.t - pos);
     }
-    const float m_new = fmaxf(m, block_max<256>(s, red)), ref = m_new == -INFINITY ? 0.f : m_new;
-    const float p = __builtin_amdgcn_exp2f(s - ref), corr = __builtin_amdgcn_exp2f(m - ref);
+    const float top = block_max<256>(seen ? fmaxf(s, -FLT_MAX) : -INFINITY, red), m_new = fmaxf(m, top);
+    if (top == -INFINITY) continue;
+    const float p = __builtin_amdgcn_exp2f(s - m_new), corr = __builtin_amdgcn_exp2f(m - m_new);
     w[tid] = seen ? p : -1.f;   // -1: not seen
     l = l * corr + block_sum<256>(p, red);
     m = m_new;
@@ -277,7 +297,7 @@ __device__ inline void slow_col(const ExtArgs& a, int h, int kv_heads, int row, 
     __syncthreads();
   }
   if (tid < D) {
-    const float y = l == 0.f ? 0.f : acc / l;
+    const float y = l == 0.f ? m == -INFINITY ? 0.f : NAN : acc / l;
     if (a.bf16)
       static_cast<__bf16*>(a.out)[at] = (__bf16)y;
     else
@@ -690,9 +710,10 @@ __global__ void __launch_bounds__(kExtWaves * 64, QB * D > 256 ? 1 : 2) ext_few_
       float l = l_all[0];
       if constexpr (QB == 2) l = qb ? l_all[1] : l;
       if (a.records == 1) {
+        bool bad = no_sum(l, row);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (!not_finite(l) && not_finite(y[r])) atomicOr(&again, 1u << mine);
+        for (int r = 0; r < 4; ++r) bad |= !not_finite(l) && not_finite(y[r]);
+        if (bad) atomicOr(&again, 1u << mine);
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -712,7 +733,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, QB * D > 256 ? 1 : 2) ext_few_
     __syncthreads();
     for (uint32_t bits = again; bits; bits &= bits - 1) {
       const int col = col0 + __builtin_ctz(bits), row = few_row(a, col);
-      slow_col<D, T>(a, h, kv_heads, row, h * a.group + col - row * a.group, lds);
+      slow_col<D, T>(args_again(), h, kv_heads, row, h * a.group + col - row * a.group, lds);
     }
     return;
   }
@@ -1271,13 +1292,13 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
       write(static_cast<__bf16*>(a.out));
     else
       write(static_cast<float*>(a.out));
-    const uint64_t any = __ballot(bad && !not_finite(l));
+    const uint64_t any = __ballot((bad && !not_finite(l)) || (live && no_sum(l, row)));
     if (lane == 0) bounds[wave][0] = int(uint32_t(any) | uint32_t(any >> 32));
     __syncthreads();
     for (int w = 0; w < kExtWaves; ++w)
       for (uint32_t bits = uint32_t(bounds[w][0]); bits; bits &= bits - 1) {
         const int c = block * 128 + w * 32 + __builtin_ctz(bits);
-        slow_col<D, T>(a, h, kv_heads, c / a.group, h * a.group + c % a.group, reinterpret_cast<float*>(smem));
+        slow_col<D, T>(args_again(), h, kv_heads, c / a.group, h * a.group + c % a.group, reinterpret_cast<float*>(smem));
       }
     return;
   }
@@ -1367,7 +1388,8 @@ __global__ void __launch_bounds__(256) ext_merge_kernel(ExtArgs a, int kv_heads,
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const float o[4] = {y.x * inv, y.y * inv, y.z * inv, y.w * inv};
-  const bool bad = !not_finite(l) && (not_finite(y.x) || not_finite(y.y) || not_finite(y.z) || not_finite(y.w));
+  const bool bad = live && !not_finite(l) &&
+                   (not_finite(y.x) || not_finite(y.y) || not_finite(y.z) || not_finite(y.w) || no_sum(l, row));
   if (live && grp == 0) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -1379,13 +1401,13 @@ __global__ void __launch_bounds__(256) ext_merge_kernel(ExtArgs a, int kv_heads,
         static_cast<float*>(a.out)[at] = o[r];
     }
   }
-  if (!__syncthreads_or(bad && live)) return;
-  if (bad && live) again[mine] = 1;
+  if (!__syncthreads_or(bad)) return;
+  if (bad) again[mine] = 1;
   __syncthreads();
   for (int k = 0; k < PER; ++k)
     if (again[k]) {
       const int q = int(blockIdx.x) * PER + k;
-      slow_col<D, T>(a, q % a.heads / a.group, kv_heads, q / a.heads, q % a.heads, slow);
+      slow_col<D, T>(args_again(), q % a.heads / a.group, kv_heads, q / a.heads, q % a.heads, slow);
     }
 }
 
