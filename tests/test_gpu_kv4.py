@@ -291,6 +291,33 @@ def test_refusals(hip, pkg):
     cache.destroy()
 
 
+@gpu
+@pytest.mark.parametrize("pos", [2 ** 31 - 1, 2 ** 40, 2 ** 63 - 2, 2 ** 63 - 1])
+def test_positions_whose_end_passes_64_bits_are_refused(hip, pkg, wl, pos):
+    """The end of the rows, pos + n, is never formed: it would be negative, and below every limit."""
+    a = hip.array(shape=(8, 8, 64))
+    caches = [hip.kv_cache(2, 64, 40, ring, dtype) for ring in (0, 40) for dtype in (0, 1, 2)]
+    for c in caches:
+        calls = [lambda: c.store(pos, 2, a, a), lambda: c.write(pos, 2, a, a), lambda: c.read(pos, 2, a, a),
+                 lambda: hip.attention_ext(c, a, a, a, a, 2, pos, 4, 2, 64), lambda: hip.attention(c, a, a, a, a, 2, pos, 4),
+                 lambda: hip.attention_noalloc(c, a, a, a, a, 2, pos, 4)]
+        for call in calls:
+            with pytest.raises(pkg.XtgError, match="full|positions|rows at|NVFP4"):
+                call()
+        assert not read(hip, c, 0, 40)[0].any()
+    w = wl.DoryWeights(wl.DORY_TINY, seed=3, context=256)
+    d = hip.dory(w)
+    x = hip.array(shape=(2, w.cfg["hidden"]))
+    for call in (lambda: d.forward(x, 2, pos, None), lambda: d.prefill(x, 2, pos, pkg.LOGITS_NONE)):
+        with pytest.raises(pkg.XtgError, match="context full"):
+            call()
+    d.destroy()
+    for c in caches:
+        c.destroy()
+    for b in (a, x):
+        b.free()
+
+
 def test_null_arguments_are_refused(pkg):
     """Without a GPU: a NULL handle or cache is an error, not a fault."""
     lib, err = pkg.lib(), ctypes.create_string_buffer(200)

@@ -2291,7 +2291,7 @@ AttnPlan attn_plan(const DevKv& c, int n_q, int heads, long long pos0, int windo
   const int group = heads / c.kv_heads;
   XTG_CHECK(group <= 8, "attention: %d query heads per KV head (at most 8)", group);
   XTG_CHECK(n_q >= 1, "attention: %d query rows", n_q);
-  XTG_CHECK(pos0 >= 0 && pos0 + n_q < (1LL << 31), "attention: positions %lld + %d beyond the 32-bit slot positions",
+  XTG_CHECK(pos0 >= 0 && pos0 < (1LL << 31) - n_q, "attention: positions %lld + %d beyond the 32-bit slot positions",
             pos0, n_q);
   AttnPlan p;
   p.group = group;

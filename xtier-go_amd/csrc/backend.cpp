@@ -444,8 +444,8 @@ void Backend::check_rows(const char* what, const DevKv* c, long long pos, int n,
   XTG_CHECK(kvs_.count(const_cast<DevKv*>(c)), "%s: unknown cache", what);
   XTG_CHECK(n >= 0 && pos >= 0, "%s: %d rows at %lld", what, n, pos);
   // kv.cpp:78: a linear cache holds positions below its capacity
-  XTG_CHECK(c->ring || pos + n <= c->slots, "KV cache full: position %lld of %lld", pos + n, c->slots);
-  XTG_CHECK(pos + n < (1LL << 31), "%s: position %lld beyond the 32-bit slot positions", what, pos + n);
+  XTG_CHECK(c->ring || pos <= c->slots - n, "KV cache full: position %lld + %d of %lld", pos, n, c->slots);
+  XTG_CHECK(pos < (1LL << 31) - n, "%s: positions %lld + %d beyond the 32-bit slot positions", what, pos, n);
   XTG_CHECK(x_dtype == kXF32 || x_dtype == kXBF16, "%s: unknown row type %d", what, x_dtype);
   XTG_CHECK(n == 0 || (k && v), "%s: NULL rows", what);
 }
@@ -681,7 +681,7 @@ void Backend::attention(const DevKv* c, int n_q, long long pos0, int heads, int 
 }
 
 void Backend::attention_ext(const ExtCall& a) {
-  XTG_CHECK(a.n_q >= 1 && a.pos0 >= 0 && a.pos0 + a.n_q < (1LL << 31), "attention_ext: %d rows at %lld", a.n_q, a.pos0);
+  XTG_CHECK(a.n_q >= 1 && a.pos0 >= 0 && a.pos0 < (1LL << 31) - a.n_q, "attention_ext: %d rows at %lld", a.n_q, a.pos0);
   XTG_CHECK(a.d == 64 || a.d == 128 || a.d == 256, "attention_ext: head_dim %d (64, 128 or 256)", a.d);
   XTG_CHECK(a.kv_heads >= 1 && a.heads >= 1 && a.heads % a.kv_heads == 0 && a.kv_heads < 65536,
             "attention_ext: %d heads over %d KV heads", a.heads, a.kv_heads);
@@ -714,8 +714,8 @@ void Backend::attn_step(DevKv* c, int m, long long pos0, int heads, int window, 
   XTG_CHECK(kvs_.count(c) && !c->fp4, "attention step: unknown cache, or an NVFP4 one");
   XTG_CHECK(!gate_rec || (m == 1 && out && !op), "attention step: the gate's records take one row, out and no operand");
   XTG_CHECK(m >= 1 && pos0 >= 0, "attention step: %d rows at %lld", m, pos0);
-  XTG_CHECK(pos0 + m < (1LL << 31), "attention step: position %lld beyond the 32-bit slot positions", pos0 + m);
-  XTG_CHECK(c->ring || pos0 + m <= c->slots, "attention step: context full (%lld + %d > %lld slots)", pos0, m,
+  XTG_CHECK(pos0 < (1LL << 31) - m, "attention step: positions %lld + %d beyond the 32-bit slot positions", pos0, m);
+  XTG_CHECK(c->ring || pos0 <= c->slots - m, "attention step: context full (%lld + %d > %lld slots)", pos0, m,
             c->slots);
   XTG_CHECK(q && k && v && g && gscale, "attention step: NULL argument");
   const AttnPlan p = attn_plan(*c, m, heads, pos0, window);

@@ -389,7 +389,7 @@ void DorySession::sublayer_decode(Layer& L, int m, long long pos0, int inst, boo
 void DorySession::run_chunk(const float* x, int m, long long pos0, bool keep_pending) {
   // packs/dory/dory.cpp:520-544 from the embedding rows; x's operand is in op_h_ on exit
   XTG_CHECK(m >= 1 && m <= kChunkRows, "dory: %d rows per chunk (1..%d)", m, kChunkRows);
-  XTG_CHECK(pos0 >= 0 && pos0 + m <= c_.context, "context full: %lld + %d > %lld tokens", pos0, m,
+  XTG_CHECK(pos0 >= 0 && pos0 <= c_.context - m, "context full: %lld + %d > %lld tokens", pos0, m,
             (long long)c_.context);
   const int H = c_.hidden;
   const size_t bytes = size_t(m) * H * sizeof(float);
@@ -492,7 +492,7 @@ void DorySession::prefill(const float* x, int n, long long pos0, int want, float
   XTG_CHECK(want == XTG_LOGITS_NONE || want == XTG_LOGITS_LAST || want == XTG_LOGITS_ALL, "dory: logits mode %d",
             want);
   XTG_CHECK(want == XTG_LOGITS_NONE || logits, "dory: NULL logits");
-  XTG_CHECK(pos0 >= 0 && pos0 + n <= c_.context, "context full: %lld + %d > %lld tokens", pos0, n,
+  XTG_CHECK(pos0 >= 0 && pos0 <= c_.context - n, "context full: %lld + %d > %lld tokens", pos0, n,
             (long long)c_.context);
   for (int off = 0; off < n; off += kChunkRows) {
     const int m = std::min(kChunkRows, n - off);
