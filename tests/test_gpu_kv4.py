@@ -307,14 +307,14 @@ def test_positions_whose_end_passes_64_bits_are_refused(hip, pkg, wl, pos):
         assert not read(hip, c, 0, 40)[0].any()
     w = wl.DoryWeights(wl.DORY_TINY, seed=3, context=256)
     d = hip.dory(w)
-    x = hip.array(shape=(2, w.cfg["hidden"]))
-    for call in (lambda: d.forward(x, 2, pos, None), lambda: d.prefill(x, 2, pos, pkg.LOGITS_NONE)):
+    x, y = hip.array(shape=(2, w.cfg["hidden"])), hip.array(shape=(2, w.cfg["vocab"]))
+    for call in (lambda: d.forward(x, 2, pos, y), lambda: d.prefill(x, 2, pos, pkg.LOGITS_NONE)):
         with pytest.raises(pkg.XtgError, match="context full"):
             call()
     d.destroy()
     for c in caches:
         c.destroy()
-    for b in (a, x):
+    for b in (a, x, y):
         b.free()
 
 
