@@ -318,6 +318,68 @@ def test_positions_whose_end_passes_64_bits_are_refused(hip, pkg, wl, pos):
         b.free()
 
 
+class Rows:
+    """What the bindings ask of a torch tensor."""
+
+    def __init__(self, dtype="torch.float32", device=0, n=512, whole=True, at=4096):
+        self.dtype, self.a = dtype, (device, n, whole, at)
+
+    def get_device(self):
+        return self.a[0]
+
+    def numel(self):
+        return self.a[1]
+
+    def is_contiguous(self):
+        return self.a[2]
+
+    def data_ptr(self):
+        return self.a[3]
+
+
+def test_arrays_that_are_not_the_rows_of_the_call(pkg):
+    """Without a GPU: an array of another dtype than the row type (BF16 rows at the default, FP32), in host memory or on
+    another device, strided, too short or freed is refused before its address goes anywhere."""
+    class Backend:
+        device = 0
+
+    freed = pkg.DeviceArray.__new__(pkg.DeviceArray)
+    freed.b, freed.ptr, freed.nbytes, freed.dtype = Backend, None, 2048, np.dtype(np.float32)
+    for a, kind, what in [(Rows("torch.bfloat16"), pkg.X_F32, "row type FP32"), (Rows(), pkg.X_BF16, "row type BF16"),
+                          (Rows("torch.float16"), pkg.X_BF16, "row type BF16"), (Rows("torch.int64"), pkg._I32, "int32"),
+                          (Rows(), 7, "row type"), (Rows(device=-1), pkg.X_F32, "memory"), (Rows(device=1), pkg.X_F32, "memory"),
+                          (Rows(whole=False), pkg.X_F32, "contiguous"), (Rows(n=511), pkg.X_F32, "511 elements"),
+                          (np.zeros(512, np.float32), pkg.X_F32, "device memory"), (freed, pkg.X_F32, "freed")]:
+        with pytest.raises(pkg.XtgError, match=what):
+            pkg._device_ptr(Backend, "q", a, 512, kind)
+    for a, kind in [(Rows(), pkg.X_F32), (Rows("torch.bfloat16"), pkg.X_BF16), (Rows("uint16"), pkg.X_BF16), (4096, 7)]:
+        assert pkg._device_ptr(Backend, "q", a, 512, kind) == 4096
+    assert pkg._device_ptr(Backend, "q", None, 512, 0) is None and pkg._device_ptr(Backend, "q", Rows(n=0, at=0), 0, 0) == 0
+
+
+@gpu
+def test_arrays_of_another_type_are_refused(hip, pkg):
+    """The default row type is FP32: BF16 arrays without x_dtype would be read and written at twice their size."""
+    cache = hip.kv_cache(2, 64, 40, 0, 2)
+    f, b, out = (hip.array(shape=(4, 4, 64), dtype=t) for t in (np.float32, np.uint16, np.float32))
+    i, j, short, host = hip.array(shape=(4,), dtype=np.int64), hip.array(shape=(3,), dtype=np.int32), hip.array(shape=(511,)), np.zeros((4, 4, 64))
+    good = dict(cache=cache, q=f, k=f, v=f, out=out, n_q=4, pos0=3, heads=4, kv_heads=2, head_dim=64)
+    hip.attention_ext(**good)
+    hip.attention_ext(**dict(good, q=f.ptr, k=f.ptr, out=out.ptr))   # addresses are the caller's
+    for change in [dict(q=b), dict(k=b), dict(out=b), dict(q=host), dict(first=i), dict(end=j), dict(slopes=i), dict(v=short),
+                   dict(out=short), dict(x_dtype=pkg.X_BF16)]:
+        with pytest.raises(pkg.XtgError):
+            hip.attention_ext(**dict(good, **change))
+    for call in (cache.write, cache.read):
+        for k, v, x in [(b, b, pkg.X_F32), (f, b, pkg.X_F32), (f, f, pkg.X_BF16), (host, f, pkg.X_F32), (f, short, pkg.X_F32)]:
+            with pytest.raises(pkg.XtgError):
+                call(0, 4, k, v, x)
+    hip.finish()
+    for a in (f, b, out, i, j, short):
+        a.free()
+    cache.destroy()
+
+
 def test_null_arguments_are_refused(pkg):
     """Without a GPU: a NULL handle or cache is an error, not a fault."""
     lib, err = pkg.lib(), ctypes.create_string_buffer(200)

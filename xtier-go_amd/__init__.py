@@ -156,7 +156,8 @@ def lib():
     return _lib
 
 
-_ErrBuf = ctypes.c_char * 2048
+_ERR_LEN = 2048
+_ErrBuf = ctypes.c_char * _ERR_LEN
 
 
 def _errbuf():
@@ -177,6 +178,60 @@ def _ptr(a):
     if isinstance(a, np.ndarray):
         return a.ctypes.data
     return a.data_ptr()   # torch.Tensor
+
+
+# What elements an array holds: X_F32, X_BF16 (as 16-bit integers too, which is how numpy holds them) or _I32. Tensors'
+# dtypes are torch's own objects, looked up by name once.
+_I32 = -2
+_KIND_OF = {"float32": X_F32, "bfloat16": X_BF16, "uint16": X_BF16, "int16": X_BF16, "int32": _I32}
+_kinds = {}
+
+
+def _device_ptr(b, name, a, n, kind):
+    """Address of n elements of a kind in backend b's device memory. An array that is elsewhere, of another dtype, strided,
+    too short or freed is refused: the kernels would read or write past it. An address (an int) or None is taken as it is."""
+    if a is None:
+        return None
+    cls = a.__class__
+    if cls is not DeviceArray and cls is not int:
+        try:   # a torch tensor as it should be
+            if _kinds[a.dtype] == kind and a.numel() >= n and a.is_contiguous() and a.get_device() == b.device:
+                return a.data_ptr()
+        except (AttributeError, KeyError):
+            pass
+    if isinstance(a, int):
+        return a
+    if isinstance(a, DeviceArray):
+        at, size, here, whole = a.ptr, a.nbytes // a.dtype.itemsize, a.b.device == b.device, True
+    elif hasattr(a, "get_device"):
+        at, size, here, whole = a.data_ptr(), a.numel(), a.get_device() == b.device, a.is_contiguous()
+    else:
+        raise XtgError("%s is not in device memory" % name)
+    if a.dtype not in _kinds:
+        _kinds[a.dtype] = _KIND_OF.get(str(a.dtype).replace("torch.", ""))
+    if _kinds[a.dtype] != kind:
+        want = {X_F32: "row type FP32", X_BF16: "row type BF16", _I32: "int32"}.get(kind, "unknown row type %s" % kind)
+        raise XtgError("%s is %s, not of the call's %s" % (name, a.dtype, want))
+    if not here:
+        raise XtgError("%s is not in the memory of the backend's device" % name)
+    if not whole:
+        raise XtgError("%s is not contiguous" % name)
+    if size < n:
+        raise XtgError("%s has %d elements, the call's rows of it take %d" % (name, size, n))
+    if n > 0 and not at:
+        raise XtgError("%s has been freed" % name)
+    return at
+
+
+def _device_rows(b, k, v, n, kind):
+    """_device_ptr of a call's k and v, in one step where both are torch tensors as they should be."""
+    try:
+        if (_kinds[k.dtype] == kind and v.dtype is k.dtype and k.numel() >= n and v.numel() >= n and k.is_contiguous() and
+                v.is_contiguous() and k.get_device() == v.get_device() == b.device):
+            return k.data_ptr(), v.data_ptr()
+    except (AttributeError, KeyError):
+        pass
+    return _device_ptr(b, "k", k, n, kind), _device_ptr(b, "v", v, n, kind)
 
 
 class _Address(int):
@@ -242,6 +297,7 @@ class HipBackend:
     """One xtg_hip handle (a device, its stream and prepared weights)."""
 
     def __init__(self, device=0):
+        self.device = device
         err = _errbuf()
         self.h = lib().xtg_hip_open(json.dumps({"device": device}).encode(), err, len(err))
         if not self.h:
@@ -465,9 +521,12 @@ class HipBackend:
         v None: the call's own rows are in the cache. q, k, v, out: device rows of x_dtype; slopes: device FP32
         [heads]; first, end: device int32 [n_q]."""
         sc = head_dim ** -0.5 if scale is None else scale
-        a = AttnExt(n_q, pos0, heads, kv_heads, head_dim, window, sc, _ptr(q), _ptr(k), _ptr(v),
-                    cache.h if cache is not None else None, _ptr(out), x_dtype, softcap, _ptr(slopes), _ptr(first),
-                    _ptr(end))
+        nq, nk = n_q * heads * head_dim, n_q * kv_heads * head_dim
+        a = AttnExt(n_q, pos0, heads, kv_heads, head_dim, window, sc, _device_ptr(self, "q", q, nq, x_dtype),
+                    _device_ptr(self, "k", k, nk, x_dtype), _device_ptr(self, "v", v, nk, x_dtype),
+                    cache.h if cache is not None else None, _device_ptr(self, "out", out, nq, x_dtype), x_dtype, softcap,
+                    _device_ptr(self, "slopes", slopes, heads, X_F32), _device_ptr(self, "first", first, n_q, _I32),
+                    _device_ptr(self, "end", end, n_q, _I32))
         err = self._err
         _check(lib().xtg_hip_attention_ext(self.h, ctypes.byref(a), err, len(err)), err)
 
@@ -616,14 +675,18 @@ class KvCache:
 
     def write(self, pos, n, k, v, x_dtype=X_F32):
         """store for device rows of x_dtype (queued)."""
-        err = self.b._err
-        _check(lib().xtg_hip_kv_write(self.b.h, self.h, pos, n, _ptr(k), _ptr(v), x_dtype, err, len(err)), err)
+        b = self.b
+        k, v = _device_rows(b, k, v, n * self.kv_heads * self.head_dim, x_dtype)
+        if _lib.xtg_hip_kv_write(b.h, self.h, pos, n, k, v, x_dtype, b._err, _ERR_LEN):
+            _check(-1, b._err)
 
     def read(self, pos, n, k, v, x_dtype=X_F32):
         """The rows of positions pos .. pos + n - 1 as the cache holds them into device k, v [n][kv_heads][head_dim] of
         x_dtype, zeros where it holds none (queued)."""
-        err = self.b._err
-        _check(lib().xtg_hip_kv_read(self.b.h, self.h, pos, n, _ptr(k), _ptr(v), x_dtype, err, len(err)), err)
+        b = self.b
+        k, v = _device_rows(b, k, v, n * self.kv_heads * self.head_dim, x_dtype)
+        if _lib.xtg_hip_kv_read(b.h, self.h, pos, n, k, v, x_dtype, b._err, _ERR_LEN):
+            _check(-1, b._err)
 
     def store_host(self, pos, k, v):
         """Convenience: upload FP32 host rows, then store them."""
