@@ -526,3 +526,14 @@ def test_refusals(hip, pkg):
     other.destroy()
     hip.finish()
     cache.destroy()
+
+
+def test_a_destroyed_cache_is_not_no_cache(hip, pkg):
+    cache, a, out = hip.kv_cache(2, 128, 64, 0, 2), hip.array(shape=(1, 8, 128)), hip.array(shape=(1, 8, 128))
+    hip.attention_ext(cache, a, a, a, out, 1, 3, 8, 2, 128)
+    hip.finish()
+    cache.destroy()
+    with pytest.raises(pkg.XtgError, match="destroyed"):
+        hip.attention_ext(cache, a, a, a, out, 1, 3, 8, 2, 128)
+    for x in (a, out):
+        x.free()

@@ -521,6 +521,8 @@ class HipBackend:
         v None: the call's own rows are in the cache. q, k, v, out: device rows of x_dtype; slopes: device FP32
         [heads]; first, end: device int32 [n_q]."""
         sc = head_dim ** -0.5 if scale is None else scale
+        if cache is not None and not cache.h:   # NULL would mean no cache
+            raise XtgError("attention_ext: the cache has been destroyed")
         nq, nk = n_q * heads * head_dim, n_q * kv_heads * head_dim
         a = AttnExt(n_q, pos0, heads, kv_heads, head_dim, window, sc, _device_ptr(self, "q", q, nq, x_dtype),
                     _device_ptr(self, "k", k, nk, x_dtype), _device_ptr(self, "v", v, nk, x_dtype),
