@@ -297,6 +297,26 @@ def test_tiny_and_huge_queries(hip, size, n, heads):
     c.free()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp8"])
+@pytest.mark.parametrize("up", [114, -114])
+@pytest.mark.parametrize("n,heads", [(2, 8), (45, 8), (26, 64)])
+def test_huge_queries_over_small_keys(hip, dtype, up, n, heads):
+    """Queries and keys near opposite ends of BF16's exponents, whose products are ordinary: an FP8 key's codes are, times
+    such a query without the key's scale, beyond FP32."""
+    rng = np.random.default_rng(n)
+    ctx, kvh, d = 300, 2, 128
+    c = Call(hip, rng, dtype, n, 0, heads, kvh, d, own=False, slots=ctx)
+    kc, vc = c.unit(rng, (ctx, kvh, d)) * np.float32(2.0 ** -up), rng.standard_normal((ctx, kvh, d)).astype(np.float32)
+    q = c.unit(rng, (n, heads, d)) * np.float32(d * 2.0 ** up)
+    c.fill(0, kc, vc)
+    for x in c.dev + [c.out]:
+        x.free()
+    c.set(0, kc, vc, q, kc[:n], vc[:n])
+    c.check(pos0=ctx - n)
+    c.check(pos0=ctx - n, softcap=5.0, window=90)
+    c.free()
+
+
 @pytest.mark.parametrize("dtype", ["nvfp4", "bf16", "fp8"])
 @pytest.mark.parametrize("n,heads", [(1, 8), (6, 8), (70, 8), (26, 64)])
 def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(hip, dtype, n, heads):

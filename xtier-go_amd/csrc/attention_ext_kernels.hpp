@@ -30,6 +30,7 @@
 #include <cfloat>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "attention_ext.hpp"
 #include "common.hpp"
@@ -84,28 +85,42 @@ __device__ inline void row_chunks(const void* p, int bf16, bool live, A at, bf16
   }
 }
 
-// The q-col's N operand chunks: to f16 times a power of two that brings the largest magnitude over the q-col's lanes
-// (`join`) to 2^8 .. 2^9, or as they are. Returns the power of two that a product has to be multiplied by.
-template <int N, class J>
-__device__ inline int to_operand(const bf16x8 (&x)[N], f16x8 (&q)[N], J join) {
-  uint32_t m = 0;
+// The q-col's N operand chunks. SCALED: times a power of two that brings the largest magnitude over the q-col's lanes (`join`)
+// to 2^8 .. 2^9, for f16; for FP8 caches (BF16 operands) only where the wave has a magnitude of 2^65 or more, since codes'
+// products are multiplied by their key's scale afterwards and could pass FP32 before it (scaling all of them cost 45 rows
+// over 4000 keys 5 %). Else as they are. Returns the power of two that a product has to be multiplied by.
+template <bool SCALED, int N, class X8, class J>
+__device__ inline int to_operand(const bf16x8 (&x)[N], X8 (&q)[N], J join) {
+  bool scaled = SCALED;
+  if constexpr (SCALED && std::is_same_v<X8, bf16x8>) {
+    uint32_t both = 0;   // the two highest bits of an exponent
 #pragma unroll
-  for (int c = 0; c < N; ++c)
+    for (int c = 0; c < N; ++c) {
+      const uint4 w = __builtin_bit_cast(uint4, x[c]);
+      both |= (w.x & w.x << 1) | (w.y & w.y << 1) | (w.z & w.z << 1) | (w.w & w.w << 1);
+    }
+    scaled = __ballot(both & 0x40004000u) != 0;
+  }
+  if (SCALED && scaled) {
+    uint32_t m = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint((float)x[c][e]) & 0x7fffffffu);
-  m = __float_as_uint(join(__uint_as_float(m & 0xff800000u)));   // powers of two, or infinity: ordered as floats
-  const int ex = m == 0u || m >= 0x7f800000u ? 0 : max(int(m >> 23) - 127 - 8, -126);   // (2^-ex is finite)
-  const float down = ldexpf(1.f, -ex);
+    for (int c = 0; c < N; ++c)
 #pragma unroll
-  for (int c = 0; c < N; ++c)
+      for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint((float)x[c][e]) & 0x7fffffffu);
+    m = __float_as_uint(join(__uint_as_float(m & 0xff800000u)));   // powers of two, or infinity: ordered as floats
+    constexpr int kLeast = std::is_same_v<X8, f16x8> ? -126 : 0;   // (2^-ex is finite; FP8: never up)
+    const int ex = m == 0u || m >= 0x7f800000u ? 0 : max(int(m >> 23) - 127 - 8, kLeast);
+    const float down = ldexpf(1.f, -ex);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[c][e] = (_Float16)((float)x[c][e] * down);
-  return ex;
-}
-template <int N, class J>
-__device__ inline int to_operand(const bf16x8 (&x)[N], bf16x8 (&q)[N], J) {
+    for (int c = 0; c < N; ++c)
 #pragma unroll
-  for (int c = 0; c < N; ++c) q[c] = x[c];
+      for (int e = 0; e < 8; ++e) q[c][e] = (float)x[c][e] * down;
+    return ex;
+  }
+  if constexpr (std::is_same_v<X8, bf16x8>) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) q[c] = x[c];
+  }
   return 0;
 }
 
@@ -567,7 +582,7 @@ struct FewQueries {
       sc[qb] = score_of(a, live ? head : 0, 1.f, 0);
     }
   }
-  template <class X8>
+  template <bool SCALED, class X8>
   __device__ void operand(const ExtArgs& a, float global, X8 (&q)[QB][D / 32]) {
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
@@ -575,7 +590,7 @@ struct FewQueries {
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) x[qb][c] = -x[qb][c];
       }
-      sc[qb].f = score_factor(a, global, to_operand(x[qb], q[qb], [](float v) { return xor32_max(xor16_max(v)); }));
+      sc[qb].f = score_factor(a, global, to_operand<SCALED>(x[qb], q[qb], [](float v) { return xor32_max(xor16_max(v)); }));
     }
   }
 };
@@ -604,7 +619,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, QB * D > 256 ? 1 : 2) ext_few_
     bf16x8 q[QB][D / 32];
     FewQueries<D, QB, OwnTile<D, T>> rows;
     rows.load(a, h, col0, lane);
-    rows.operand(a, 1.f, q);
+    rows.template operand<false>(a, 1.f, q);
     const int t = (split - a.splits) * kExtWaves + wave, p = a.pos0 + 32 * t;   // (p + 32 can pass 2^31)
     bool any = false;   // a q-col that sees one of the tile's keys
 #pragma unroll
@@ -638,7 +653,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, QB * D > 256 ? 1 : 2) ext_few_
       tile.load_k(a, h, t, lane);
       int4 p0 = sp[t * 8], p1 = sp[t * 8 + 4];
       tile.load_v(a, h, t, lane);
-      rows.operand(a, T == kNvfp4 ? a.kglobal : 1.f, q);
+      rows.template operand<T != kBf16>(a, T == kNvfp4 ? a.kglobal : 1.f, q);
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) rows.span[qb] = cached_span(a, rows.span[qb]);
       for (; t < t_end; t += kExtWaves) {
@@ -1218,7 +1233,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
 #pragma unroll
       for (int c = 0; c < R::NS; ++c) x[c] = -x[c];
     }
-    const int ex = to_operand(x, q, [](float y) { return xor32_max(y); });
+    const int ex = to_operand<S != kBf16>(x, q, [](float y) { return xor32_max(y); });
     sc = score_of(a, live ? head : 0, global, ex);
 #pragma unroll
     for (int c = 0; c < QL; ++c) ql[c * 256] = q[R::NS - QL + c];
