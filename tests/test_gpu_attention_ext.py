@@ -123,6 +123,66 @@ def test_changed_scores_of_many(hip, d, dtype, kw):
     c.free()
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", ["nvfp4", "bf16", "fp8"])
+@pytest.mark.parametrize("n,ctx", [(1, 3000), (2, 8200)])
+def test_more_than_sixteen_records(hip, d, dtype, n, ctx):
+    """A decoded token over a long cache, whose records several groups of lanes join."""
+    c = Call(hip, np.random.default_rng(ctx + d), dtype, n, ctx, *HEADS[d], d)
+    hip.profile()
+    c.check()
+    names = hip.profile_report()
+    hip.profile(False)
+    assert "ext_merge_kernel<%d, %d, %d>" % (d, o.KV[dtype], 1024 // d) in names, names
+    c.check(softcap=8.0, slopes=np.linspace(0.001, 0.01, c.heads))
+    c.check(first=np.full(n, ctx - 40))   # most records saw nothing
+    c.free()
+
+
+@pytest.mark.parametrize("n,heads", [(1, 8), (7, 8), (45, 8), (50, 64)])
+def test_weights_over_an_nvfp4_cache_keep_eleven_bits(hip, n, heads):
+    """FP32 rows out and no keys of the call's own: half a step of f16's weights is the bound that decides."""
+    c = Call(hip, np.random.default_rng(n), "nvfp4", n, 600, heads, 2, 128, x_dtype=o.F32, own=False)
+    c.check(pos0=600 - n)
+    c.check(pos0=500, softcap=9.0, window=100)
+    c.free()
+
+
+@pytest.mark.parametrize("dtype", ["nvfp4", "bf16", "fp8", "none"])
+@pytest.mark.parametrize("n,heads", [(1, 8), (20, 8), (45, 64)])
+def test_the_first_and_last_key_of_a_span(hip, dtype, n, heads):
+    """The keys at both ends of what a row sees and beside them outweigh all others, so that one too many or too few shows."""
+    rng = np.random.default_rng(n)
+    ctx, kvh, d = 0 if dtype == "none" else 3000, 2, 128
+    n = n if dtype != "none" else n + 3000
+    c = Call(hip, rng, dtype, n, ctx, heads, kvh, d, slots=ctx)
+    u = c.unit(rng, (1, 1, d))
+    kc, vc = c.unit(rng, (ctx, kvh, d)), rng.standard_normal((ctx, kvh, d)).astype(np.float32)
+    k, v = c.unit(rng, (n, kvh, d)), rng.standard_normal((n, kvh, d)).astype(np.float32)
+    q = np.repeat(np.repeat(u * d, n, 0), heads, 1).astype(np.float32)
+    both, vals = np.concatenate([kc, k]), np.concatenate([vc, v])
+    spans = [(1023, 2048), (1000, 1001), (31, 2977)] + ([(2990, 3000)] if ctx else [])
+    for lo, hi in spans:
+        for p in (lo - 1, lo, hi - 1, hi):
+            both[p] = u
+        vals[lo - 1], vals[hi] = 50.0, -50.0
+    if ctx:
+        c.fill(0, both[:ctx], vals[:ctx])
+    for x in c.dev + [c.out]:
+        x.free()
+    c.set(0, both[:ctx], vals[:ctx], q, both[ctx:], vals[ctx:])
+    if dtype == "none":   # (rows enough for any kernel; a few of them are looked at)
+        c.q = c.q[-3:]
+    for lo, hi in spans:
+        if ctx:
+            c.check(first=np.full(n, lo), end=np.full(n, hi))
+        else:
+            got = c.run(first=np.full(n, lo), end=np.full(n, hi))[-3:]
+            out, size, most = o.attend(c.q, *c.keys, c.at, n - 3, d ** -0.5, first=np.full(3, lo), end=np.full(3, hi))
+            assert (np.abs(got - out) <= o.tolerance(out, size, most, d, 8, c.x)).all()
+    c.free()
+
+
 def test_key_splits_of_many(hip):
     """Enough tiles to be split over work-groups, with a window and documents that leave some of them without keys."""
     c = Call(hip, np.random.default_rng(5), "nvfp4", 32, 3000, 64, 2, 128)
