@@ -217,7 +217,8 @@ int xtg_hip_attention_noalloc(xtg_hip* h, const xtg_attn_args* a, char* err, int
  * Rows are x_dtype: BF16, or FP32, of which q, k and v are rounded to BF16 as they are read (as a cache rounds what it
  * stores) and out is not. Scores, their maxima and sums and the output are held in FP32; the softmax weights enter the
  * product with V as f16 (11 bits; NVFP4 caches) or BF16 (8 bits; others, and own keys). No gradient. head_dim 64, 128 or
- * 256; n_q * heads up to 2^30; out overlaps no input. Queued; the first call of a shape sizes scratch memory (make it before a graph capture). */
+ * 256; n_q * heads up to 2^30; out overlaps no input. Queued; the first call of a number of rows, heads and a cache's size
+ * sizes scratch memory, for every position of the cache (make it before a graph capture). */
 typedef struct xtg_attn_ext {
   int n_q;
   int64_t pos0;

@@ -12,7 +12,8 @@ namespace xtg::hip {
 
 // Calls of up to this many q-cols take ext_few_kernel, which starts sooner (one launch less, no barriers) and dequantises
 // a tile again for every 32 of them: over 4000 NVFP4 keys of 128 dims, 32 / 8 heads, 384 q-cols took 27.6 us (many: 44.1),
-// 768 51.6 (63.6), 1024 64.4 (53.9).
+// 768 51.6 (63.6), 1024 64.4 (53.9). One number of q-cols for every length and head size: other shapes were not measured, and
+// the longer the cache, the fewer q-cols it takes for the other kernel to be faster.
 constexpr int kFewCols = 768;
 
 // The plan for the cache's slots lo .. slots - 1.

@@ -8,17 +8,20 @@
 //
 // Operands have 16 bits: BF16 for BF16 and FP8 caches and the call's own keys, f16 for NVFP4 caches, whose values
 // (E2M1 code times E4M3 scale) f16 holds exactly and whose weights then keep 11 bits; q, BF16, is exact in both (in f16
-// times a power of two for each q-col). Scores, sums and accumulators are FP32.
+// times a power of two for each q-col, elements under 2^-25 of its largest to within 2^-33 of that). Weights beside BF16
+// values keep 8 bits: one type for both operands, which f16's range rules out for V, and a second term of each weight would
+// be half again as many matrix ops. An output is then off by up to 2^-8 of its weighted |v|, of the size of the rounding
+// of a BF16 output. Scores, sums and accumulators are FP32.
 //
 //   ext_few_kernel: up to some hundred q-cols (kFewCols; a decode or verify step, a short turn). Each wave takes 32-slot
 //     tiles of its own straight from the cache's operand layout into registers; work-groups split the tiles of a KV head,
 //     and more of them take the call's own keys. One row is bound by the cache's bytes (32768 NVFP4 keys of 8 heads of 128
-//     dims: 9 us for 38 MB, 4.2 TB/s), more rows by the vector ALUs (a tile is dequantised for every 32 q-cols).
+//     dims: 11.1 us for 38 MB, 3.4 TB/s), more rows by the vector ALUs (a tile is dequantised for every 32 q-cols).
 //   ext_rows_kernel: more q-cols (a prompt chunk). Four waves of 32 q-cols share tiles through LDS: each is dequantised
 //     once per work-group. The call's own keys are packed as BF16 tiles first (ext_pack_kernel). Bound by what a SIMD issues:
-//     the matrix ops of its two waves (36 % of the time at 2.1 GHz) and their vector ALU work (50 %: exponentials, masks,
-//     dequantisation) hardly overlap, while LDS is busy for 28 %. 512 rows over 16384 NVFP4 keys, 32 / 8 heads of 128 dims:
-//     154 us, 0.9 PFLOP/s; 1500 capped rows over 2500 keys, 16 / 4 heads of 256 dims: 93 us, 0.52.
+//     the matrix ops of its two waves (38 % of the time at 2.1 GHz) and their vector ALU work (48 %: exponentials, masks,
+//     dequantisation) hardly overlap, while LDS is busy for 29 %. 512 rows over 16384 NVFP4 keys, 32 / 8 heads of 128 dims:
+//     154 us, 0.9 PFLOP/s; 1500 capped rows over 2500 keys, 16 / 4 heads of 256 dims: 96 us, 0.50.
 //   ext_merge_kernel: joins the records of a q-col in their order.
 //
 // Values that are not finite: a score that is masked is replaced, so a key's only reach the q-cols that see it. Not so a

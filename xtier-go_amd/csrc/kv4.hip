@@ -4,8 +4,8 @@
 // a decoded token's rows are one step of a few loads in each. Of K a thread takes a few dims of a key, rows read as they
 // lie; of V a few dims of 8 keys, so that it reads and writes whole words of codes. A ring's last rows and first rows can
 // share a tile, which is still one work-group's in a store, since a V word holds the codes of 8 slots and the nibbles of
-// other rows stay. 32749 BF16 rows of 8 heads of 128 dims written and then read: 81 us for 344 MB, 4.2 TB/s (a copy of
-// 4 GB reaches 4.7); one row 9.3, which is the two calls' queueing.
+// other rows stay. 32749 BF16 rows of 8 heads of 128 dims written and then read: 82 us for 344 MB, 4.2 TB/s (a copy of
+// 4 GB reaches 4.7); one row 9.5, which is the two calls' queueing.
 #include <algorithm>
 
 #include "attention_ext.hpp"
