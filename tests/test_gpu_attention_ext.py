@@ -297,6 +297,36 @@ def test_scales_and_sharp_softmaxes(hip, scale, n, heads):
     c.free()
 
 
+@pytest.mark.parametrize("dtype", ["nvfp4", "bf16", "fp8", "none"])
+@pytest.mark.parametrize("scale", [1e4, 1e6, 1e8, 1e10, 1e30])
+@pytest.mark.parametrize("n,heads", [(2, 8), (45, 8), (26, 64), (150, 64)])
+def test_scores_beyond_the_integers_of_fp32(hip, dtype, scale, n, heads):
+    """Scores up to 1e32 of either sign, whose last bits are worth far more than an exponential's range: one key stands out
+    by half of them, and its value is the output."""
+    rng = np.random.default_rng(n)
+    ctx, kvh, d = 0 if dtype == "none" else 300, 2, 128
+    c = Call(hip, rng, dtype, n, ctx, heads, kvh, d)
+    u = c.unit(rng, (1, 1, d))
+    q = np.repeat(np.repeat(u * d, n, 0), heads, 1).astype(np.float32)
+    vc, v = (rng.standard_normal((m, kvh, d)).astype(np.float32) for m in (ctx, n))
+    for sign in (1, -1):   # the best key: the largest score, or the one least below zero
+        kc, k = (np.repeat(np.repeat((0.5 if sign > 0 else -1.0) * u, m, 0), kvh, 1).astype(np.float32) for m in (ctx, n))
+        (kc if ctx else k)[0] = (1.0 if sign > 0 else -0.5) * u
+        if ctx:
+            c.fill(0, kc, vc)
+        for x in c.dev + [c.out]:
+            x.free()
+        c.set(0, kc, vc, q, k, v)
+        want = np.repeat(c.keys[1][0], heads // kvh, 0)
+        for kw in (dict(), dict(slopes=np.full(heads, 0.01)), dict(window=n + 200 if ctx else 0, first=np.zeros(n))):
+            got = c.run(scale=scale, **kw)
+            if kw.get("window"):   # the best key is out of the window: all are alike
+                assert np.isfinite(got).all() and (np.abs(got) <= np.abs(c.keys[1]).max()).all()
+            else:   # half a step of a weight of 8 bits (or of its product with an FP8 value's scale), and of a BF16 output
+                assert (np.abs(got - want) <= np.abs(want) * (2.0 ** -7 + 2.0 ** -14)).all()
+    c.free()
+
+
 @pytest.mark.parametrize("cap", [1e-38, 1e-3, 1024.0])
 @pytest.mark.parametrize("n,heads", [(2, 8), (26, 64)])
 def test_tiny_and_large_caps(hip, cap, n, heads):

@@ -220,6 +220,9 @@ template <int MOD>
 __device__ inline float finish(const Score& s, float x, float minus) {
   return MOD == kCap ? fmaf(-2.f * s.top, x, s.top - minus) : MOD ? x - minus : fmaf(x, s.f, -minus);
 }
+// From here on a plain score's product is rounded before the maximum, which is rounded, is subtracted: in one operation the
+// best key's exponent is off by up to half an ulp of the maximum, 1/4 below and more than weights have range for from 2^28 on.
+constexpr float kLarge = 8388608.f;   // 2^23
 
 __device__ inline bool not_finite(float x) { return !(fabsf(x) <= FLT_MAX); }
 
@@ -1056,6 +1059,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
     constexpr int QL = D == 256 && S != kBf16 ? 2 : 0;   // chunks of q in LDS, for the same reason
     X8* const ql = reinterpret_cast<X8*>(smem + R::kLds - 4096 * QL) + wave * 64 + lane;
     Score sc;
+    float sc_f = 1.f;   // Score::f of the tile's plain scores (1: they have been multiplied)
     bf16x8 x[R::NS];
     row_chunks(a.q, a.bf16, live, [&](int c) { return (live ? q_at : size_t(8 * half)) + size_t(16 * c); }, x);
     Stage<D, S> stage;
@@ -1192,6 +1196,16 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = best<MOD>(mx, y[b][r]);
       mx = xor32_max(finish<MOD>(sc, mx, 0.f));
+      if constexpr (MOD == 0) {
+        sc_f = sc.f;
+        if (__ballot(fabsf(mx) >= kLarge && fabsf(mx) <= FLT_MAX)) {
+          sc_f = 1.f;
+#pragma unroll
+          for (int b = 0; b < R::KB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) y[b][r] *= sc.f;
+        }
+      }
       if (__ballot(mx > m + kSlack)) {
         const float to = mx > m + kSlack ? mx : m;
         const float corr = __builtin_amdgcn_exp2f(m - (to == -INFINITY ? 0.f : to));
@@ -1218,7 +1232,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            float p = __builtin_amdgcn_exp2f(finish<MOD>(sc, y[b][4 * j + r], ref));
+            float p = __builtin_amdgcn_exp2f(MOD ? finish<MOD>(sc, y[b][4 * j + r], ref) : fmaf(y[b][4 * j + r], sc_f, -ref));
             sum += p;
             if constexpr (S == kFp8) p *= v4[r];
             w[2 * b + (j & 1)][(j >> 1) * 4 + r] = p;
