@@ -137,7 +137,7 @@ void xtg_hip_kv_destroy(xtg_hip* h, xtg_hip_kv* kv);
 /* Replaces KvCache::store (kv.h:35, kv.cpp:75-112): rows of positions pos .. pos + n - 1 from device FP32 k, v
  * [n][kv_heads][head_dim], rounded to BF16 (nearest even), or for FP8 scaled by amax / 448 of each (row, head)
  * and rounded as kv.cpp:19-40 does; a ring keeps the last `ring` rows; queued. A linear cache refuses positions
- * beyond its capacity ("KV cache full"). */
+ * beyond its capacity ("KV cache full"). Into an NVFP4 cache it is xtg_hip_kv_write, which wants rows 16-byte aligned. */
 int xtg_hip_kv_store(xtg_hip* h, xtg_hip_kv* kv, int64_t pos, int n, const float* k, const float* v, char* err,
                      int err_len);
 /* An NVFP4 cache's values are code * scale * global, with one global for K and one for V: powers of two from 2^-60 to
