@@ -26,6 +26,7 @@ extern "C" {
 
 typedef struct xtg_hip xtg_hip;
 typedef struct xtg_hip_kv xtg_hip_kv;
+typedef struct xtg_hip_paged xtg_hip_paged;
 
 /* An NVFP4 weight [n_out][k] in ModelOpt's layout: E2M1 codes two per byte (element 2j in the low nibble of byte
  * j), one E4M3 scale per 16 inputs, one FP32 scale for the tensor; w[n][j] = e2m1 * e4m3(scale[n][j/16]) * global.
@@ -237,6 +238,77 @@ typedef struct xtg_attn_ext {
   const int32_t* end;     /* device [n_q], or NULL */
 } xtg_attn_ext;
 int xtg_hip_attention_ext(xtg_hip* h, const xtg_attn_ext* a, char* err, int err_len);
+
+/* ---------------------------------------------------------------------------------------- paged caches */
+
+/* Many sequences' keys and values in one pool of pages (no counterpart in the reference, whose sessions own a cache each).
+ * A page holds page_size positions (a power of two from 32 to 4096) of every KV head, in any of the cache dtypes; which
+ * page holds which positions of which sequence is the caller's table, in device memory, so that a page is given to another
+ * sequence, or shared by the sequences of a common prefix, by writing its number there. New pages are zeros. NULL on
+ * failure. */
+xtg_hip_paged* xtg_hip_paged_create(xtg_hip* h, int kv_heads, int head_dim, int64_t pages, int page_size, int dtype,
+                                    char* err, int err_len);
+void xtg_hip_paged_destroy(xtg_hip* h, xtg_hip_paged* c);
+/* xtg_hip_kv_globals for an NVFP4 pool; before anything is written. */
+int xtg_hip_paged_globals(xtg_hip* h, xtg_hip_paged* c, float k_global, float v_global, char* err, int err_len);
+
+/* Whose the rows of a call are. Sequence s has rows starts[s] .. starts[s + 1] - 1 (none where they are equal), at positions
+ * pos[s], pos[s] + 1, ..; rows behind starts[n_seqs] are nobody's, and no call writes anything for them. starts NULL: row s
+ * is sequence s's (n_rows == n_seqs: a decode step). pos[s] < 0 leaves sequence s out. Position p of sequence s is in page
+ * pages[s * max_pages + p / page_size]; a number that is no page of the pool, or a position behind the table's, is no page.
+ * The arrays are device memory, read by the kernels as they run: a captured graph follows what is in them at its replay.
+ * starts must not decrease. max_pages * page_size is 2^30 at most. */
+typedef struct xtg_paged_rows {
+  int n_seqs, n_rows;
+  const int32_t* pos;      /* [n_seqs] */
+  const int32_t* starts;   /* [n_seqs + 1], or NULL */
+  const int32_t* pages;    /* [n_seqs][max_pages] */
+  int max_pages;
+} xtg_paged_rows;
+
+/* The rows' keys and values into their sequences' pages, as xtg_hip_kv_write rounds and scales them, after what the Q/K
+ * producer does to q and k (xtg_hip_qk_rope_norm): rotation by the row's position (theta 0: none; pairs (i, i + head_dim / 2)
+ * by pos * theta^(-2i/head_dim), an angle held in 64 bits, where the producer's are FP32 products), justnorm per head (norm != 0),
+ * and q times qscale (NULL: no scale). q may be NULL; q_out, rows of q's stride, may be q. A row whose position has no page
+ * is not stored (its q_out is written all the same). Rows are x_dtype, x_stride elements apart (0: packed; else a multiple of
+ * 16 bytes), 16-byte aligned. A page that a call writes is in one sequence's table at that place. Queued; the first call of a
+ * theta makes its table (make it before a graph capture). */
+typedef struct xtg_paged_append {
+  int heads;               /* of q */
+  const void* q;           /* device [n_rows][heads][head_dim], or NULL */
+  void* q_out;
+  const void* k;           /* device [n_rows][kv_heads][head_dim] */
+  const void* v;
+  int64_t q_stride, k_stride, v_stride;
+  int x_dtype;
+  float theta;
+  int norm;
+  const float* qscale;     /* device [heads * head_dim], 16-byte aligned, or NULL */
+} xtg_paged_append;
+int xtg_hip_paged_append(xtg_hip* h, xtg_hip_paged* c, const xtg_paged_rows* rows, const xtg_paged_append* a, char* err,
+                         int err_len);
+/* The other way, as xtg_hip_kv_read: the rows' keys and values as the pages hold them into packed device k, v
+ * [n_rows][kv_heads][head_dim] of x_dtype, 16-byte aligned; zeros for a row whose position has no page. Queued. */
+int xtg_hip_paged_read(xtg_hip* h, const xtg_hip_paged* c, const xtg_paged_rows* rows, void* k, void* v, int x_dtype,
+                       char* err, int err_len);
+/* Attention of the rows over their own sequences' pages, which hold their keys and values already (append first): a row at
+ * position t sees positions p <= t, and p > t - window where window > 0, with scores as xtg_hip_attention_ext's: (q . k) * scale,
+ * then softcap * tanh(s / softcap) where softcap > 0. Rows of a sequence that is left out get zeros; a row that sees a
+ * position without a page, or whose scores are all minus infinity, NaN. What is in a page beside the positions that a row
+ * sees, NaN too, is nothing to it. Rows are x_dtype (FP32 q is rounded to BF16, out is not); precision as xtg_hip_attention_ext. Up to
+ * 128 q heads per KV head; n_rows * heads up to 2^30; out, packed, overlaps no input. Queued; the first call of so many rows, sequences and
+ * heads sizes scratch memory, whatever the sequences' lengths (make it before a graph capture). */
+typedef struct xtg_paged_attn {
+  int heads;
+  const void* q;           /* device [n_rows][heads][head_dim], q_stride elements apart (0: packed), 16-byte aligned */
+  int64_t q_stride;
+  void* out;               /* device [n_rows][heads][head_dim] */
+  int x_dtype;
+  int window;
+  float scale, softcap;    /* softcap 0: none; up to 1024 */
+} xtg_paged_attn;
+int xtg_hip_paged_attention(xtg_hip* h, const xtg_hip_paged* c, const xtg_paged_rows* rows, const xtg_paged_attn* a, char* err,
+                            int err_len);
 
 /* ----------------------------------------------------------------------------------------- row kernels */
 

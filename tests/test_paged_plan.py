@@ -1,0 +1,129 @@
+"""The host's side of paged attention, and what the kernels make of a call's arrays (csrc/paged.hpp), through the library
+without a GPU: the work-groups and records that a call is given cover what its sequences ask for, whatever their lengths;
+rows, positions and pages out of range stay out; scratch goes by the rows, sequences and heads alone."""
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+PROGRAM = r"""
+#include <cstdio>
+#include <vector>
+#include "paged.hpp"
+using namespace xtg::hip;
+int main() {
+  DevPaged c;
+  PagedAttnCall a = {};
+  int with_starts, cus;
+  while (std::scanf("%d %d %d %d %d %d %d %d %d %d", &c.kv_heads, &c.pages, &c.shift, &a.heads, &a.seqs.n_seqs, &a.seqs.n_rows,
+                    &a.seqs.max_pages, &a.window, &with_starts, &cus) == 10) {
+    c.head_dim = 128, c.size = 1 << c.shift;
+    std::vector<int> pos(a.seqs.n_seqs), starts(a.seqs.n_seqs + 1), table(size_t(a.seqs.n_seqs) * a.seqs.max_pages);
+    for (int& x : pos) if (std::scanf("%d", &x) != 1) return 1;
+    if (with_starts) for (int& x : starts) if (std::scanf("%d", &x) != 1) return 1;
+    for (size_t x = 0; x < table.size(); ++x) table[x] = int(x * 7919 % 101) - 20;
+    a.cache = &c, a.seqs.pos = pos.data(), a.seqs.starts = with_starts ? starts.data() : nullptr, a.seqs.table = table.data();
+    a.seqs.pages = c.pages, a.seqs.shift = c.shift;
+    const PagedPlan p = paged_plan(a, cus);
+    PagedArgs k = {};
+    k.s = a.seqs, k.group = a.heads / c.kv_heads, k.cols = p.cols, k.budget = p.budget, k.window = a.window;
+    float total = 0;
+    for (int s = 0; s < a.seqs.n_seqs; ++s) { const Extent x = extent(k, s); total += float(x.blocks) * float(x.tiles); }
+    long long tasks = 0, records = 0, bad = 0;
+    for (int s = 0; s < a.seqs.n_seqs; ++s) {
+      const Extent x = extent(k, s);
+      const int n = parts_of(k, x.tiles, total);
+      tasks += (long long)x.blocks * n;
+      if (n > 1) records += (long long)x.blocks * n;
+      bad += x.q.row0 < 0 || x.q.n < 0 || x.q.row0 + x.q.n > a.seqs.n_rows || x.tiles < 0 || x.lo < 0;
+      bad += x.tiles > 0 && (x.lo + x.tiles) * 32 > a.seqs.max_pages << c.shift;
+      for (int at : {0, x.q.pos, x.q.pos + x.q.n, kMostPositions - 1, (a.seqs.max_pages << c.shift) - 1, a.seqs.max_pages << c.shift}) {
+        if (at < 0) continue;
+        const int page = page_of(a.seqs, s, at);
+        bad += page < -1 || page >= c.pages || (at >= a.seqs.max_pages << c.shift && page != -1);
+      }
+    }
+    std::printf("%lld %d %lld %d %lld %zu\n", tasks, p.tasks, records, p.records, bad, p.bytes());
+  }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def run(pkg, tmp_path_factory):
+    d = tmp_path_factory.mktemp("paged")
+    (d / "plan.cpp").write_text(PROGRAM)
+    subprocess.run(["g++", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include",
+                    "-I" + os.path.join(ROOT, "xtier-go_amd", "csrc"), str(d / "plan.cpp"), pkg.LIB_PATH,
+                    "-Wl,-rpath," + os.path.dirname(pkg.LIB_PATH), "-L/opt/rocm/lib", "-lamdhip64", "-o",
+                    str(d / "plan")], check=True)
+
+    def go(calls):
+        text = "".join("%d %d %d %d %d %d %d %d %d %d\n%s\n%s\n" % (
+            *head, " ".join(map(str, pos)), " ".join(map(str, starts)) if head[8] else "") for head, pos, starts in calls)
+        out = subprocess.run([str(d / "plan")], input=text, capture_output=True, text=True, check=True).stdout
+        rows = [tuple(map(int, line.split())) for line in out.splitlines()]
+        assert len(rows) == len(calls)
+        return rows
+    return go
+
+
+def call(kvh, heads, pos, rows=None, window=0, max_pages=40, shift=6, cus=256, pages=60):
+    starts = np.concatenate([[0], np.cumsum(rows)]) if rows is not None else []
+    n_rows = int(starts[-1]) if rows is not None else len(pos)
+    return (kvh, pages, shift, heads, len(pos), n_rows, max_pages, window, int(rows is not None), cus), list(pos), list(starts)
+
+
+def test_tasks_and_records_cover_any_lengths(run):
+    rng = np.random.default_rng(3)
+    calls = []
+    for _ in range(300):
+        n, kvh = int(rng.integers(1, 300)), int(rng.choice([1, 2, 4, 8, 40]))
+        heads, window = kvh * int(rng.choice([1, 2, 3, 4, 8, 17, 128])), int(rng.choice([0, 0, 1, 100, 1024]))
+        top = int(rng.choice([1, 40, 2000, 40 * 64 + 500]))
+        pos = rng.integers(-3, top, n)
+        kind = rng.integers(0, 4)
+        rows = None if kind == 0 else rng.integers(0, int(rng.choice([2, 9, 700])), n)
+        if kind == 3:
+            rows = np.zeros(n, np.int64)
+            rows[rng.integers(0, n)] = 3000
+        calls.append(call(kvh, heads, pos, rows, window, cus=int(rng.choice([1, 64, 256]))))
+    for c, (tasks, most, records, room, bad, _) in zip(calls, run(calls)):
+        assert tasks <= most and records <= room and bad == 0, (c, tasks, most, records, room, bad)
+
+
+def test_arrays_out_of_range_stay_out(run):
+    """Starts that decrease or pass the call's rows, positions near 2^31, tables with numbers that are no pages."""
+    big = 2 ** 31 - 1
+    calls = []
+    for pos, starts in (([big, 5, -big - 1], [0, 2, 1, 9]), ([0, 0, 0], [-5, 100, big, -big]), ([big, big - 1, 2 ** 30], [0, 3, 6, 8]),
+                        ([7, 7, 7], [8, 4, 2, 0])):
+        head = (2, 60, 5, 8, 3, 8, 40, 0, 1, 256)
+        for window in (0, 1, 50, big):
+            calls.append((head[:7] + (window,) + head[8:], pos, starts))
+    for c, (_, _, _, _, bad, _) in zip(calls, run(calls)):
+        assert bad == 0, c
+
+
+def test_scratch_goes_by_rows_sequences_and_heads(run):
+    """A captured decode step's lengths change: the scratch of its first call is enough for all."""
+    got = run([call(8, 32, [p] * 64, max_pages=4000) for p in (0, 31, 5000, 200000)] +
+              [call(8, 32, [p] * 4, [512, 1, 1, 1], max_pages=4000) for p in (0, 31, 5000, 200000)])
+    assert len({g[5] for g in got[:4]}) == 1 and len({g[5] for g in got[4:]}) == 1
+
+
+def test_a_destroyed_pool_is_refused(pkg):
+    """NULL handles are errors with a message, not calls (no GPU is asked)."""
+    import ctypes
+    lib, err = pkg.lib(), ctypes.create_string_buffer(200)
+    rows, a, b = pkg.PagedRowsArgs(), pkg.PagedAppendArgs(), pkg.PagedAttnArgs()
+    for rc in (lib.xtg_hip_paged_append(None, None, ctypes.byref(rows), ctypes.byref(a), err, 200),
+               lib.xtg_hip_paged_read(None, None, ctypes.byref(rows), None, None, 0, err, 200),
+               lib.xtg_hip_paged_attention(None, None, ctypes.byref(rows), ctypes.byref(b), err, 200),
+               lib.xtg_hip_paged_globals(None, None, 1.0, 1.0, err, 200)):
+        assert rc == -1 and b"NULL argument" in err.value
+    assert not lib.xtg_hip_paged_create(None, 8, 128, 4, 64, 0, err, 200)
+    lib.xtg_hip_paged_destroy(None, None)

@@ -57,6 +57,23 @@ _F = ctypes.c_float
 _I64 = ctypes.c_int64
 
 
+class PagedRowsArgs(ctypes.Structure):
+    """xtg_paged_rows."""
+    _fields_ = [("n_seqs", _I), ("n_rows", _I), ("pos", _P), ("starts", _P), ("pages", _P), ("max_pages", _I)]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    """xtg_paged_append."""
+    _fields_ = [("heads", _I), ("q", _P), ("q_out", _P), ("k", _P), ("v", _P), ("q_stride", _I64), ("k_stride", _I64),
+                ("v_stride", _I64), ("x_dtype", _I), ("theta", _F), ("norm", _I), ("qscale", _P)]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    """xtg_paged_attn."""
+    _fields_ = [("heads", _I), ("q", _P), ("q_stride", _I64), ("out", _P), ("x_dtype", _I), ("window", _I), ("scale", _F),
+                ("softcap", _F)]
+
+
 class DoryConfig(ctypes.Structure):
     """xtg_dory_config."""
     _fields_ = [(n, _I) for n in ("hidden", "ffn", "heads", "kv_heads", "head_dim", "vocab", "n_in", "n_rec", "n_out",
@@ -99,6 +116,12 @@ SIGNATURES = [
     ("xtg_hip_attention", _I, [_P, ctypes.POINTER(AttnArgs)] + _ERR),
     ("xtg_hip_attention_noalloc", _I, [_P, ctypes.POINTER(AttnArgs)] + _ERR),
     ("xtg_hip_attention_ext", _I, [_P, ctypes.POINTER(AttnExt)] + _ERR),
+    ("xtg_hip_paged_create", _P, [_P, _I, _I, _I64, _I, _I] + _ERR),
+    ("xtg_hip_paged_destroy", None, [_P, _P]),
+    ("xtg_hip_paged_globals", _I, [_P, _P, _F, _F] + _ERR),
+    ("xtg_hip_paged_append", _I, [_P, _P, ctypes.POINTER(PagedRowsArgs), ctypes.POINTER(PagedAppendArgs)] + _ERR),
+    ("xtg_hip_paged_read", _I, [_P, _P, ctypes.POINTER(PagedRowsArgs), _P, _P, _I] + _ERR),
+    ("xtg_hip_paged_attention", _I, [_P, _P, ctypes.POINTER(PagedRowsArgs), ctypes.POINTER(PagedAttnArgs)] + _ERR),
     ("xtg_hip_qk_rope_norm", _I, [_P, _P, _P, _I, _I, _I, _I, _I64, _F, _P] + _ERR),
     ("xtg_hip_slerp_residual", _I, [_P, _P, _P, _P, _I, _I] + _ERR),
     ("xtg_hip_swiglu_norm", _I, [_P, _P, _P, _P, _P, _I, _I] + _ERR),
@@ -532,6 +555,16 @@ class HipBackend:
         err = self._err
         _check(lib().xtg_hip_attention_ext(self.h, ctypes.byref(a), err, len(err)), err)
 
+    # ---- paged caches
+    def paged_cache(self, kv_heads, head_dim, pages, page_size=64, dtype=KV_BF16):
+        """A pool of pages of page_size positions (a power of two from 32 to 4096) for many sequences."""
+        return PagedCache(self, kv_heads, head_dim, pages, page_size, dtype)
+
+    def paged_rows(self, pos, pages, n_rows=None, starts=None):
+        """Whose the rows of a call are (xtg_paged_rows), for any number of calls on pools of the same pages: device int32
+        pos [n_seqs], pages [n_seqs][max_pages] and, unless row s is sequence s's, starts [n_seqs + 1]."""
+        return PagedRows(self, pos, pages, n_rows, starts)
+
     # ---- the Dory decode step
     def dory(self, weights):
         """A decode session over DoryWeights (xtier_go_amd.workloads); the weights stay referenced by it."""
@@ -729,6 +762,89 @@ class KvCache:
         """Device copy of this cache's whole state into dst (same shape, ring and dtype)."""
         err = _errbuf()
         _check(lib().xtg_hip_kv_copy(self.b.h, self.h, dst.h, err, len(err)), err)
+
+
+class PagedRows:
+    """Which sequences the rows of a call belong to, and where their positions lie (HipBackend.paged_rows). The arrays are
+    the caller's: what is in them may change between calls, and is read when a call runs."""
+
+    def __init__(self, backend, pos, pages, n_rows=None, starts=None):
+        if len(pages.shape) != 2:
+            raise XtgError("pages is not [n_seqs][max_pages]")
+        n_seqs, max_pages = (int(x) for x in pages.shape)
+        n_rows = n_seqs if n_rows is None else n_rows
+        self.b, self.n_seqs, self.n_rows = backend, n_seqs, n_rows
+        self.arrays = pos, pages, starts   # held as long as this is
+        self.args = PagedRowsArgs(n_seqs, n_rows, _device_ptr(backend, "pos", pos, n_seqs, _I32),
+                                  _device_ptr(backend, "starts", starts, n_seqs + 1, _I32),
+                                  _device_ptr(backend, "pages", pages, n_seqs * max_pages, _I32), max_pages)
+        self.ref = ctypes.byref(self.args)
+
+
+class PagedCache:
+    """A pool of pages of keys and values (xtg_hip_paged): rows appended, read back, and attended to."""
+
+    def __init__(self, backend, kv_heads, head_dim, pages, page_size=64, dtype=KV_BF16):
+        self.b = backend
+        self.kv_heads, self.head_dim, self.pages, self.page_size = kv_heads, head_dim, pages, page_size
+        err = _errbuf()
+        self.h = lib().xtg_hip_paged_create(backend.h, kv_heads, head_dim, pages, page_size, dtype, err, len(err))
+        if not self.h:
+            raise XtgError(err.value.decode(errors="replace"))
+
+    def destroy(self):
+        if self.h and self.b.h:
+            lib().xtg_hip_paged_destroy(self.b.h, self.h)
+        self.h = None
+
+    def globals(self, k_global, v_global):
+        """The two powers of two that an NVFP4 pool's scales are multiplied by; before anything is written."""
+        err = _errbuf()
+        _check(lib().xtg_hip_paged_globals(self.b.h, self.h, k_global, v_global, err, len(err)), err)
+
+    def _elems(self, rows, heads, stride):
+        """Elements of an array of the call's rows."""
+        width = heads * self.head_dim
+        return rows.n_rows * width if not stride else max(0, rows.n_rows - 1) * stride + (width if rows.n_rows else 0)
+
+    def append(self, rows, k, v, x_dtype=X_F32, q=None, q_out=None, heads=0, theta=0.0, norm=False, qscale=None,
+               q_stride=0, k_stride=0, v_stride=0):
+        """Queued: the rows' k and v into their pages, k (and q, into q_out, which may be q) rotated by position (theta 0:
+        not) and normalised per head first (norm), q then times qscale (xtg_hip_paged_append). Device rows of x_dtype,
+        packed or `stride` elements apart."""
+        b, kv = self.b, self.kv_heads
+        if not k_stride and not v_stride:
+            k, v = _device_rows(b, k, v, rows.n_rows * kv * self.head_dim, x_dtype)
+        else:
+            k = _device_ptr(b, "k", k, self._elems(rows, kv, k_stride), x_dtype)
+            v = _device_ptr(b, "v", v, self._elems(rows, kv, v_stride), x_dtype)
+        if q is not None:
+            n = self._elems(rows, heads, q_stride)
+            q, q_out = _device_ptr(b, "q", q, n, x_dtype), _device_ptr(b, "q_out", q_out, n, x_dtype)
+        if qscale is not None:
+            qscale = _device_ptr(b, "qscale", qscale, heads * self.head_dim, X_F32)
+        a = PagedAppendArgs(heads, q, q_out, k, v, q_stride, k_stride, v_stride, x_dtype, theta, norm, qscale)
+        if _lib.xtg_hip_paged_append(b.h, self.h, rows.ref, ctypes.byref(a), b._err, _ERR_LEN):
+            _check(-1, b._err)
+
+    def read(self, rows, k, v, x_dtype=X_F32):
+        """Queued: the rows' k and v as the pages hold them into packed device rows of x_dtype, zeros where there is no
+        page (xtg_hip_paged_read)."""
+        b = self.b
+        k, v = _device_rows(b, k, v, rows.n_rows * self.kv_heads * self.head_dim, x_dtype)
+        if _lib.xtg_hip_paged_read(b.h, self.h, rows.ref, k, v, x_dtype, b._err, _ERR_LEN):
+            _check(-1, b._err)
+
+    def attention(self, rows, q, out, heads, x_dtype=X_F32, window=0, scale=None, softcap=0.0, q_stride=0):
+        """Queued: attention of the rows over their sequences' pages, their own keys among them (xtg_hip_paged_attention):
+        a row at position t sees p <= t, and p > t - window; scores softcap * tanh(scale * q.k / softcap)."""
+        b, d = self.b, self.head_dim
+        n = rows.n_rows * heads * d
+        q = _device_ptr(b, "q", q, n if not q_stride else self._elems(rows, heads, q_stride), x_dtype)
+        a = PagedAttnArgs(heads, q, q_stride, _device_ptr(b, "out", out, n, x_dtype), x_dtype, window,
+                          d ** -0.5 if scale is None else scale, softcap)
+        if _lib.xtg_hip_paged_attention(b.h, self.h, rows.ref, ctypes.byref(a), b._err, _ERR_LEN):
+            _check(-1, b._err)
 
 
 class DeviceArray:

@@ -38,7 +38,7 @@ Backend::~Backend() {
   for (auto& kv : weights_) (void)hipFree(kv.second.tiles);
   for (auto& kv : bf16_weights_) (void)hipFree(kv.second.tiles);
   for (void* p : allocs_) (void)hipFree(p);
-  for (void* p : {op_, opb_, hx_, hy_, part_, kproc_, stage_, sample_, ext_, static_cast<void*>(ident_rope_)})
+  for (void* p : {op_, opb_, hx_, hy_, part_, kproc_, stage_, sample_, ext_, paged_part_, static_cast<void*>(ident_rope_)})
     if (p) (void)hipFree(p);
   for (void* p : retired_) (void)hipFree(p);
   for (DevKv* c : kvs_) {
@@ -47,6 +47,12 @@ Backend::~Backend() {
       if (p) (void)hipFree(p);
     delete c;
   }
+  for (DevPaged* c : paged_) {
+    for (void* p : {c->k, c->v, c->ks, c->vs})
+      if (p) (void)hipFree(p);
+    delete c;
+  }
+  for (auto& f : turn_freq_) (void)hipFree(f.second);
   for (auto& f : inv_freq_) (void)hipFree(f.second);
   for (auto& t : rope_) (void)hipFree(t.p);
   for (const Pending& p : pending_) {
@@ -426,15 +432,19 @@ void Backend::kv_destroy(DevKv* c) {
   delete c;
 }
 
+static void check_globals(const char* what, float kglobal, float vglobal) {
+  for (float g : {kglobal, vglobal}) {
+    int e = 0;
+    XTG_CHECK(g > 0.f && std::frexp(g, &e) == 0.5f && e >= -59 && e <= 61,
+              "%s: %g is not a power of two from 2^-60 to 2^60", what, double(g));
+  }
+}
+
 void Backend::kv_globals(DevKv* c, float kglobal, float vglobal) {
   XTG_CHECK(kvs_.count(c), "kv_globals: unknown cache");
   XTG_CHECK(c->fp4, "kv_globals: not an NVFP4 cache");
   XTG_CHECK(!c->written, "kv_globals: the cache has been written (release it first)");
-  for (float g : {kglobal, vglobal}) {
-    int e = 0;
-    XTG_CHECK(g > 0.f && std::frexp(g, &e) == 0.5f && e >= -59 && e <= 61,
-              "kv_globals: %g is not a power of two from 2^-60 to 2^60", double(g));
-  }
+  check_globals("kv_globals", kglobal, vglobal);
   c->kglobal = kglobal;
   c->vglobal = vglobal;
 }
@@ -762,6 +772,170 @@ void Backend::attn_step(DevKv* c, int m, long long pos0, int heads, int window, 
     timed([&] { return launch_attn_gate_heads(p, heads, part, g, gscale, out, gate_rec, stream_); });
   else
     timed([&] { return launch_attn_gate(p, m, heads, part, g, gscale, out, op, stream_); });
+}
+
+// --------------------------------------------------------------------------------------------- paged caches
+
+namespace {
+
+// The backend's device as the current one, as long as it lives.
+struct OnDevice {
+  int before = 0;
+  explicit OnDevice(int device) {
+    HIP_CHECK(hipGetDevice(&before));
+    if (before != device) HIP_CHECK(hipSetDevice(device));
+    else before = -1;
+  }
+  ~OnDevice() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
+}  // namespace
+
+DevPaged* Backend::paged_create(int kv_heads, int head_dim, long long pages, int page_size, int dtype) {
+  XTG_CHECK(!capturing_, "paged_create: not during a graph capture");
+  XTG_CHECK(dtype == XTG_KV_BF16 || dtype == XTG_KV_FP8 || dtype == XTG_KV_NVFP4, "paged_create: unknown KV dtype %d", dtype);
+  XTG_CHECK(head_dim == 64 || head_dim == 128 || head_dim == 256, "paged_create: head_dim %d (64, 128 or 256)", head_dim);
+  XTG_CHECK(kv_heads > 0 && kv_heads < 65536, "paged_create: %d KV heads", kv_heads);
+  XTG_CHECK(page_size >= 32 && page_size <= 4096 && (page_size & (page_size - 1)) == 0,
+            "paged_create: pages of %d positions (a power of two from 32 to 4096)", page_size);
+  XTG_CHECK(pages > 0 && pages < (1LL << 31) / kv_heads, "paged_create: %lld pages", pages);
+  const OnDevice on(device_);
+  auto c = std::make_unique<DevPaged>();
+  c->kv_heads = kv_heads;
+  c->head_dim = head_dim;
+  c->pages = int(pages);
+  c->size = page_size;
+  while (1 << c->shift < page_size) ++c->shift;
+  c->type = dtype;
+  try {
+    for (void** p : {&c->k, &c->v}) {
+      HIP_CHECK(hipMalloc(p, c->data_bytes()));
+      HIP_CHECK(hipMemsetAsync(*p, 0, c->data_bytes(), stream_));
+    }
+    if (c->scale_bytes())
+      for (void** p : {&c->ks, &c->vs}) {
+        HIP_CHECK(hipMalloc(p, c->scale_bytes()));
+        HIP_CHECK(hipMemsetAsync(*p, 0, c->scale_bytes(), stream_));
+      }
+    paged_.insert(c.get());
+  } catch (...) {
+    (void)hipStreamSynchronize(stream_);
+    for (void* p : {c->k, c->v, c->ks, c->vs})
+      if (p) (void)hipFree(p);
+    throw;
+  }
+  return c.release();
+}
+
+void Backend::paged_destroy(DevPaged* c) {
+  auto it = paged_.find(c);
+  if (it == paged_.end()) return;
+  XTG_CHECK(!capturing_, "paged_destroy: not during a graph capture");
+  for (void* p : {c->k, c->v, c->ks, c->vs}) dev_free(p);
+  paged_.erase(it);
+  delete c;
+}
+
+void Backend::paged_globals(DevPaged* c, float kglobal, float vglobal) {
+  XTG_CHECK(paged_.count(c), "paged_globals: unknown cache");
+  XTG_CHECK(c->type == XTG_KV_NVFP4, "paged_globals: not an NVFP4 cache");
+  XTG_CHECK(!c->written, "paged_globals: the cache has been written");
+  check_globals("paged_globals", kglobal, vglobal);
+  c->kglobal = kglobal;
+  c->vglobal = vglobal;
+}
+
+// The checks that the three calls share.
+Seqs Backend::paged_rows(const char* what, const DevPaged* c, const xtg_paged_rows& r) const {
+  XTG_CHECK(paged_.count(const_cast<DevPaged*>(c)), "%s: unknown cache", what);
+  XTG_CHECK(r.n_seqs >= 0 && r.n_rows >= 0 && r.n_rows < (1 << 30) && r.n_seqs < (1 << 24), "%s: %d rows of %d sequences", what,
+            r.n_rows, r.n_seqs);
+  XTG_CHECK(r.starts || r.n_rows == r.n_seqs, "%s: %d rows of %d sequences without starts", what, r.n_rows, r.n_seqs);
+  XTG_CHECK(r.max_pages >= 1 && (long long)r.max_pages * c->size <= (1 << 30), "%s: %d pages of %d positions a sequence (2^30 positions at most)",
+            what, r.max_pages, c->size);
+  XTG_CHECK(r.n_seqs == 0 || (r.pos && r.pages), "%s: NULL positions or pages", what);
+  for (const int32_t* p : {r.pos, r.starts, r.pages})
+    XTG_CHECK(reinterpret_cast<uintptr_t>(p) % 4 == 0, "%s: positions, starts and pages must be 4-byte aligned", what);
+  return {r.pos, r.starts, r.pages, r.n_seqs, r.n_rows, r.max_pages, c->pages, c->shift};
+}
+
+// The elements from a row to the next one of `width` elements, 0 given for `width`.
+static long long row_stride(const char* what, const char* name, int64_t given, long long width, int x_dtype) {
+  if (given == 0) return width;
+  XTG_CHECK(given >= width && given < (1LL << 31), "%s: a stride of %lld elements for %s rows of %lld", what, (long long)given, name, width);
+  XTG_CHECK(given % (x_dtype == kXBF16 ? 8 : 4) == 0, "%s: a stride of %lld elements for %s, which is no multiple of 16 bytes", what,
+            (long long)given, name);
+  return given;
+}
+
+void Backend::paged_append(DevPaged* c, const xtg_paged_rows& rows, const xtg_paged_append& a) {
+  const Seqs s = paged_rows("paged_append", c, rows);
+  XTG_CHECK(a.x_dtype == kXF32 || a.x_dtype == kXBF16, "paged_append: unknown row type %d", a.x_dtype);
+  XTG_CHECK(!a.q == !a.q_out, "paged_append: one of q and q_out is NULL (both, or neither)");
+  XTG_CHECK(!a.q || (a.heads >= 1 && a.heads < (1 << 20)), "paged_append: %d q heads", a.heads);
+  XTG_CHECK(a.q || !a.qscale, "paged_append: a scale without q");
+  XTG_CHECK(a.theta == 0.f || (std::isfinite(a.theta) && a.theta >= 1.f), "paged_append: theta %g (0, or 1 and more)", double(a.theta));
+  if (rows.n_rows == 0 || rows.n_seqs == 0) return;
+  XTG_CHECK(a.k && a.v, "paged_append: NULL rows");
+  for (const void* p : {a.k, a.v, a.q, static_cast<const void*>(a.q_out), static_cast<const void*>(a.qscale)})
+    XTG_CHECK(aligned16(p), "paged_append: rows and the scale must be 16-byte aligned");
+  PagedAppend p = {};
+  const long long kv = (long long)c->kv_heads * c->head_dim, q = (long long)a.heads * c->head_dim;
+  p.heads = a.heads;
+  p.q = a.q, p.k = a.k, p.v = a.v, p.q_out = a.q_out;
+  p.ldk = row_stride("paged_append", "k", a.k_stride, kv, a.x_dtype);
+  p.ldv = row_stride("paged_append", "v", a.v_stride, kv, a.x_dtype);
+  if (a.q) p.ldq = row_stride("paged_append", "q", a.q_stride, q, a.x_dtype);
+  p.x_dtype = a.x_dtype, p.norm = a.norm;
+  p.freq = a.theta > 0.f ? turn_freq(a.theta, c->head_dim) : nullptr;
+  p.qscale = a.qscale;
+  c->written = true;
+  timed([&] { return launch_paged_append(*c, s, p, stream_); });
+}
+
+void Backend::paged_read(const DevPaged* c, const xtg_paged_rows& rows, void* k, void* v, int x_dtype) {
+  const Seqs s = paged_rows("paged_read", c, rows);
+  XTG_CHECK(x_dtype == kXF32 || x_dtype == kXBF16, "paged_read: unknown row type %d", x_dtype);
+  if (rows.n_rows == 0 || rows.n_seqs == 0) return;
+  XTG_CHECK(k && v, "paged_read: NULL rows");
+  XTG_CHECK(aligned16(k) && aligned16(v), "paged_read: rows must be 16-byte aligned");
+  timed([&] { return launch_paged_read(*c, s, k, v, x_dtype == kXBF16, stream_); });
+}
+
+void Backend::paged_attention(const DevPaged* c, const xtg_paged_rows& rows, const xtg_paged_attn& a) {
+  const Seqs s = paged_rows("paged_attention", c, rows);
+  XTG_CHECK(a.x_dtype == kXF32 || a.x_dtype == kXBF16, "paged_attention: unknown row type %d", a.x_dtype);
+  XTG_CHECK(a.heads >= 1 && a.heads % c->kv_heads == 0 && a.heads / c->kv_heads <= 128,
+            "paged_attention: %d heads over %d KV heads (up to 128 for each)", a.heads, c->kv_heads);
+  XTG_CHECK((long long)rows.n_rows * a.heads <= (1LL << 30), "paged_attention: %d rows of %d heads (2^30 at most)", rows.n_rows, a.heads);
+  XTG_CHECK(std::isfinite(a.scale), "paged_attention: scale %g", double(a.scale));
+  XTG_CHECK(a.softcap >= 0.f && a.softcap <= 1024.f, "paged_attention: softcap %g (0 to 1024)", double(a.softcap));
+  if (rows.n_rows == 0 || rows.n_seqs == 0) return;
+  XTG_CHECK(a.q && a.out, "paged_attention: NULL rows");
+  XTG_CHECK(aligned16(a.q) && aligned16(a.out), "paged_attention: rows must be 16-byte aligned");
+  PagedAttnCall p = {};
+  p.cache = c, p.seqs = s, p.heads = a.heads, p.q = a.q, p.out = a.out;
+  p.ldq = row_stride("paged_attention", "q", a.q_stride, (long long)a.heads * c->head_dim, a.x_dtype);
+  p.x_dtype = a.x_dtype, p.window = a.window, p.scale = a.scale, p.softcap = a.softcap;
+  const PagedPlan plan = paged_plan(p, cus_);
+  ensure(paged_part_, paged_part_size_, plan.bytes());
+  launch_paged_attn(p, plan, paged_part_, stream_, [&](auto&& launch) { timed(launch); });
+}
+
+const double* Backend::turn_freq(float theta, int d) {
+  for (auto& f : turn_freq_)
+    if (f.first.first == theta && f.first.second == d) return f.second;
+  XTG_CHECK(!capturing_, "rotation: the frequencies for theta %g, head_dim %d must exist before a graph capture", double(theta), d);
+  std::vector<double> h(size_t(d / 2));
+  for (int i = 0; i < d / 2; ++i) h[size_t(i)] = 2.0 / 3.14159265358979323846 * std::pow(double(theta), -2.0 * i / d);
+  const OnDevice on(device_);
+  double* p = nullptr;
+  HIP_CHECK(hipMalloc(&p, h.size() * sizeof(double)));
+  HIP_CHECK(hipMemcpy(p, h.data(), h.size() * sizeof(double), hipMemcpyHostToDevice));
+  turn_freq_.push_back({{theta, d}, p});
+  return p;
 }
 
 // ---------------------------------------------------------------------------------------------- row kernels

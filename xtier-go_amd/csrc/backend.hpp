@@ -15,6 +15,7 @@
 #include "attention_ext.hpp"
 #include "common.hpp"
 #include "kernels.hpp"
+#include "paged.hpp"
 #include "rows.hpp"
 #include "xtg_hip.h"
 
@@ -92,6 +93,16 @@ class Backend {
   // another open backend on the device holds the array (attn_scratch_claim: the first caller keeps it until closed).
   void attention_noalloc(const DevKv* c, int n_q, long long pos0, int heads, int window, float scale, const float* q,
                          const float* k, const float* v, float* out);
+  // Paged caches (paged.hpp): a pool of pages; rows of many sequences into it, back, and attention over it. rows: the
+  // fields of xtg_paged_rows.
+  DevPaged* paged_create(int kv_heads, int head_dim, long long pages, int page_size, int dtype);
+  void paged_destroy(DevPaged* c);
+  void paged_globals(DevPaged* c, float kglobal, float vglobal);
+  void paged_append(DevPaged* c, const xtg_paged_rows& rows, const xtg_paged_append& a);
+  void paged_read(const DevPaged* c, const xtg_paged_rows& rows, void* k, void* v, int x_dtype);
+  void paged_attention(const DevPaged* c, const xtg_paged_rows& rows, const xtg_paged_attn& a);
+  // quarter turns a position of the pairs of a head of d dims, 2 / pi * theta^(-2i/d) in 64 bits, kept on the device
+  const double* turn_freq(float theta, int d);
   // Attention over a cache of any dtype with capped, biased and masked scores (attention_ext.hpp).
   void attention_ext(const ExtCall& a);
   // The attention half of a Dory sublayer (packs/dory/dory.cpp:482-515) on device rows q [m][heads][d],
@@ -232,6 +243,11 @@ class Backend {
   size_t sample_size_ = 0;
   void* ext_ = nullptr;      // attention_ext: packed own keys and records
   size_t ext_size_ = 0;
+  void* paged_part_ = nullptr;   // paged attention: records, and where each q-col's are
+  size_t paged_part_size_ = 0;
+  Seqs paged_rows(const char* what, const DevPaged* c, const xtg_paged_rows& rows) const;
+  std::unordered_set<DevPaged*> paged_;
+  std::vector<std::pair<std::pair<float, int>, double*>> turn_freq_;
   int cus_ = 0;
   std::unordered_set<DevKv*> kvs_;
   std::vector<std::pair<std::pair<float, int>, float*>> inv_freq_;

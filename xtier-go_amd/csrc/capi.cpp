@@ -259,6 +259,51 @@ int xtg_hip_attention_ext(xtg_hip* h, const xtg_attn_ext* a, char* err, int err_
   });
 }
 
+xtg_hip_paged* xtg_hip_paged_create(xtg_hip* h, int kv_heads, int head_dim, int64_t pages, int page_size, int dtype, char* err,
+                                    int err_len) {
+  xtg::hip::DevPaged* c = nullptr;
+  int rc = guarded(err, err_len, [&] {
+    XTG_CHECK(h, "paged_create: NULL handle");
+    c = h->b->paged_create(kv_heads, head_dim, pages, page_size, dtype);
+  });
+  return rc == 0 ? reinterpret_cast<xtg_hip_paged*>(c) : nullptr;
+}
+
+void xtg_hip_paged_destroy(xtg_hip* h, xtg_hip_paged* c) {
+  if (h && c) guarded(nullptr, 0, [&] { h->b->paged_destroy(reinterpret_cast<xtg::hip::DevPaged*>(c)); });
+}
+
+int xtg_hip_paged_globals(xtg_hip* h, xtg_hip_paged* c, float k_global, float v_global, char* err, int err_len) {
+  return guarded(err, err_len, [&] {
+    XTG_CHECK(h && c, "paged_globals: NULL argument");
+    h->b->paged_globals(reinterpret_cast<xtg::hip::DevPaged*>(c), k_global, v_global);
+  });
+}
+
+int xtg_hip_paged_append(xtg_hip* h, xtg_hip_paged* c, const xtg_paged_rows* rows, const xtg_paged_append* a, char* err,
+                         int err_len) {
+  return guarded(err, err_len, [&] {
+    XTG_CHECK(h && c && rows && a, "paged_append: NULL argument");
+    h->b->paged_append(reinterpret_cast<xtg::hip::DevPaged*>(c), *rows, *a);
+  });
+}
+
+int xtg_hip_paged_read(xtg_hip* h, const xtg_hip_paged* c, const xtg_paged_rows* rows, void* k, void* v, int x_dtype, char* err,
+                       int err_len) {
+  return guarded(err, err_len, [&] {
+    XTG_CHECK(h && c && rows, "paged_read: NULL argument");
+    h->b->paged_read(reinterpret_cast<const xtg::hip::DevPaged*>(c), *rows, k, v, x_dtype);
+  });
+}
+
+int xtg_hip_paged_attention(xtg_hip* h, const xtg_hip_paged* c, const xtg_paged_rows* rows, const xtg_paged_attn* a, char* err,
+                            int err_len) {
+  return guarded(err, err_len, [&] {
+    XTG_CHECK(h && c && rows && a, "paged_attention: NULL argument");
+    h->b->paged_attention(reinterpret_cast<const xtg::hip::DevPaged*>(c), *rows, *a);
+  });
+}
+
 int xtg_hip_qk_rope_norm(xtg_hip* h, float* q, float* k, int m, int heads, int kv_heads, int head_dim, int64_t pos0,
                          float theta, const float* qscale, char* err, int err_len) {
   return guarded(err, err_len, [&] {

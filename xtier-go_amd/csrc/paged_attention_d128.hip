@@ -1,0 +1,8 @@
+// The kernels of paged_attention_kernels.hpp for heads of 128 dims.
+#include "paged_attention_kernels.hpp"
+
+namespace xtg::hip {
+
+template void paged_launch<128>(const PagedAttnCall&, const PagedPlan&, const PagedArgs&, hipStream_t, const PagedTimed&);
+
+}  // namespace xtg::hip
