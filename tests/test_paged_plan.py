@@ -31,13 +31,24 @@ int main() {
     PagedArgs k = {};
     k.s = a.seqs, k.group = a.heads / c.kv_heads, k.cols = p.cols, k.budget = p.budget, k.window = a.window;
     float total = 0;
-    for (int s = 0; s < a.seqs.n_seqs; ++s) { const Extent x = extent(k, s); total += float(x.blocks) * float(x.tiles); }
+    int blocks = 0;
+    for (int s = 0; s < a.seqs.n_seqs; ++s) {
+      const Extent x = extent(k, s);
+      total += float(x.blocks) * float(x.tiles), blocks += x.blocks;
+    }
+    int chunk = first_chunk(k, total, blocks);
+    for (int step = 0; step < kChunkSteps; ++step) {
+      int n = 0;
+      for (int s = 0; s < a.seqs.n_seqs; ++s) { const Extent x = extent(k, s); n += x.blocks * parts_of(x, chunk); }
+      if (!next_chunk(k, chunk, n, blocks)) break;
+    }
     long long tasks = 0, records = 0, bad = 0;
     for (int s = 0; s < a.seqs.n_seqs; ++s) {
       const Extent x = extent(k, s);
-      const int n = parts_of(k, x.tiles, total);
+      const int n = parts_of(x, chunk);
       tasks += (long long)x.blocks * n;
-      if (n > 1) records += (long long)x.blocks * n;
+      if (n > 1) records += (long long)x.blocks * n * x.cols(k);
+      bad += (x.many && !p.many) || (!x.many && x.blocks > 1);
       bad += x.q.row0 < 0 || x.q.n < 0 || x.q.row0 + x.q.n > a.seqs.n_rows || x.tiles < 0 || x.lo < 0;
       bad += x.tiles > 0 && (x.lo + x.tiles) * 32 > a.seqs.max_pages << c.shift;
       for (int at : {0, x.q.pos, x.q.pos + x.q.n, kMostPositions - 1, (a.seqs.max_pages << c.shift) - 1, a.seqs.max_pages << c.shift}) {

@@ -48,6 +48,7 @@ constexpr float kLog2e = 1.44269504088896341f;
 
 // What the kernels take.
 struct ExtArgs {
+  static constexpr bool kStream = false;   // work-groups share tiles
   const void *q, *k, *v;
   void* out;
   const uint8_t *ck, *cv;

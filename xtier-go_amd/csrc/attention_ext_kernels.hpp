@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, QB * D > 256 ? 1 : 2) ext_few_
     if (32 * t < a.own && __ballot(any)) {
       OwnTile<D, T> tile(a, h, kv_heads, t, lane);
       auto at = [&](int e) { return 32 * t + 4 * g + e < a.own ? p + 4 * g + e : -1; };
-      few_tile<D, QB, MOD>(tile, q, rows.span, rows.sc, st, make_int4(at(0), at(1), at(2), at(3)),
+      few_tile<D, QB, MOD>(tile, [&](int qb, int c) { return q[qb][c]; }, rows.span, rows.sc, st, make_int4(at(0), at(1), at(2), at(3)),
                            make_int4(at(16), at(17), at(18), at(19)), [] {}, [] {});
     }
   } else {
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, QB * D > 256 ? 1 : 2) ext_few_
         const int n = min(t + kExtWaves, t_end - 1);   // past the end: loaded again, and not used
         const int4 c0 = p0, c1 = p1;
         few_tile<D, QB, MOD>(
-            tile, q, rows.span, rows.sc, st, c0, c1,
+            tile, [&](int qb, int c) { return q[qb][c]; }, rows.span, rows.sc, st, c0, c1,
             [&] {
               tile.load_k(a, tile_at(a, h, n), lane);
               p0 = sp[n * 8], p1 = sp[n * 8 + 4];
@@ -461,187 +461,6 @@ __global__ void __launch_bounds__(256) ext_pack_kernel(const void* __restrict__ 
 
 // --------------------------------------------------------------------------------------------------- many q-cols
 
-// A tile of TK keys in LDS: K as [32-key block][16-dim step][64 lanes] entries of 8 dims, V as [32-row block][key step]
-// [64 lanes] entries of 8 keys: A operands of v_mfma_f32_32x32x16. Lane (half, i) of a K entry has key i and dims
-// 8 half .. +8 of the step, of a V entry row i and keys 8 a + 4 half + e, 16 + 8 a + 4 half + e (e = 0 .. 3) of step
-// a = 0, 1 of a 32-key block: what the lane's scores are of. A cache's entries are these too, in another order.
-// Two buffers of each, with the tiles' positions, FP8 scales and first and last position.
-template <int D>
-struct Rows {
-  static constexpr int TK = D == 256 ? 32 : 64;
-  static constexpr int KB = TK / 32, NS = D / 16, NB = D / 32, KS = TK / 16;
-  static constexpr int kEntries = TK * D / 8;           // of K, and of V
-  static constexpr int PER = kEntries / 256;            // entries a thread stages
-  static constexpr int kInfo = 3 * TK + 4;              // ints of a tile's positions, scales and extremes
-  static constexpr size_t kLds = size_t(kEntries) * 64 + size_t(kInfo) * 8 + 2048 + (D == 256 ? 2 * 4096 : 0);
-  // (and room to turn the output; for heads of 256 dims, for two chunks of q)
-};
-
-// What a thread stages of a tile: loads in flight (raw), then entries written to LDS. A cache of an odd number of 32-slot
-// tiles ends in the middle of a 64-key tile (`half`): its other half is zeros.
-template <int D, int T>
-struct Stage;
-
-// BF16: entries as they are. Also the packed own keys.
-template <int D>
-struct Stage<D, kBf16> {
-  using R = Rows<D>;
-  uint4 k[R::PER], v[R::PER];
-  __device__ static void load(uint4 (&x)[R::PER], const uint4* c, int h, int pad, int tile, bool half) {
-    const size_t at = (size_t(h) * size_t(pad) + size_t(tile) * R::TK) * (D / 8) + threadIdx.x;
-#pragma unroll
-    for (int u = 0; u < R::PER; ++u) x[u] = half && 2 * u >= R::PER ? make_uint4(0, 0, 0, 0) : c[at + u * 256];
-  }
-  __device__ void load_k(const uint4* ck, int h, int pad, int tile, bool half) { load(k, ck, h, pad, tile, half); }
-  __device__ void load_v(const uint4* cv, int h, int pad, int tile, bool half) { load(v, cv, h, pad, tile, half); }
-  // The tile straight into its place in LDS: 64 entries a wave's load, a lane's the one that comes to its part of them.
-  __device__ static void direct(const uint4* c, int h, int pad, int tile, uint4* to, bool v) {
-    const uint4* from = c + (size_t(h) * size_t(pad) + size_t(tile) * R::TK) * (D / 8);
-    const int lane = int(threadIdx.x) & 63, half = lane >> 5, i = lane & 31;
-    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
-#pragma unroll
-    for (int u = 0; u < R::PER; ++u) {
-      const int row = u * 4 + wave;   // of 64 entries
-      int x;
-      if (v) {
-        const int dd = row / R::KS * 2 + (i >> 4), ks = row % R::KS;
-        x = (ks >> 1) * 4 * D + dd * 64 + ((ks & 1) * 2 + half) * 16 + (i & 15);
-      } else {
-        const int b = row / R::NS * 2 + (i >> 4), st = row % R::NS;
-        x = b * 2 * D + (st >> 1) * 64 + ((st & 1) * 2 + half) * 16 + (i & 15);
-      }
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + x),
-                                       (__attribute__((address_space(3))) void*)(to + row * 64), 16, 0, 0);
-    }
-  }
-  // entry x of a BF16 tile of TK keys to its place
-  __device__ static int k_place(int x) {
-    const int b = x / (2 * D), c = x / 64 % (D / 32), g = x >> 4 & 3, i = x & 15;
-    return ((b >> 1) * R::NS + 2 * c + (g >> 1)) * 64 + (g & 1) * 32 + (b & 1) * 16 + i;
-  }
-  __device__ static int v_place(int x) {
-    const int t = x / (4 * D), dd = x / 64 % (D / 16), g = x >> 4 & 3, i = x & 15;
-    return ((dd >> 1) * R::KS + 2 * t + (g >> 1)) * 64 + (g & 1) * 32 + (dd & 1) * 16 + i;
-  }
-  __device__ void store_k(uint4* lk) const {
-#pragma unroll
-    for (int u = 0; u < R::PER; ++u) lk[k_place(int(threadIdx.x) + u * 256)] = k[u];
-  }
-  __device__ void store_v(uint4* lv) const {
-#pragma unroll
-    for (int u = 0; u < R::PER; ++u) lv[v_place(int(threadIdx.x) + u * 256)] = v[u];
-  }
-};
-
-// FP8: a 16-byte load is two entries' codes.
-template <int D>
-struct Stage<D, kFp8> {
-  using R = Rows<D>;
-  using B = Stage<D, kBf16>;
-  uint4 k[R::PER / 2], v[R::PER / 2];
-  __device__ static void load(uint4 (&x)[R::PER / 2], const uint4* c, int h, int pad, int tile, bool half) {
-    const size_t at = (size_t(h) * size_t(pad) + size_t(tile) * R::TK) * (D / 16) + threadIdx.x;
-#pragma unroll
-    for (int u = 0; u < R::PER / 2; ++u) {
-      const bool past = half && int(threadIdx.x) + u * 256 >= R::kEntries / 4;
-      x[u] = past ? make_uint4(0, 0, 0, 0) : c[at + u * 256];
-    }
-  }
-  __device__ void load_k(const uint4* ck, int h, int pad, int tile, bool half) { load(k, ck, h, pad, tile, half); }
-  __device__ void load_v(const uint4* cv, int h, int pad, int tile, bool half) { load(v, cv, h, pad, tile, half); }
-  __device__ static int first(int u) {   // of BF16's entries
-    const int x = int(threadIdx.x) + u * 256;
-    return (x >> 6) * 128 + (x & 63);
-  }
-  __device__ void store_k(uint4* lk) const {
-#pragma unroll
-    for (int u = 0; u < R::PER / 2; ++u) {
-      lk[B::k_place(first(u))] = __builtin_bit_cast(uint4, fp8_operand(k[u].x, k[u].y));
-      lk[B::k_place(first(u) + 64)] = __builtin_bit_cast(uint4, fp8_operand(k[u].z, k[u].w));
-    }
-  }
-  __device__ void store_v(uint4* lv) const {
-#pragma unroll
-    for (int u = 0; u < R::PER / 2; ++u) {
-      lv[B::v_place(first(u))] = __builtin_bit_cast(uint4, fp8_operand(v[u].x, v[u].y));
-      lv[B::v_place(first(u) + 64)] = __builtin_bit_cast(uint4, fp8_operand(v[u].z, v[u].w));
-    }
-  }
-};
-
-// NVFP4: a thread's codes are PER entries of K, which share a key, and PER of V, which share their keys' scales.
-template <int D>
-struct Stage<D, kNvfp4> {
-  using R = Rows<D>;
-  uint32_t k[R::PER], v[R::PER], ks;
-  uint2 vs;
-  __device__ void load_k(const ExtArgs& a, int h, int tile, bool half) {
-    const size_t at = size_t(h) * size_t(a.slots_pad) + size_t(tile) * R::TK;
-    const int tid = int(threadIdx.x);
-#pragma unroll
-    for (int u = 0; u < R::PER; ++u) k[u] = 0;
-    ks = 0;
-    if (half && tid >= 128) return;
-    take(k, a.ck + at * (D / 2), tid);
-    const uint8_t* s = static_cast<const uint8_t*>(a.ks) + at * (D / 16);
-    ks = D == 64 ? s[tid] : reinterpret_cast<const uint16_t*>(s)[tid];
-  }
-  // V: a wave has half a 32-slot tile's words (256 dims: a quarter)
-  __device__ void load_v(const ExtArgs& a, int h, int tile, bool half) {
-    const size_t at = size_t(h) * size_t(a.slots_pad) + size_t(tile) * R::TK;
-    const int tid = int(threadIdx.x), lane = tid & 63, part = tid >> 6, t = D == 256 ? 0 : part >> 1;
-#pragma unroll
-    for (int u = 0; u < R::PER; ++u) v[u] = 0;
-    vs = make_uint2(0, 0);
-    if (half && tid >= 128) return;
-    take_v(a.cv + at * (D / 2), part, lane);
-    const uint2* sv = reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.vs) + at * (D / 16));
-    vs = sv[t * (D / 4) + (lane >> 4) * (D / 16) + (lane & 15) * (D / 16) / 16];
-  }
-  __device__ void take(uint32_t (&w)[R::PER], const uint8_t* p, int tid) {
-    if constexpr (R::PER == 4) {
-      const uint4 x = reinterpret_cast<const uint4*>(p)[tid];
-      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-    } else {
-      const uint2 x = reinterpret_cast<const uint2*>(p)[tid];
-      w[0] = x.x, w[1] = x.y;
-    }
-  }
-  // words of products first_dd(part) .. of a lane
-  __device__ void take_v(const uint8_t* p, int part, int lane) {
-    if constexpr (R::PER == 4) {
-      const uint4 x = reinterpret_cast<const uint4*>(p)[part * 64 + lane];   // [tile][4 products][lane]
-      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-    } else {   // 64 dims: one 16-byte group a tile, half of it a wave
-      const uint2 x = reinterpret_cast<const uint2*>(p)[((part >> 1) * 64 + lane) * 2 + (part & 1)];
-      v[0] = x.x, v[1] = x.y;
-    }
-  }
-  __device__ void store_k(uint4* lk) const {
-    const int tid = int(threadIdx.x), lane = tid & 63, part = tid >> 6, g = lane >> 4, i = lane & 15;
-    // D = 64, 128: 16-slot block `part`; 256: block part / 2, chunk part % 2
-    const int b = D == 256 ? part >> 1 : part, chunk = D == 256 ? part & 1 : 0;
-#pragma unroll
-    for (int c = 0; c < R::PER; ++c) {
-      const int dim8 = chunk * 16 + g * R::PER + c;   // dims 8 dim8 .. +8
-      lk[((b >> 1) * R::NS + (dim8 >> 1)) * 64 + (dim8 & 1) * 32 + (b & 1) * 16 + i] =
-          __builtin_bit_cast(uint4, dequant8(k[c], scale_pair(ks, c >> 1)));
-    }
-  }
-  __device__ void store_v(uint4* lv) const {
-    const int tid = int(threadIdx.x), lane = tid & 63, part = tid >> 6, g = lane >> 4, i = lane & 15;
-    f16x2 s[4];
-    v_scales(vs, s);
-    const int t = D == 256 ? 0 : part >> 1, dd0 = (D == 256 ? part : part & 1) * R::PER;
-#pragma unroll
-    for (int c = 0; c < R::PER; ++c) {
-      const int dd = dd0 + c;
-      lv[((dd >> 1) * R::KS + 2 * t + (g >> 1)) * 64 + (g & 1) * 32 + (dd & 1) * 16 + i] =
-          __builtin_bit_cast(uint4, dequant8_pairs(v[c], s));
-    }
-  }
-};
-
 // The tiles of TK keys that a work-group goes over (its split's part): of the cache (a linear one's slots are positions),
 // then of the call's own keys, from the first to the last that one of its q-cols sees. lo_top, hi_low: positions from
 // the one to below the other are seen by all of the wave's q-cols.
@@ -726,10 +545,11 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
     // dims, whose stages fit, took 39.5 us so and 40.7 directly)
     constexpr bool kDirect = D == 256 && S == kBf16;
     const int rows_pad = OWN ? (a.own + 63) / 64 * 64 : a.slots_pad;
+    auto tile_entries = [&](int t) { return (size_t(h) * size_t(rows_pad) + size_t(t) * R::TK) * (D / 8); };
     auto load_k = [&](int t) {
       if constexpr (kDirect) {   // (past the last: nothing)
         if (t < e)
-          stage.direct(OWN ? a.pk : reinterpret_cast<const uint4*>(a.ck), h, rows_pad, t, kbuf + ((t - f) & 1) * R::kEntries, false);
+          stage.direct((OWN ? a.pk : reinterpret_cast<const uint4*>(a.ck)) + tile_entries(t), kbuf + ((t - f) & 1) * R::kEntries, false);
       }
       t = min(t, e - 1);   // past the last: loaded again, and not used
       pos = -1;
@@ -754,7 +574,7 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
     auto load_v = [&](int t) {
       if constexpr (kDirect) {
         if (t < e)
-          stage.direct(OWN ? a.pv : reinterpret_cast<const uint4*>(a.cv), h, rows_pad, t, vbuf + ((t - f) & 1) * R::kEntries, true);
+          stage.direct((OWN ? a.pv : reinterpret_cast<const uint4*>(a.cv)) + tile_entries(t), vbuf + ((t - f) & 1) * R::kEntries, true);
         return;
       }
       t = min(t, e - 1);
@@ -945,40 +765,10 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
       for (int r = 0; r < 16; ++r) bad |= live && not_finite(acc[d][r]);
     const long long out = live ? (long long)((size_t(row) * size_t(a.heads) + size_t(head)) * D) : -1;
     __syncthreads();   // the last tile's buffer, and bounds
-    // a lane has a q-col's values 512 bytes or more from its neighbour's: they are turned in LDS, a wave its own 32 rows
-    auto write = [&](auto* to) {
-      using X = std::remove_pointer_t<decltype(to)>;
-      constexpr int DP = sizeof(X) == 4 && D > 128 ? 128 : D, PITCH = DP + 16 / int(sizeof(X));   // dims of a pass
-      static_assert(kExtWaves * 32 * PITCH * sizeof(X) <= R::kLds, "the tiles' buffers hold the rows");
-      X* mine = reinterpret_cast<X*>(smem) + wave * 32 * PITCH;
-#pragma unroll
-      for (int p = 0; p < D; p += DP) {
-        if (p) __syncthreads();
-#pragma unroll
-        for (int d = 0; d < R::NB; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int v = 32 * d + 8 * (r >> 2) + (r & 3);   // and 4 half
-            const int low = Tile<D, T>::dim(v >> 4, v & 15), step = Tile<D, T>::dim(0, 4) - Tile<D, T>::dim(0, 0);
-            if (low < p || low >= p + DP) continue;   // (with half = 1 on the same side)
-            mine[(lane & 31) * PITCH + low - p + half * step] = X(acc[d][r] * inv);
-          }
-        __syncthreads();
-        constexpr int CH = DP * int(sizeof(X)) / 16, PER = 64 / CH;   // 16-byte pieces of a row; rows at a time
-#pragma unroll
-        for (int c = 0; c < 32; c += PER) {
-          const int of = c + lane / CH, piece = lane % CH;
-          const int lo32 = __shfl(int(uint32_t(out)), of), hi32 = __shfl(int(out >> 32), of);
-          if (hi32 < 0) continue;
-          const size_t at = (size_t(uint32_t(hi32)) << 32 | size_t(uint32_t(lo32))) + size_t(p);
-          reinterpret_cast<uint4*>(to + at)[piece] = reinterpret_cast<const uint4*>(mine + of * PITCH)[piece];
-        }
-      }
-    };
     if (a.bf16)
-      write(static_cast<__bf16*>(a.out));
+      turned_rows<D, T>(static_cast<__bf16*>(a.out), acc, inv, out, smem);
     else
-      write(static_cast<float*>(a.out));
+      turned_rows<D, T>(static_cast<float*>(a.out), acc, inv, out, smem);
     const uint64_t any = __ballot((bad && !not_finite(l)) || (live && no_sum(l, row)));
     if (lane == 0) bounds[wave][0] = int(uint32_t(any) | uint32_t(any >> 32));
     __syncthreads();

@@ -180,9 +180,18 @@ constexpr float kLarge = 8388608.f;   // 2^23
 
 __device__ inline bool not_finite(float x) { return !(fabsf(x) <= FLT_MAX); }
 
+// A load of a tile's codes. STREAM: past the caches, for a cache that is read once (decode steps of 64 sequences over 8-bit
+// pages: 100.7 -> 90.6 us; but a prompt's blocks, which read the same tiles, 82 -> 86).
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <bool STREAM>
+__device__ inline uint4 load16(const uint4* p) {
+  if constexpr (STREAM) return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
+  return *p;
+}
+
 // A wave's tile of 32 slots: the keys of a lane's scores are slots 4 g + e and 16 + 4 g + e - 4. k(b, st), v(dd): the
 // operands; dim(dd, r): the dim of row r of product dd. A tile is loaded from `at`, its first slot's place in the head-major arrays
-// a.ck, a.cv, a.ks and a.vs.
+// a.ck, a.cv, a.ks and a.vs (A::kStream: load16).
 template <int D, int T>
 struct Tile;
 
@@ -198,13 +207,13 @@ struct Tile<D, kBf16> {
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) kw[b][c] = p[(b * (D / 32) + c) * 64];
+      for (int c = 0; c < D / 32; ++c) kw[b][c] = load16<A::kStream>(p + (b * (D / 32) + c) * 64);
   }
   template <class A>
   __device__ void load_v(const A& a, size_t at, int lane) {
     const uint4* p = reinterpret_cast<const uint4*>(a.cv) + at * (D / 8) + lane;
 #pragma unroll
-    for (int dd = 0; dd < D / 16; ++dd) vw[dd] = p[dd * 64];
+    for (int dd = 0; dd < D / 16; ++dd) vw[dd] = load16<A::kStream>(p + dd * 64);
   }
   __device__ bf16x8 k(int b, int st) const { return __builtin_bit_cast(bf16x8, kw[b][st]); }
   __device__ void begin_v() {}
@@ -224,7 +233,7 @@ struct Tile<D, kFp8> {
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) kw[b][c] = p[(b * (D / 64) + c) * 64];
+      for (int c = 0; c < D / 64; ++c) kw[b][c] = load16<A::kStream>(p + (b * (D / 64) + c) * 64);
     load8(ks, static_cast<const float*>(a.ks) + at + 4 * (lane >> 4));
     load8(vs, static_cast<const float*>(a.vs) + at + 4 * (lane >> 4));
   }
@@ -236,7 +245,7 @@ struct Tile<D, kFp8> {
   __device__ void load_v(const A& a, size_t at, int lane) {
     const uint4* p = reinterpret_cast<const uint4*>(a.cv) + at * (D / 16) + lane;
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) vw[c] = p[c * 64];
+    for (int c = 0; c < D / 32; ++c) vw[c] = load16<A::kStream>(p + c * 64);
   }
   __device__ bf16x8 k(int b, int st) const {
     const uint4 w = kw[b][st >> 1];
@@ -302,23 +311,42 @@ struct FewState {
   f32x4 acc[QB][D / 16];
 };
 
-// One tile. next_k loads the next tile's keys once this one's are used, next_v its values: each load has about half a
+// A q operand in LDS says so with kInLds: its chunks are then read one ahead of their products, no sooner (all at once they
+// took as many registers as an operand that is kept there).
+template <class Q, class = void>
+struct InLds : std::false_type {};
+template <class Q>
+struct InLds<Q, std::enable_if_t<Q::kInLds>> : std::true_type {};
+
+// One tile. q(qb, c): chunk c of the operand of a lane's q-col in block qb. next_k loads the next tile's keys once this one's are used, next_v its values: each load has about half a
 // tile's work to land behind.
-template <int D, int QB, int MOD, class TILE, class X8, class NK, class NV>
-__device__ inline void few_tile(TILE& T, const X8 (&q)[QB][D / 32], const Span (&span)[QB],
+template <int D, int QB, int MOD, class TILE, class Q, class NK, class NV>
+__device__ inline void few_tile(TILE& T, Q&& q, const Span (&span)[QB],
                                 const Score (&sc)[QB], FewState<D, QB>& st, int4 p0, int4 p1, NK&& next_k, NV&& next_v) {
   const int pos[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
+  using X8 = decltype(q(0, 0));
+  constexpr bool kAhead = InLds<std::remove_reference_t<Q>>::value;
   f32x4 s[QB][2];
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) s[qb][0] = s[qb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  X8 x[QB], ahead[QB];
 #pragma unroll
-  for (int b = 0; b < 2; ++b)
+  for (int qb = 0; qb < QB; ++qb) ahead[qb] = q(qb, 0);
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
+  for (int c = 0; c < D / 32; ++c) {
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+      x[qb] = ahead[qb];
+      if (c + 1 < D / 32) ahead[qb] = q(qb, c + 1);
+    }
+    if constexpr (kAhead) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
       const X8 k = T.k(b, c);
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) s[qb][b] = mfma16(k, q[qb][c], s[qb][b]);
+      for (int qb = 0; qb < QB; ++qb) s[qb][b] = mfma16(k, x[qb], s[qb][b]);
     }
+  }
   float ks[8], vs[8];
   if constexpr (TILE::kScaled) {
 #pragma unroll
@@ -368,6 +396,227 @@ __device__ inline void few_tile(TILE& T, const X8 (&q)[QB][D / 32], const Span (
     for (int qb = 0; qb < QB; ++qb) st.acc[qb][dd] = mfma16(v, w[qb], st.acc[qb][dd]);
   }
   next_v();
+}
+
+// ------------------------------------------------------------------------------------------ tiles in LDS
+
+// A tile of TK keys in LDS: K as [32-key block][16-dim step][64 lanes] entries of 8 dims, V as [32-row block][key step]
+// [64 lanes] entries of 8 keys: A operands of v_mfma_f32_32x32x16. Lane (half, i) of a K entry has key i and dims
+// 8 half .. +8 of the step, of a V entry row i and keys 8 a + 4 half + e, 16 + 8 a + 4 half + e (e = 0 .. 3) of step
+// a = 0, 1 of a 32-key block: what the lane's scores are of. A cache's entries are these too, in another order.
+// Two buffers of each, with the tiles' positions, FP8 scales and first and last position.
+template <int D>
+struct Rows {
+  static constexpr int TK = D == 256 ? 32 : 64;
+  static constexpr int KB = TK / 32, NS = D / 16, NB = D / 32, KS = TK / 16;
+  static constexpr int kEntries = TK * D / 8;           // of K, and of V
+  static constexpr int PER = kEntries / 256;            // entries a thread stages
+  static constexpr int kInfo = 3 * TK + 4;              // ints of a tile's positions, scales and extremes
+  static constexpr size_t kLds = size_t(kEntries) * 64 + size_t(kInfo) * 8 + 2048 + (D == 256 ? 2 * 4096 : 0);
+  // (and room to turn the output; for heads of 256 dims, for two chunks of q)
+};
+
+// A thread's number among the 256 that share tiles.
+__device__ inline int stage_thread() { return int(threadIdx.x) & 255; }
+
+// What a thread stages of a tile: loads in flight (raw), then entries written to LDS. A cache of an odd number of 32-slot
+// tiles ends in the middle of a 64-key tile (`half`): its other half is zeros.
+template <int D, int T>
+struct Stage;
+
+// BF16: entries as they are. Also the packed own keys.
+template <int D>
+struct Stage<D, kBf16> {
+  using R = Rows<D>;
+  uint4 k[R::PER], v[R::PER];
+  __device__ static void load(uint4 (&x)[R::PER], const uint4* c, int h, int pad, int tile, bool half) {
+    const size_t at = (size_t(h) * size_t(pad) + size_t(tile) * R::TK) * (D / 8) + size_t(stage_thread());
+#pragma unroll
+    for (int u = 0; u < R::PER; ++u) x[u] = half && 2 * u >= R::PER ? make_uint4(0, 0, 0, 0) : c[at + u * 256];
+  }
+  __device__ void load_k(const uint4* ck, int h, int pad, int tile, bool half) { load(k, ck, h, pad, tile, half); }
+  __device__ void load_v(const uint4* cv, int h, int pad, int tile, bool half) { load(v, cv, h, pad, tile, half); }
+  // The tile straight into its place in LDS: 64 entries a wave's load, a lane's the one that comes to its part of them.
+  __device__ static void direct(const uint4* from, uint4* to, bool v) {
+    const int lane = stage_thread() & 63, half = lane >> 5, i = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(stage_thread() >> 6);
+#pragma unroll
+    for (int u = 0; u < R::PER; ++u) {
+      const int row = u * 4 + wave;   // of 64 entries
+      int x;
+      if (v) {
+        const int dd = row / R::KS * 2 + (i >> 4), ks = row % R::KS;
+        x = (ks >> 1) * 4 * D + dd * 64 + ((ks & 1) * 2 + half) * 16 + (i & 15);
+      } else {
+        const int b = row / R::NS * 2 + (i >> 4), st = row % R::NS;
+        x = b * 2 * D + (st >> 1) * 64 + ((st & 1) * 2 + half) * 16 + (i & 15);
+      }
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + x),
+                                       (__attribute__((address_space(3))) void*)(to + row * 64), 16, 0, 0);
+    }
+  }
+  // entry x of a BF16 tile of TK keys to its place
+  __device__ static int k_place(int x) {
+    const int b = x / (2 * D), c = x / 64 % (D / 32), g = x >> 4 & 3, i = x & 15;
+    return ((b >> 1) * R::NS + 2 * c + (g >> 1)) * 64 + (g & 1) * 32 + (b & 1) * 16 + i;
+  }
+  __device__ static int v_place(int x) {
+    const int t = x / (4 * D), dd = x / 64 % (D / 16), g = x >> 4 & 3, i = x & 15;
+    return ((dd >> 1) * R::KS + 2 * t + (g >> 1)) * 64 + (g & 1) * 32 + (dd & 1) * 16 + i;
+  }
+  __device__ void store_k(uint4* lk) const {
+#pragma unroll
+    for (int u = 0; u < R::PER; ++u) lk[k_place(stage_thread() + u * 256)] = k[u];
+  }
+  __device__ void store_v(uint4* lv) const {
+#pragma unroll
+    for (int u = 0; u < R::PER; ++u) lv[v_place(stage_thread() + u * 256)] = v[u];
+  }
+};
+
+// FP8: a 16-byte load is two entries' codes.
+template <int D>
+struct Stage<D, kFp8> {
+  using R = Rows<D>;
+  using B = Stage<D, kBf16>;
+  uint4 k[R::PER / 2], v[R::PER / 2];
+  __device__ static void load(uint4 (&x)[R::PER / 2], const uint4* c, int h, int pad, int tile, bool half) {
+    const size_t at = (size_t(h) * size_t(pad) + size_t(tile) * R::TK) * (D / 16) + size_t(stage_thread());
+#pragma unroll
+    for (int u = 0; u < R::PER / 2; ++u) {
+      const bool past = half && stage_thread() + u * 256 >= R::kEntries / 4;
+      x[u] = past ? make_uint4(0, 0, 0, 0) : c[at + u * 256];
+    }
+  }
+  __device__ void load_k(const uint4* ck, int h, int pad, int tile, bool half) { load(k, ck, h, pad, tile, half); }
+  __device__ void load_v(const uint4* cv, int h, int pad, int tile, bool half) { load(v, cv, h, pad, tile, half); }
+  __device__ static int first(int u) {   // of BF16's entries
+    const int x = stage_thread() + u * 256;
+    return (x >> 6) * 128 + (x & 63);
+  }
+  __device__ void store_k(uint4* lk) const {
+#pragma unroll
+    for (int u = 0; u < R::PER / 2; ++u) {
+      lk[B::k_place(first(u))] = __builtin_bit_cast(uint4, fp8_operand(k[u].x, k[u].y));
+      lk[B::k_place(first(u) + 64)] = __builtin_bit_cast(uint4, fp8_operand(k[u].z, k[u].w));
+    }
+  }
+  __device__ void store_v(uint4* lv) const {
+#pragma unroll
+    for (int u = 0; u < R::PER / 2; ++u) {
+      lv[B::v_place(first(u))] = __builtin_bit_cast(uint4, fp8_operand(v[u].x, v[u].y));
+      lv[B::v_place(first(u) + 64)] = __builtin_bit_cast(uint4, fp8_operand(v[u].z, v[u].w));
+    }
+  }
+};
+
+// NVFP4: a thread's codes are PER entries of K, which share a key, and PER of V, which share their keys' scales.
+template <int D>
+struct Stage<D, kNvfp4> {
+  using R = Rows<D>;
+  uint32_t k[R::PER], v[R::PER], ks;
+  uint2 vs;
+  template <class A>
+  __device__ void load_k(const A& a, int h, int tile, bool half) {
+    const size_t at = size_t(h) * size_t(a.slots_pad) + size_t(tile) * R::TK;
+    const int tid = stage_thread();
+#pragma unroll
+    for (int u = 0; u < R::PER; ++u) k[u] = 0;
+    ks = 0;
+    if (half && tid >= 128) return;
+    take(k, a.ck + at * (D / 2), tid);
+    const uint8_t* s = static_cast<const uint8_t*>(a.ks) + at * (D / 16);
+    ks = D == 64 ? s[tid] : reinterpret_cast<const uint16_t*>(s)[tid];
+  }
+  // V: a wave has half a 32-slot tile's words (256 dims: a quarter)
+  template <class A>
+  __device__ void load_v(const A& a, int h, int tile, bool half) {
+    const size_t at = size_t(h) * size_t(a.slots_pad) + size_t(tile) * R::TK;
+    const int tid = stage_thread(), lane = tid & 63, part = tid >> 6, t = D == 256 ? 0 : part >> 1;
+#pragma unroll
+    for (int u = 0; u < R::PER; ++u) v[u] = 0;
+    vs = make_uint2(0, 0);
+    if (half && tid >= 128) return;
+    take_v(a.cv + at * (D / 2), part, lane);
+    const uint2* sv = reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.vs) + at * (D / 16));
+    vs = sv[t * (D / 4) + (lane >> 4) * (D / 16) + (lane & 15) * (D / 16) / 16];
+  }
+  __device__ void take(uint32_t (&w)[R::PER], const uint8_t* p, int tid) {
+    if constexpr (R::PER == 4) {
+      const uint4 x = reinterpret_cast<const uint4*>(p)[tid];
+      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else {
+      const uint2 x = reinterpret_cast<const uint2*>(p)[tid];
+      w[0] = x.x, w[1] = x.y;
+    }
+  }
+  // words of products first_dd(part) .. of a lane
+  __device__ void take_v(const uint8_t* p, int part, int lane) {
+    if constexpr (R::PER == 4) {
+      const uint4 x = reinterpret_cast<const uint4*>(p)[part * 64 + lane];   // [tile][4 products][lane]
+      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    } else {   // 64 dims: one 16-byte group a tile, half of it a wave
+      const uint2 x = reinterpret_cast<const uint2*>(p)[((part >> 1) * 64 + lane) * 2 + (part & 1)];
+      v[0] = x.x, v[1] = x.y;
+    }
+  }
+  __device__ void store_k(uint4* lk) const {
+    const int tid = stage_thread(), lane = tid & 63, part = tid >> 6, g = lane >> 4, i = lane & 15;
+    // D = 64, 128: 16-slot block `part`; 256: block part / 2, chunk part % 2
+    const int b = D == 256 ? part >> 1 : part, chunk = D == 256 ? part & 1 : 0;
+#pragma unroll
+    for (int c = 0; c < R::PER; ++c) {
+      const int dim8 = chunk * 16 + g * R::PER + c;   // dims 8 dim8 .. +8
+      lk[((b >> 1) * R::NS + (dim8 >> 1)) * 64 + (dim8 & 1) * 32 + (b & 1) * 16 + i] =
+          __builtin_bit_cast(uint4, dequant8(k[c], scale_pair(ks, c >> 1)));
+    }
+  }
+  __device__ void store_v(uint4* lv) const {
+    const int tid = stage_thread(), lane = tid & 63, part = tid >> 6, g = lane >> 4, i = lane & 15;
+    f16x2 s[4];
+    v_scales(vs, s);
+    const int t = D == 256 ? 0 : part >> 1, dd0 = (D == 256 ? part : part & 1) * R::PER;
+#pragma unroll
+    for (int c = 0; c < R::PER; ++c) {
+      const int dd = dd0 + c;
+      lv[((dd >> 1) * R::KS + 2 * t + (g >> 1)) * 64 + (g & 1) * 32 + (dd & 1) * 16 + i] =
+          __builtin_bit_cast(uint4, dequant8_pairs(v[c], s));
+    }
+  }
+};
+
+// The accumulators of 128 q-cols, 32 a wave, times inv as rows of `to`, a lane's at `out` (-1: not written). A lane has a
+// q-col's values 512 bytes or more from its neighbour's: they are turned in LDS, a wave its own 32 rows.
+template <int D, int T, class X>
+__device__ inline void turned_rows(X* to, const f32x16 (&acc)[Rows<D>::NB], float inv, long long out, uint8_t* smem) {
+  using R = Rows<D>;
+  constexpr int DP = sizeof(X) == 4 && D > 128 ? 128 : D, PITCH = DP + 16 / int(sizeof(X));   // dims of a pass
+  static_assert(4 * 32 * PITCH * sizeof(X) <= R::kLds, "the tiles' buffers hold the rows");
+  const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) >> 6, half = lane >> 5;
+  X* mine = reinterpret_cast<X*>(smem) + wave * 32 * PITCH;
+#pragma unroll
+  for (int p = 0; p < D; p += DP) {
+    if (p) __syncthreads();
+#pragma unroll
+    for (int d = 0; d < R::NB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int v = 32 * d + 8 * (r >> 2) + (r & 3);   // and 4 half
+        const int low = Tile<D, T>::dim(v >> 4, v & 15), step = Tile<D, T>::dim(0, 4) - Tile<D, T>::dim(0, 0);
+        if (low < p || low >= p + DP) continue;   // (with half = 1 on the same side)
+        mine[(lane & 31) * PITCH + low - p + half * step] = X(acc[d][r] * inv);
+      }
+    __syncthreads();
+    constexpr int CH = DP * int(sizeof(X)) / 16, PER = 64 / CH;   // 16-byte pieces of a row; rows at a time
+#pragma unroll
+    for (int c = 0; c < 32; c += PER) {
+      const int of = c + lane / CH, piece = lane % CH;
+      const int lo32 = __shfl(int(uint32_t(out)), of), hi32 = __shfl(int(out >> 32), of);
+      if (hi32 < 0) continue;
+      const size_t at = (size_t(uint32_t(hi32)) << 32 | size_t(uint32_t(lo32))) + size_t(p);
+      reinterpret_cast<uint4*>(to + at)[piece] = reinterpret_cast<const uint4*>(mine + of * PITCH)[piece];
+    }
+  }
 }
 
 }  // namespace xtg::hip

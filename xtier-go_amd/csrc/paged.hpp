@@ -91,31 +91,35 @@ struct PagedAttnCall {
   float scale, softcap;
 };
 
-// How an attention call is cut up. A q-col is a (row, q head of a KV head). A sequence's q-cols go in blocks of `cols`; of a
-// block's keys, a work-group takes one of several parts for one KV head, about `budget` work-groups a KV head in all, and
-// leaves a record (accumulator, maximum, sum) for each q-col where there is more than one part.
+// How an attention call is cut up. A q-col is a (row, q head of a KV head). A sequence of up to `cols` of them (a decode or
+// verify step) is one block of `cols`, whose work-groups' waves take tiles of their own; one of more goes in blocks of
+// kManyCols, whose work-groups' waves share tiles. Of a block's keys a work-group takes one of several parts for one KV head,
+// about `budget` work-groups a KV head in all, and leaves a record (accumulator, maximum, sum) for each q-col where there is
+// more than one part.
 struct PagedPlan {
   int cols = 16, budget = 1;
+  bool many = false;             // a sequence of the call can have more than `cols` q-cols
   int tasks = 1;                 // work-groups a KV head, at most
-  int records = 1;               // of them with a record, at most
+  int records = 0;               // q-cols of a KV head with records, at most: those of its work-groups with more than one part
   size_t acc_bytes = 0, ml_bytes = 0, info_bytes = 0;
   size_t bytes() const { return acc_bytes + ml_bytes + info_bytes; }
 };
 PagedPlan paged_plan(const PagedAttnCall& a, int cus);
 
-constexpr int kPagedWaves = 4;
-// Fewest tiles of a work-group that shares its keys with others: one a wave.
-constexpr int kPagedLeast = kPagedWaves;
+constexpr int kManyCols = 128;
+// Fewest tiles of a part: one a wave; and of a block of many q-cols, whose records are as large as 32 tiles.
+constexpr int kFewLeast = 4, kManyLeast = 32;
 
 struct PagedArgs {
+  static constexpr bool kStream = true;   // a sequence of one block: its tiles are read once
   Seqs s;
   const void* q;
   void* out;
   const uint8_t *ck, *cv;
   const void *ks, *vs;
-  float *acc, *ml;               // records [record][KV head][cols][d], [..][2]
-  int4* info;                    // of each q-col [row][q head of its KV head]: first record, the next one's distance,
-                                 // parts << 8 | col, sequence
+  float *acc, *ml;               // records: of a piece, [KV head][its q-cols][d], [..][2]
+  int4* info;                    // of each q-col [row][q head of its KV head]: its piece's place, the blocks of its sequence
+                                 // << 1 | many, parts << 8 | col, sequence
   long long ldq;
   int heads, kv_heads, group, cols, budget, records, window, bf16;
   uint32_t group_inv;            // ceil(2^16 / group)
@@ -128,11 +132,15 @@ struct PagedArgs {
 // sequence that is left out has its rows' blocks, and no tile.
 struct Extent {
   Seq q;
+  bool many;
   int blocks, tiles, lo;
+  __host__ __device__ int cols(const PagedArgs& a) const { return many ? kManyCols : a.cols; }
 };
 __host__ __device__ inline Extent extent(const PagedArgs& a, int s) {
-  Extent x = {seq_at(a.s, s), 0, 0, 0};
-  x.blocks = int(((long long)x.q.n * a.group + a.cols - 1) / a.cols);
+  Extent x = {seq_at(a.s, s), false, 0, 0, 0};
+  const long long cols = (long long)x.q.n * a.group;
+  x.many = cols > a.cols;
+  x.blocks = int((cols + x.cols(a) - 1) / x.cols(a));
   if (x.q.pos >= 0 && x.q.n > 0) {
     const int cap = a.s.max_pages << a.s.shift, end = x.q.pos + x.q.n < cap ? x.q.pos + x.q.n : cap;
     const int lo = a.window > 0 && x.q.pos >= a.window ? x.q.pos - a.window + 1 : 0;
@@ -142,13 +150,26 @@ __host__ __device__ inline Extent extent(const PagedArgs& a, int s) {
   }
   return x;
 }
-// The parts of a block's tiles, where `total` is the sum of all blocks' tiles.
-__host__ __device__ inline int parts_of(const PagedArgs& a, int tiles, float total) {
-  int chunk = int(total / float(a.budget)) + 1;   // tiles of a part
-  if (chunk < kPagedLeast) chunk = kPagedLeast;
-  const int n = (tiles + chunk - 1) / chunk;
+// The parts of a block's tiles, `chunk` tiles each; of many q-cols about as many.
+__host__ __device__ inline int parts_of(const Extent& x, int chunk) {
+  if (x.many && chunk < kManyLeast) chunk = kManyLeast;
+  const int n = (x.tiles + (x.many ? chunk / 2 : chunk - 1)) / chunk;
   return n > 1 ? n : 1;
 }
+// The tiles of a part: an even share of all blocks' tiles `total` for each of `budget` work-groups, then, as begun parts
+// make more than that (`tasks`), a larger one, unless the blocks alone are as many. Returns whether it changed.
+// One long sequence takes half as many work-groups, one a CU: more than 32 records of a q-col cost the merge more than the
+// second one a CU brings (one token over 32768 BF16 positions of 8 KV heads of 128 dims: 32.2 -> 30.0 us).
+__host__ __device__ inline int first_chunk(const PagedArgs& a, float total, int blocks) {
+  const int chunk = int(total / float(blocks * 32LL < a.budget ? (a.budget + 1) / 2 : a.budget)) + 1;
+  return chunk < kFewLeast ? kFewLeast : chunk;
+}
+__host__ __device__ inline bool next_chunk(const PagedArgs& a, int& chunk, int tasks, int blocks) {
+  if (tasks <= a.budget || blocks >= a.budget || chunk >= 1 << 24) return false;
+  chunk += int(float(chunk) * float(tasks - a.budget) / float(a.budget)) + 1;
+  return true;
+}
+constexpr int kChunkSteps = 3;
 
 using PagedTimed = std::function<void(const std::function<std::string()>&)>;
 void launch_paged_attn(const PagedAttnCall& a, const PagedPlan& p, void* scratch, hipStream_t stream, const PagedTimed& timed);

@@ -12,20 +12,23 @@ namespace xtg::hip {
 
 PagedPlan paged_plan(const PagedAttnCall& a, int cus) {
   PagedPlan p;
-  const int kv_heads = a.cache->kv_heads, group = a.heads / kv_heads;
+  const int kv_heads = a.cache->kv_heads, group = a.heads / kv_heads, seqs = a.seqs.n_seqs;
   const long long cols = (long long)a.seqs.n_rows * group;
-  p.cols = cols <= 16LL * a.seqs.n_seqs ? 16 : 32;
-  // the work-groups that are resident at once, two a CU
-  p.budget = std::max(1, 2 * cus / kv_heads);
+  // 32 q-cols a work-group where sequences have more than 16 on the average, but not a prompt's number
+  p.cols = cols > 16LL * seqs && cols <= 32LL * seqs ? 32 : 16;
+  // (heads of 256 dims: 32 do not fit a wave's registers where work-groups have eight)
+  const long long most = a.seqs.starts ? cols : group;   // q-cols of a sequence
+  if (a.cache->head_dim == 256 && most > p.cols) p.cols = 16;
+  p.many = most > p.cols;
+  // the work-groups that are resident at once
+  p.budget = std::max(1, (p.many ? cus : 2 * cus) / kv_heads);
   // a sequence's last block and a block's last part are begun ones; and total / budget is rounded, in FP32
-  const long long blocks = a.seqs.starts ? cols / p.cols + a.seqs.n_seqs : (long long)a.seqs.n_seqs * ((group + p.cols - 1) / p.cols);
-  const long long tasks = blocks + p.budget + p.budget / 64 + 1;
-  XTG_CHECK(tasks * kv_heads < (1LL << 31), "paged_attention: %d rows of %d sequences and %d heads", a.seqs.n_rows,
-            a.seqs.n_seqs, a.heads);
+  const long long parts = p.budget + p.budget / 64 + 1, tasks = (p.many ? cols / kManyCols : 0) + seqs + parts;
+  XTG_CHECK(tasks * kv_heads < (1LL << 31), "paged_attention: %d rows of %d sequences and %d heads", a.seqs.n_rows, seqs, a.heads);
   p.tasks = int(tasks);
   // a block of several parts has at least one whole part's tiles for every two of them
-  p.records = int(std::min<long long>(tasks, 2 * (p.budget + p.budget / 64 + 1)));
-  const size_t n = size_t(p.records) * size_t(kv_heads) * size_t(p.cols);
+  p.records = int(std::min(tasks, 2 * parts)) * (p.many ? kManyCols : p.cols);
+  const size_t n = size_t(p.records) * size_t(kv_heads);
   p.acc_bytes = n * size_t(a.cache->head_dim) * sizeof(float);
   p.ml_bytes = n * 2 * sizeof(float);
   p.info_bytes = size_t(a.seqs.n_rows) * size_t(group) * sizeof(int4);

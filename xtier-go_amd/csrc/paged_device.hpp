@@ -21,6 +21,9 @@ __device__ inline int wave_scan(int v) {
   return v;
 }
 
+// Sum of v over a wave, in every lane.
+__device__ inline int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+
 // Piece `task` of the sequences' pieces laid end to end, count(s) of sequence s: its sequence and its number there, by a wave
 // (every lane gets both); false past the last.
 template <class C>
