@@ -28,6 +28,8 @@ PagedPlan paged_plan(const PagedAttnCall& a, int cus) {
   p.tasks = int(tasks);
   // a block of several parts has at least one whole part's tiles for every two of them
   p.records = int(std::min(tasks, 2 * parts)) * (p.many ? kManyCols : p.cols);
+  // (tables of a few hundred positions: no block has a second part, and no merge is launched)
+  if (((long long)a.seqs.max_pages << a.seqs.shift) <= 32 * kFewLeast) p.records = 0;
   const size_t n = size_t(p.records) * size_t(kv_heads);
   p.acc_bytes = n * size_t(a.cache->head_dim) * sizeof(float);
   p.ml_bytes = n * 2 * sizeof(float);

@@ -59,10 +59,13 @@ template <bool MANY>
 __device__ inline bool piece_of(const PagedArgs& a, int task, Piece& p) {
   // about `budget` work-groups a KV head share the tiles of all blocks evenly
   const int lane = int(__lane_id());
+  Extent own = {};   // of the lane's sequence among the first 64, which is looked up once
+  if (lane < a.s.n_seqs) own = extent(a, lane);
+  auto extent_of = [&](int s) { return s < 64 ? own : extent(a, s); };
   float total = 0.f;
   int all = 0;
   for (int s = lane; s < a.s.n_seqs; s += 64) {
-    const Extent x = extent(a, s);
+    const Extent x = extent_of(s);
     total += float(x.blocks) * float(x.tiles);
     all += x.blocks;
   }
@@ -71,7 +74,7 @@ __device__ inline bool piece_of(const PagedArgs& a, int task, Piece& p) {
   for (int step = 0; step < kChunkSteps && all < a.budget; ++step) {
     int n = 0;
     for (int s = lane; s < a.s.n_seqs; s += 64) {
-      const Extent x = extent(a, s);
+      const Extent x = extent_of(s);
       n += x.blocks * parts_of(x, chunk);
     }
     if (!next_chunk(a, chunk, wave_total(n), all)) break;
@@ -84,7 +87,7 @@ __device__ inline bool piece_of(const PagedArgs& a, int task, Piece& p) {
       int n = 0, splits = 1;
       Extent x = {};
       if (s < a.s.n_seqs) {
-        x = extent(a, s);
+        x = extent_of(s);
         splits = parts_of(x, chunk);
         n = int(x.many) == role ? x.blocks * splits : 0;
       }
@@ -719,6 +722,7 @@ __device__ inline void many_piece(const PagedArgs& a, const Piece& p, int h, uin
             for (int r = 0; r < 4; ++r) y[b][4 * j + r] = begin<MOD>(sc, T == kFp8 ? s[b][4 * j + r] * k4[r] : s[b][4 * j + r], 0);
           }
         if (first < lo_top || first + R::TK > hi_low) {
+          asm volatile("");   // (kept behind the branch: asked for every tile, masks are a fifth of its vector operations)
           const int at = first + 4 * half - span.lo;
 #pragma unroll
           for (int b = 0; b < R::KB; ++b)
@@ -1050,7 +1054,7 @@ void paged_go(const PagedAttnCall& c, const PagedPlan& p, const PagedArgs& a, hi
     HIP_CHECK(hipGetLastError());
     return strf("paged_attn_kernel<%d, %d, %d, %d, %d>", D, p.cols / 16, T, MOD, int(p.many));
   });
-  timed([&] {
+  if (p.records > 0) timed([&] {
     const int total = c.seqs.n_rows * c.heads, n = total <= kMergeFew ? 0 : total <= kMergeMost ? 1 : 4;
     auto go = [&](auto kernel, int cols) {
       hipLaunchKernelGGL(kernel, dim3(unsigned((total + cols - 1) / cols)), dim3(256), 0, stream, a, total);

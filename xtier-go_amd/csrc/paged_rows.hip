@@ -144,13 +144,17 @@ __device__ inline bool tile_task(const Seqs& s, int kv_heads, int id, TileTask& 
 template <int D, int T, class X>
 __device__ inline void append_tile(const AppendArgs& a, uint32_t* not_finite) {
   constexpr int C = D / 16, KP = 256 / C < 32 ? 256 / C : 32, P = D / 64;
-  TileTask t;
-  if (!tile_task(a.s, a.kv_heads, int(blockIdx.x), t) || t.page < 0) return;   // (the whole work-group)
   const int tid = int(threadIdx.x), size = 1 << a.s.shift;
-  const int hh = t.page * a.kv_heads + t.head;   // the pool's head
   const int c = tid % C, key0 = tid / C;
+  // Loads go out as soon as what they need is known: frequencies, then the rows, then the page.
+  double f[8] = {};
+  if (a.freq) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = a.freq[8 * c + e];
+  }
+  TileTask t;
+  if (!tile_task(a.s, a.kv_heads, int(blockIdx.x), t)) return;   // (the whole work-group)
   const int v_dim = (tid & 63) * P, g = tid >> 6;
-  // every load of the rows goes out first
   float lo[32 / KP][8], hi[32 / KP][8], v[8][P];
   float2 cs[32 / KP][8];
   uint32_t live = 0;   // of V's 8 slots
@@ -178,14 +182,14 @@ __device__ inline void append_tile(const AppendArgs& a, uint32_t* not_finite) {
     }
   }
   if (a.freq) {
-    double f[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = a.freq[8 * c + e];
 #pragma unroll
     for (int u = 0; u < 32 / KP; ++u)
 #pragma unroll
       for (int e = 0; e < 8; ++e) cs[u][e] = turned(32 * t.tile + u * KP + key0, f[e]);
   }
+
+  if (t.page < 0) return;   // (the whole work-group)
+  const int hh = t.page * a.kv_heads + t.head;   // the pool's head
 
   // ---- K
 #pragma unroll
@@ -342,6 +346,18 @@ template <int D, class X>
 __device__ inline void append_q(const AppendArgs& a, int row, float2* cs_lds) {
   constexpr int C = D / 16;
   const Seqs& s = a.s;
+  const int chunks = a.heads * C;
+  const X* rows = static_cast<const X*>(a.q) + (long long)row * a.ldq;
+  float lo[8], hi[8];
+  auto load = [&](int x) {
+    const X* from = rows + x / C * D + x % C * 8;
+    load_row4(from, lo);
+    load_row4(from + D / 2, hi);
+  };
+  // loads go out first: the first row's and the frequencies
+  double f = 0.0;
+  if (a.freq && int(threadIdx.x) < D / 2) f = a.freq[threadIdx.x];
+  if (int(threadIdx.x) < chunks) load(int(threadIdx.x));
   int seq = row;
   if (s.starts) {
     int n = 0;   // starts at or before the row
@@ -356,18 +372,14 @@ __device__ inline void append_q(const AppendArgs& a, int row, float2* cs_lds) {
   const int at = row - q.row0;
   if (q.pos < 0 || uint32_t(at) >= uint32_t(q.n)) return;   // (the whole work-group)
   if (a.freq) {
-    if (int(threadIdx.x) < D / 2) cs_lds[threadIdx.x] = turned(q.pos + at, a.freq[threadIdx.x]);
+    if (int(threadIdx.x) < D / 2) cs_lds[threadIdx.x] = turned(q.pos + at, f);
     __syncthreads();
   }
-  const int chunks = a.heads * C;
   for (int x0 = 0; x0 < chunks; x0 += 256) {
     const int x = x0 + int(threadIdx.x), head = x / C, c = x % C;
     if (x >= chunks) break;   // (whole rows of lanes: chunks is a multiple of C)
-    const X* from = static_cast<const X*>(a.q) + (long long)row * a.ldq + head * D;
-    float lo[8], hi[8];
     float2 cs[8];
-    load_row4(from + 8 * c, lo);
-    load_row4(from + D / 2 + 8 * c, hi);
+    if (x0) load(x);
     if (a.freq) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) cs[e] = cs_lds[8 * c + e];
