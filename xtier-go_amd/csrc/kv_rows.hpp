@@ -82,6 +82,15 @@ __device__ inline void store_row4(__bf16* p, const float (&x)[N]) {
     *reinterpret_cast<uint32_t*>(p) = __builtin_bit_cast(uint32_t, b);
     return;
   }
+  if constexpr (N % 8 == 0) {
+#pragma unroll
+    for (int e = 0; e < N; e += 8) {
+      const __bf16 b[8] = {(__bf16)x[e], (__bf16)x[e + 1], (__bf16)x[e + 2], (__bf16)x[e + 3],
+                           (__bf16)x[e + 4], (__bf16)x[e + 5], (__bf16)x[e + 6], (__bf16)x[e + 7]};
+      *reinterpret_cast<uint4*>(p + e) = __builtin_bit_cast(uint4, b);
+    }
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < N; e += 4) {
     const __bf16 b[4] = {(__bf16)x[e], (__bf16)x[e + 1], (__bf16)x[e + 2], (__bf16)x[e + 3]};

@@ -503,9 +503,7 @@ struct PagedStage : Stage<D, T> {
   }
   __device__ void load_k(const PagedArgs& a, size_t at0, size_t at1) {
     const int tid = stage_thread();
-    if constexpr (T == kBf16) {
-      load<R::kEntries>(this->k, reinterpret_cast<const uint4*>(a.ck), at0, at1);
-    } else if constexpr (T == kFp8) {
+    if constexpr (T == kFp8) {
       load<R::kEntries / 2>(this->k, reinterpret_cast<const uint4*>(a.ck), at0, at1);
     } else {
       const size_t at = D == 256 || tid < 128 ? at0 : at1 - 32;   // (in whole tiles' numbering: the second half's own place)
@@ -516,9 +514,7 @@ struct PagedStage : Stage<D, T> {
   }
   __device__ void load_v(const PagedArgs& a, size_t at0, size_t at1) {
     const int tid = stage_thread(), lane = tid & 63, part = tid >> 6;
-    if constexpr (T == kBf16) {
-      load<R::kEntries>(this->v, reinterpret_cast<const uint4*>(a.cv), at0, at1);
-    } else if constexpr (T == kFp8) {
+    if constexpr (T == kFp8) {
       load<R::kEntries / 2>(this->v, reinterpret_cast<const uint4*>(a.cv), at0, at1);
     } else {
       const size_t at = D == 256 || tid < 128 ? at0 : at1 - 32;
@@ -529,16 +525,7 @@ struct PagedStage : Stage<D, T> {
     }
   }
   __device__ void mask_v(int first, int lo, int hi) {
-    const int tid = stage_thread();
-    if constexpr (T == kBf16) {
-#pragma unroll
-      for (int u = 0; u < R::PER; ++u) {
-        const int x = tid + u * 256;
-        const uint32_t ok = valid_of(first + 32 * (x / (4 * D)) + 4 * (x >> 4 & 3), lo, hi);
-        uint4& w = this->v[u];
-        w.x &= pair(ok, 0), w.y &= pair(ok, 2), w.z &= pair(ok, 4), w.w &= pair(ok, 6);
-      }
-    } else if constexpr (T == kFp8) {
+    if constexpr (T == kFp8) {
 #pragma unroll
       for (int u = 0; u < R::PER / 2; ++u) {
         const int x = S::first(u);
@@ -548,9 +535,26 @@ struct PagedStage : Stage<D, T> {
       }
     }   // (NVFP4: as in PagedTile)
   }
-  // BF16 tiles of 256 dims straight into LDS, as Stage::direct; and the same of what a lane loaded, once it is there
-  __device__ static void direct(const uint4* c, size_t at, uint4* to, bool v) {
-    S::direct(c + at * (D / 8), to, v);
+  // BF16 tiles straight into LDS: 64 entries a wave's load, a lane's the one that comes to its part of them; and the mask of
+  // what a lane loaded, once it is there
+  __device__ static void direct(const uint4* c, size_t at0, size_t at1, uint4* to, bool v) {
+    const int tid = stage_thread(), half = tid >> 5 & 1, i = tid & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+#pragma unroll
+    for (int u = 0; u < R::PER; ++u) {
+      const int row = u * 4 + wave;   // of 64 entries
+      // of the 32-slot half: entries of 16-slot blocks and 32-dim chunks, or of 16-dim blocks
+      int part, x;
+      if (v) {
+        const int ks = row % R::KS;
+        part = ks >> 1, x = (row / R::KS * 2 + (i >> 4)) * 64 + ((ks & 1) * 2 + half) * 16 + (i & 15);
+      } else {
+        const int st = row % R::NS;
+        part = row / R::NS, x = (i >> 4) * 2 * D + (st >> 1) * 64 + ((st & 1) * 2 + half) * 16 + (i & 15);
+      }
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(c + (part ? at1 : at0) * (D / 8) + x),
+                                       (__attribute__((address_space(3))) void*)(to + row * 64), 16, 0, 0);
+    }
   }
   __device__ static void mask_direct(uint4* lv, int first, int lo, int hi) {
     const int lane = int(threadIdx.x) & 63, wave = stage_thread() >> 6;
@@ -622,7 +626,7 @@ __device__ inline void many_piece(const PagedArgs& a, const Piece& p, int h, uin
     const size_t q_at = live ? size_t(p.q.row0 + row) * size_t(a.ldq) + size_t(head) * D + size_t(8 * half) : size_t(8 * half);
     row_chunks(a.q, a.bf16, live, [&](int c) { return q_at + size_t(16 * c); }, x);
     PagedStage<D, T> stage;
-    constexpr bool kDirect = D == 256 && T == kBf16;   // (see ext_rows_kernel)
+    constexpr bool kDirect = T == kBf16;
     // the pages of the next 64 tiles' 32-slot halves, one a lane
     int pages = -1, from = f;
     constexpr int HALVES = R::TK / 32;
@@ -642,8 +646,8 @@ __device__ inline void many_piece(const PagedArgs& a, const Piece& p, int h, uin
       t = min(t, e - 1);   // past the last: loaded again, and not used
       const size_t at0 = place_of(a, page0, h, t * R::TK), at1 = HALVES == 2 ? place_of(a, page1, h, t * R::TK + 32) : at0;
       if constexpr (kDirect) {
-        stage.direct(reinterpret_cast<const uint4*>(a.ck), at0, kbuf + buffer(t), false);
-        stage.direct(reinterpret_cast<const uint4*>(a.cv), at0, vbuf + buffer(t), true);
+        stage.direct(reinterpret_cast<const uint4*>(a.ck), at0, at1, kbuf + buffer(t), false);
+        stage.direct(reinterpret_cast<const uint4*>(a.cv), at0, at1, vbuf + buffer(t), true);
       } else {
         stage.load_k(a, at0, at1);
         stage.load_v(a, at0, at1);
@@ -1036,10 +1040,10 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(PagedArgs a, int total
 template <int D, int T, int MOD>
 void paged_go(const PagedAttnCall& c, const PagedPlan& p, const PagedArgs& a, hipStream_t stream, const PagedTimed& timed) {
   timed([&] {
-    const dim3 grid{unsigned(p.tasks) * unsigned(a.kv_heads)}, block{p.many ? 512u : 256u};
+    const dim3 grid{unsigned(p.tasks) * unsigned(a.kv_heads)};
     auto go = [&](auto kernel, size_t lds) {
       allow_lds(reinterpret_cast<const void*>(kernel), lds);
-      hipLaunchKernelGGL(kernel, grid, block, lds, stream, a);
+      paged_queue(kernel, grid, p.many ? 512 : 256, lds, stream, a);
     };
     if (p.cols == 32 && !p.many)
       go(&paged_attn_kernel<D, 2, T, MOD, false>, paged_lds<D, 2, T, false>());
@@ -1051,13 +1055,12 @@ void paged_go(const PagedAttnCall& c, const PagedPlan& p, const PagedArgs& a, hi
       go(&paged_attn_kernel<D, 2, T, MOD, true>, paged_lds<D, 2, T, true>());
     else
       fail("paged_attention: a plan of 32 q-cols for heads of 256 dims");
-    HIP_CHECK(hipGetLastError());
     return strf("paged_attn_kernel<%d, %d, %d, %d, %d>", D, p.cols / 16, T, MOD, int(p.many));
   });
   if (p.records > 0) timed([&] {
     const int total = c.seqs.n_rows * c.heads, n = total <= kMergeFew ? 0 : total <= kMergeMost ? 1 : 4;
     auto go = [&](auto kernel, int cols) {
-      hipLaunchKernelGGL(kernel, dim3(unsigned((total + cols - 1) / cols)), dim3(256), 0, stream, a, total);
+      paged_queue(kernel, dim3(unsigned((total + cols - 1) / cols)), 256, 0, stream, a, total);
     };
     if (n == 0)
       go(&paged_merge_kernel<D, T, 4, 1>, 1);
@@ -1065,7 +1068,6 @@ void paged_go(const PagedAttnCall& c, const PagedPlan& p, const PagedArgs& a, hi
       go(&paged_merge_kernel<D, T, 1, 1>, 4);
     else
       go(&paged_merge_kernel<D, T, 1, 4>, 16);
-    HIP_CHECK(hipGetLastError());
     return strf("paged_merge_kernel<%d, %d, %d, %d>", D, T, n == 0 ? 4 : 1, n > 1 ? n : 1);
   });
 }

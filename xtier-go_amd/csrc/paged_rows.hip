@@ -453,9 +453,8 @@ std::string launch_paged_append(const DevPaged& c, const Seqs& s, const PagedApp
   a.tasks = int(tiles);
   const bool bf16 = p.x_dtype == kXBF16;
   for_shape(c.head_dim, c.type, bf16, [&](auto D, auto T, auto x) {
-    hipLaunchKernelGGL((paged_append_kernel<D(), T(), decltype(x)>), dim3(unsigned(groups)), dim3(256), 0, stream, a);
+    paged_queue(&paged_append_kernel<D(), T(), decltype(x)>, dim3(unsigned(groups)), 256, 0, stream, a);
   });
-  HIP_CHECK(hipGetLastError());
   return strf("paged_append_kernel<%d, %d, %s>", c.head_dim, c.type, bf16 ? "bf16" : "float");
 }
 
@@ -550,9 +549,8 @@ std::string launch_paged_read(const DevPaged& c, const Seqs& s, void* k, void* v
   const long long groups = most_tiles(s) * c.kv_heads;
   XTG_CHECK(groups < (1LL << 31), "paged_read: %d rows of %d sequences and %d KV heads", s.n_rows, s.n_seqs, c.kv_heads);
   for_shape(c.head_dim, c.type, bf16, [&](auto D, auto T, auto x) {
-    hipLaunchKernelGGL((paged_read_kernel<D(), T(), decltype(x)>), dim3(unsigned(groups)), dim3(256), 0, stream, a);
+    paged_queue(&paged_read_kernel<D(), T(), decltype(x)>, dim3(unsigned(groups)), 256, 0, stream, a);
   });
-  HIP_CHECK(hipGetLastError());
   return strf("paged_read_kernel<%d, %d, %s>", c.head_dim, c.type, bf16 ? "bf16" : "float");
 }
 
