@@ -765,10 +765,40 @@ __global__ void __launch_bounds__(kExtWaves * 64, 2) ext_rows_kernel(ExtArgs a, 
       for (int r = 0; r < 16; ++r) bad |= live && not_finite(acc[d][r]);
     const long long out = live ? (long long)((size_t(row) * size_t(a.heads) + size_t(head)) * D) : -1;
     __syncthreads();   // the last tile's buffer, and bounds
+    // a lane has a q-col's values 512 bytes or more from its neighbour's: they are turned in LDS, a wave its own 32 rows
+    auto write = [&](auto* to) {
+      using X = std::remove_pointer_t<decltype(to)>;
+      constexpr int DP = sizeof(X) == 4 && D > 128 ? 128 : D, PITCH = DP + 16 / int(sizeof(X));   // dims of a pass
+      static_assert(kExtWaves * 32 * PITCH * sizeof(X) <= R::kLds, "the tiles' buffers hold the rows");
+      X* mine = reinterpret_cast<X*>(smem) + wave * 32 * PITCH;
+#pragma unroll
+      for (int p = 0; p < D; p += DP) {
+        if (p) __syncthreads();
+#pragma unroll
+        for (int d = 0; d < R::NB; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int v = 32 * d + 8 * (r >> 2) + (r & 3);   // and 4 half
+            const int low = Tile<D, T>::dim(v >> 4, v & 15), step = Tile<D, T>::dim(0, 4) - Tile<D, T>::dim(0, 0);
+            if (low < p || low >= p + DP) continue;   // (with half = 1 on the same side)
+            mine[(lane & 31) * PITCH + low - p + half * step] = X(acc[d][r] * inv);
+          }
+        __syncthreads();
+        constexpr int CH = DP * int(sizeof(X)) / 16, PER = 64 / CH;   // 16-byte pieces of a row; rows at a time
+#pragma unroll
+        for (int c = 0; c < 32; c += PER) {
+          const int of = c + lane / CH, piece = lane % CH;
+          const int lo32 = __shfl(int(uint32_t(out)), of), hi32 = __shfl(int(out >> 32), of);
+          if (hi32 < 0) continue;
+          const size_t at = (size_t(uint32_t(hi32)) << 32 | size_t(uint32_t(lo32))) + size_t(p);
+          reinterpret_cast<uint4*>(to + at)[piece] = reinterpret_cast<const uint4*>(mine + of * PITCH)[piece];
+        }
+      }
+    };
     if (a.bf16)
-      turned_rows<D, T>(static_cast<__bf16*>(a.out), acc, inv, out, smem);
+      write(static_cast<__bf16*>(a.out));
     else
-      turned_rows<D, T>(static_cast<float*>(a.out), acc, inv, out, smem);
+      write(static_cast<float*>(a.out));
     const uint64_t any = __ballot((bad && !not_finite(l)) || (live && no_sum(l, row)));
     if (lane == 0) bounds[wave][0] = int(uint32_t(any) | uint32_t(any >> 32));
     __syncthreads();

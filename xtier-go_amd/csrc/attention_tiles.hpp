@@ -416,21 +416,22 @@ struct Rows {
   // (and room to turn the output; for heads of 256 dims, for two chunks of q)
 };
 
-// A thread's number among the 256 that share tiles.
-__device__ inline int stage_thread() { return int(threadIdx.x) & 255; }
+// A thread's number among the 256 that share tiles; GROUPS: the work-group has more than one such.
+template <bool GROUPS>
+__device__ inline int stage_thread() { return GROUPS ? int(threadIdx.x) & 255 : int(threadIdx.x); }
 
 // What a thread stages of a tile: loads in flight (raw), then entries written to LDS. A cache of an odd number of 32-slot
 // tiles ends in the middle of a 64-key tile (`half`): its other half is zeros.
-template <int D, int T>
+template <int D, int T, bool GROUPS = false>
 struct Stage;
 
 // BF16: entries as they are. Also the packed own keys.
-template <int D>
-struct Stage<D, kBf16> {
+template <int D, bool GROUPS>
+struct Stage<D, kBf16, GROUPS> {
   using R = Rows<D>;
   uint4 k[R::PER], v[R::PER];
   __device__ static void load(uint4 (&x)[R::PER], const uint4* c, int h, int pad, int tile, bool half) {
-    const size_t at = (size_t(h) * size_t(pad) + size_t(tile) * R::TK) * (D / 8) + size_t(stage_thread());
+    const size_t at = (size_t(h) * size_t(pad) + size_t(tile) * R::TK) * (D / 8) + size_t(stage_thread<GROUPS>());
 #pragma unroll
     for (int u = 0; u < R::PER; ++u) x[u] = half && 2 * u >= R::PER ? make_uint4(0, 0, 0, 0) : c[at + u * 256];
   }
@@ -438,8 +439,8 @@ struct Stage<D, kBf16> {
   __device__ void load_v(const uint4* cv, int h, int pad, int tile, bool half) { load(v, cv, h, pad, tile, half); }
   // The tile straight into its place in LDS: 64 entries a wave's load, a lane's the one that comes to its part of them.
   __device__ static void direct(const uint4* from, uint4* to, bool v) {
-    const int lane = stage_thread() & 63, half = lane >> 5, i = lane & 31;
-    const int wave = __builtin_amdgcn_readfirstlane(stage_thread() >> 6);
+    const int lane = stage_thread<GROUPS>() & 63, half = lane >> 5, i = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(stage_thread<GROUPS>() >> 6);
 #pragma unroll
     for (int u = 0; u < R::PER; ++u) {
       const int row = u * 4 + wave;   // of 64 entries
@@ -466,32 +467,32 @@ struct Stage<D, kBf16> {
   }
   __device__ void store_k(uint4* lk) const {
 #pragma unroll
-    for (int u = 0; u < R::PER; ++u) lk[k_place(stage_thread() + u * 256)] = k[u];
+    for (int u = 0; u < R::PER; ++u) lk[k_place(stage_thread<GROUPS>() + u * 256)] = k[u];
   }
   __device__ void store_v(uint4* lv) const {
 #pragma unroll
-    for (int u = 0; u < R::PER; ++u) lv[v_place(stage_thread() + u * 256)] = v[u];
+    for (int u = 0; u < R::PER; ++u) lv[v_place(stage_thread<GROUPS>() + u * 256)] = v[u];
   }
 };
 
 // FP8: a 16-byte load is two entries' codes.
-template <int D>
-struct Stage<D, kFp8> {
+template <int D, bool GROUPS>
+struct Stage<D, kFp8, GROUPS> {
   using R = Rows<D>;
-  using B = Stage<D, kBf16>;
+  using B = Stage<D, kBf16, GROUPS>;
   uint4 k[R::PER / 2], v[R::PER / 2];
   __device__ static void load(uint4 (&x)[R::PER / 2], const uint4* c, int h, int pad, int tile, bool half) {
-    const size_t at = (size_t(h) * size_t(pad) + size_t(tile) * R::TK) * (D / 16) + size_t(stage_thread());
+    const size_t at = (size_t(h) * size_t(pad) + size_t(tile) * R::TK) * (D / 16) + size_t(stage_thread<GROUPS>());
 #pragma unroll
     for (int u = 0; u < R::PER / 2; ++u) {
-      const bool past = half && stage_thread() + u * 256 >= R::kEntries / 4;
+      const bool past = half && stage_thread<GROUPS>() + u * 256 >= R::kEntries / 4;
       x[u] = past ? make_uint4(0, 0, 0, 0) : c[at + u * 256];
     }
   }
   __device__ void load_k(const uint4* ck, int h, int pad, int tile, bool half) { load(k, ck, h, pad, tile, half); }
   __device__ void load_v(const uint4* cv, int h, int pad, int tile, bool half) { load(v, cv, h, pad, tile, half); }
   __device__ static int first(int u) {   // of BF16's entries
-    const int x = stage_thread() + u * 256;
+    const int x = stage_thread<GROUPS>() + u * 256;
     return (x >> 6) * 128 + (x & 63);
   }
   __device__ void store_k(uint4* lk) const {
@@ -511,15 +512,15 @@ struct Stage<D, kFp8> {
 };
 
 // NVFP4: a thread's codes are PER entries of K, which share a key, and PER of V, which share their keys' scales.
-template <int D>
-struct Stage<D, kNvfp4> {
+template <int D, bool GROUPS>
+struct Stage<D, kNvfp4, GROUPS> {
   using R = Rows<D>;
   uint32_t k[R::PER], v[R::PER], ks;
   uint2 vs;
   template <class A>
   __device__ void load_k(const A& a, int h, int tile, bool half) {
     const size_t at = size_t(h) * size_t(a.slots_pad) + size_t(tile) * R::TK;
-    const int tid = stage_thread();
+    const int tid = stage_thread<GROUPS>();
 #pragma unroll
     for (int u = 0; u < R::PER; ++u) k[u] = 0;
     ks = 0;
@@ -532,7 +533,7 @@ struct Stage<D, kNvfp4> {
   template <class A>
   __device__ void load_v(const A& a, int h, int tile, bool half) {
     const size_t at = size_t(h) * size_t(a.slots_pad) + size_t(tile) * R::TK;
-    const int tid = stage_thread(), lane = tid & 63, part = tid >> 6, t = D == 256 ? 0 : part >> 1;
+    const int tid = stage_thread<GROUPS>(), lane = tid & 63, part = tid >> 6, t = D == 256 ? 0 : part >> 1;
 #pragma unroll
     for (int u = 0; u < R::PER; ++u) v[u] = 0;
     vs = make_uint2(0, 0);
@@ -561,7 +562,7 @@ struct Stage<D, kNvfp4> {
     }
   }
   __device__ void store_k(uint4* lk) const {
-    const int tid = stage_thread(), lane = tid & 63, part = tid >> 6, g = lane >> 4, i = lane & 15;
+    const int tid = stage_thread<GROUPS>(), lane = tid & 63, part = tid >> 6, g = lane >> 4, i = lane & 15;
     // D = 64, 128: 16-slot block `part`; 256: block part / 2, chunk part % 2
     const int b = D == 256 ? part >> 1 : part, chunk = D == 256 ? part & 1 : 0;
 #pragma unroll
@@ -572,7 +573,7 @@ struct Stage<D, kNvfp4> {
     }
   }
   __device__ void store_v(uint4* lv) const {
-    const int tid = stage_thread(), lane = tid & 63, part = tid >> 6, g = lane >> 4, i = lane & 15;
+    const int tid = stage_thread<GROUPS>(), lane = tid & 63, part = tid >> 6, g = lane >> 4, i = lane & 15;
     f16x2 s[4];
     v_scales(vs, s);
     const int t = D == 256 ? 0 : part >> 1, dd0 = (D == 256 ? part : part & 1) * R::PER;
@@ -584,39 +585,5 @@ struct Stage<D, kNvfp4> {
     }
   }
 };
-
-// The accumulators of 128 q-cols, 32 a wave, times inv as rows of `to`, a lane's at `out` (-1: not written). A lane has a
-// q-col's values 512 bytes or more from its neighbour's: they are turned in LDS, a wave its own 32 rows.
-template <int D, int T, class X>
-__device__ inline void turned_rows(X* to, const f32x16 (&acc)[Rows<D>::NB], float inv, long long out, uint8_t* smem) {
-  using R = Rows<D>;
-  constexpr int DP = sizeof(X) == 4 && D > 128 ? 128 : D, PITCH = DP + 16 / int(sizeof(X));   // dims of a pass
-  static_assert(4 * 32 * PITCH * sizeof(X) <= R::kLds, "the tiles' buffers hold the rows");
-  const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) >> 6, half = lane >> 5;
-  X* mine = reinterpret_cast<X*>(smem) + wave * 32 * PITCH;
-#pragma unroll
-  for (int p = 0; p < D; p += DP) {
-    if (p) __syncthreads();
-#pragma unroll
-    for (int d = 0; d < R::NB; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int v = 32 * d + 8 * (r >> 2) + (r & 3);   // and 4 half
-        const int low = Tile<D, T>::dim(v >> 4, v & 15), step = Tile<D, T>::dim(0, 4) - Tile<D, T>::dim(0, 0);
-        if (low < p || low >= p + DP) continue;   // (with half = 1 on the same side)
-        mine[(lane & 31) * PITCH + low - p + half * step] = X(acc[d][r] * inv);
-      }
-    __syncthreads();
-    constexpr int CH = DP * int(sizeof(X)) / 16, PER = 64 / CH;   // 16-byte pieces of a row; rows at a time
-#pragma unroll
-    for (int c = 0; c < 32; c += PER) {
-      const int of = c + lane / CH, piece = lane % CH;
-      const int lo32 = __shfl(int(uint32_t(out)), of), hi32 = __shfl(int(out >> 32), of);
-      if (hi32 < 0) continue;
-      const size_t at = (size_t(uint32_t(hi32)) << 32 | size_t(uint32_t(lo32))) + size_t(p);
-      reinterpret_cast<uint4*>(to + at)[piece] = reinterpret_cast<const uint4*>(mine + of * PITCH)[piece];
-    }
-  }
-}
 
 }  // namespace xtg::hip

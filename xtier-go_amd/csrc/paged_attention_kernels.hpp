@@ -464,9 +464,9 @@ __device__ inline void few_piece(const PagedArgs& a, const Piece& p, int h, uint
 // (heads of 256 dims: a tile is 32 slots, at0). first: of the tile's first position; lo, hi: values of other positions
 // are taken as zeros.
 template <int D, int T>
-struct PagedStage : Stage<D, T> {
+struct PagedStage : Stage<D, T, true> {
   using R = Rows<D>;
-  using S = Stage<D, T>;
+  using S = Stage<D, T, true>;
   __device__ static uint32_t valid_of(int base, int lo, int hi) {   // of keys base + e, base + 16 + e (e = 0 .. 3)
     uint32_t m = 0;
 #pragma unroll
@@ -488,7 +488,7 @@ struct PagedStage : Stage<D, T> {
   // 16-byte pieces tid, tid + 256, .. of the tile's N, half of them at each place
   template <int N>
   __device__ static void load(uint4 (&x)[N / 256], const uint4* c, size_t at0, size_t at1) {
-    const int tid = stage_thread();
+    const int tid = stage_thread<true>();
 #pragma unroll
     for (int u = 0; u < N / 256; ++u) {
       if constexpr (D == 256) {
@@ -502,7 +502,7 @@ struct PagedStage : Stage<D, T> {
     }
   }
   __device__ void load_k(const PagedArgs& a, size_t at0, size_t at1) {
-    const int tid = stage_thread();
+    const int tid = stage_thread<true>();
     if constexpr (T == kFp8) {
       load<R::kEntries / 2>(this->k, reinterpret_cast<const uint4*>(a.ck), at0, at1);
     } else {
@@ -513,7 +513,7 @@ struct PagedStage : Stage<D, T> {
     }
   }
   __device__ void load_v(const PagedArgs& a, size_t at0, size_t at1) {
-    const int tid = stage_thread(), lane = tid & 63, part = tid >> 6;
+    const int tid = stage_thread<true>(), lane = tid & 63, part = tid >> 6;
     if constexpr (T == kFp8) {
       load<R::kEntries / 2>(this->v, reinterpret_cast<const uint4*>(a.cv), at0, at1);
     } else {
@@ -538,7 +538,7 @@ struct PagedStage : Stage<D, T> {
   // BF16 tiles straight into LDS: 64 entries a wave's load, a lane's the one that comes to its part of them; and the mask of
   // what a lane loaded, once it is there
   __device__ static void direct(const uint4* c, size_t at0, size_t at1, uint4* to, bool v) {
-    const int tid = stage_thread(), half = tid >> 5 & 1, i = tid & 31;
+    const int tid = stage_thread<true>(), half = tid >> 5 & 1, i = tid & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 #pragma unroll
     for (int u = 0; u < R::PER; ++u) {
@@ -557,7 +557,7 @@ struct PagedStage : Stage<D, T> {
     }
   }
   __device__ static void mask_direct(uint4* lv, int first, int lo, int hi) {
-    const int lane = int(threadIdx.x) & 63, wave = stage_thread() >> 6;
+    const int lane = int(threadIdx.x) & 63, wave = stage_thread<true>() >> 6;
 #pragma unroll
     for (int u = 0; u < R::PER; ++u) {
       const int row = u * 4 + wave, ks = row % R::KS;
@@ -582,11 +582,45 @@ constexpr size_t many_lds() {
   return tiles > states ? (tiles > turned ? tiles : turned) : states > turned ? states : turned;
 }
 
+// The accumulators of 128 q-cols, 32 a wave, times inv as rows of `to`, a lane's at `out` (-1: not written). A lane has a
+// q-col's values 512 bytes or more from its neighbour's: they are turned in LDS, a wave its own 32 rows.
+template <int D, int T, class X>
+__device__ inline void turned_rows(X* to, const f32x16 (&acc)[Rows<D>::NB], float inv, long long out, uint8_t* smem) {
+  using R = Rows<D>;
+  constexpr int DP = sizeof(X) == 4 && D > 128 ? 128 : D, PITCH = DP + 16 / int(sizeof(X));   // dims of a pass
+  static_assert(4 * 32 * PITCH * sizeof(X) <= R::kLds, "the tiles' buffers hold the rows");
+  const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) >> 6, half = lane >> 5;
+  X* mine = reinterpret_cast<X*>(smem) + wave * 32 * PITCH;
+#pragma unroll
+  for (int p = 0; p < D; p += DP) {
+    if (p) __syncthreads();
+#pragma unroll
+    for (int d = 0; d < R::NB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int v = 32 * d + 8 * (r >> 2) + (r & 3);   // and 4 half
+        const int low = Tile<D, T>::dim(v >> 4, v & 15), step = Tile<D, T>::dim(0, 4) - Tile<D, T>::dim(0, 0);
+        if (low < p || low >= p + DP) continue;   // (with half = 1 on the same side)
+        mine[(lane & 31) * PITCH + low - p + half * step] = X(acc[d][r] * inv);
+      }
+    __syncthreads();
+    constexpr int CH = DP * int(sizeof(X)) / 16, PER = 64 / CH;   // 16-byte pieces of a row; rows at a time
+#pragma unroll
+    for (int c = 0; c < 32; c += PER) {
+      const int of = c + lane / CH, piece = lane % CH;
+      const int lo32 = __shfl(int(uint32_t(out)), of), hi32 = __shfl(int(out >> 32), of);
+      if (hi32 < 0) continue;
+      const size_t at = (size_t(uint32_t(hi32)) << 32 | size_t(uint32_t(lo32))) + size_t(p);
+      reinterpret_cast<uint4*>(to + at)[piece] = reinterpret_cast<const uint4*>(mine + of * PITCH)[piece];
+    }
+  }
+}
+
 template <int D, int T, int MOD>
 __device__ inline void many_piece(const PagedArgs& a, const Piece& p, int h, uint8_t* smem, int (&bad_cols)[8]) {
   using R = Rows<D>;
   using X8 = typename OperandOf<T>::type;
-  const int tid = stage_thread(), lane = tid & 63, half = lane >> 5;
+  const int tid = stage_thread<true>(), lane = tid & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), group = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 8);
   const bool out_of = p.q.pos < 0;
   // rows of the block and of the wave, and positions that some row of the block sees
