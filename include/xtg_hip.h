@@ -257,7 +257,7 @@ int xtg_hip_paged_globals(xtg_hip* h, xtg_hip_paged* c, float k_global, float v_
  * is sequence s's (n_rows == n_seqs: a decode step). pos[s] < 0 leaves sequence s out. Position p of sequence s is in page
  * pages[s * max_pages + p / page_size]; a number that is no page of the pool, or a position behind the table's, is no page.
  * The arrays are device memory, read by the kernels as they run: a captured graph follows what is in them at its replay.
- * starts must not decrease. max_pages * page_size is 2^30 at most. */
+ * starts must not decrease. max_pages * page_size is 2^30 at most; n_rows is below 2^24, n_seqs below 2^20. */
 typedef struct xtg_paged_rows {
   int n_seqs, n_rows;
   const int32_t* pos;      /* [n_seqs] */
@@ -296,7 +296,7 @@ int xtg_hip_paged_read(xtg_hip* h, const xtg_hip_paged* c, const xtg_paged_rows*
  * then softcap * tanh(s / softcap) where softcap > 0. Rows of a sequence that is left out get zeros; a row that sees a
  * position without a page, or whose scores are all minus infinity, NaN. What is in a page beside the positions that a row
  * sees, NaN too, is nothing to it. Rows are x_dtype (FP32 q is rounded to BF16, out is not); precision as xtg_hip_attention_ext. Up to
- * 128 q heads per KV head; n_rows * heads up to 2^30; out, packed, overlaps no input. Queued; the first call of so many rows, sequences and
+ * 128 q heads per KV head; n_rows * heads up to 2^27; out, packed, overlaps no input. Queued; the first call of so many rows, sequences and
  * heads sizes scratch memory, whatever the sequences' lengths (make it before a graph capture). */
 typedef struct xtg_paged_attn {
   int heads;

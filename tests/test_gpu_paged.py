@@ -375,8 +375,8 @@ def test_one_token_each(hip, d, dtype, kw):
 def test_rows_of_any_number(hip, d, dtype, kw):
     """Decoded tokens, verify steps, turns and prompts in one call; sequences without rows and left-out ones."""
     rng = np.random.default_rng(d + 1)
-    n = [1, 8, 0, 37, 1, 130, 3, 1]
-    pos = [200, 0, 50, 33, 0, 70, -1, 511]
+    n = [1, 8, 0, 37, 1, 130, 3, 1, 90]
+    pos = [200, 0, 50, 33, 0, 70, -1, 511, -7]
     p = Pool(hip, rng, dtype, HEADS[d][1], d, [max(0, a) + m for a, m in zip(pos, n)], page=32)
     p.fill()
     p.check(pos, n, HEADS[d][0], **kw)
@@ -404,6 +404,65 @@ def test_head_groups(hip, heads, kvh):
     p.fill()
     p.check([499, 69, 8], [1, 1, 1], heads, rows=p.rows([499, 69, 8], [1, 1, 1], one_each=True))
     p.check([480, 0, 1], [19, 70, 8], heads)
+    p.free()
+
+
+@pytest.mark.parametrize("d,page", [(64, 32), (64, 64), (128, 32), (128, 4096), (256, 32), (256, 512)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_prompts_over_pages_of_any_size(hip, d, page, dtype):
+    """Blocks of 128 q-cols whose tiles of 64 keys are one page's or two's, from the first position on and after some; FP32
+    rows too, whose output is turned in two passes."""
+    rng = np.random.default_rng(d + page)
+    n, pos = [260, 33, 1], [0, 95, 40]
+    p = Pool(hip, rng, dtype, HEADS[d][1], d, [a + m for a, m in zip(pos, n)], page=page)
+    p.fill()
+    p.check(pos, n, HEADS[d][0])
+    p.check(pos, n, HEADS[d][0], x_dtype=o.F32, window=70)
+    p.free()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_prompt_chunk_over_a_long_context(hip, dtype, d):
+    """Blocks of many q-cols whose keys are split over work-groups, and joined."""
+    rng = np.random.default_rng(d + 3)
+    heads, kvh = {64: 8, 128: 8, 256: 4}[d], 1
+    p = Pool(hip, rng, dtype, kvh, d, [5000, 600], page=64)
+    p.fill()
+    p.check([4980, 599], [20, 1], heads)
+    p.check([4980, 560], [20, 40], heads, softcap=15.0, spread=3.0)
+    p.free()
+
+
+def test_prompt_blocks_with_rows_that_end_in_different_tiles(hip):
+    """A group of one q head: a block of 128 q-cols is 128 rows, over four tiles' diagonals."""
+    rng = np.random.default_rng(19)
+    p = Pool(hip, rng, "bf16", 2, 64, [700, 300])
+    p.fill()
+    p.check([300, 0], [400, 300], 2)
+    p.check([300, 0], [400, 300], 2, window=33)
+    p.free()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [1e4, 1e8, 1e10])
+@pytest.mark.parametrize("n", [1, 40])
+def test_scores_beyond_the_integers_of_fp32(hip, dtype, scale, n):
+    """Scores so large that one key takes all the weight: its value comes back. Keys whose scores are further from the best
+    than its rounding (2^-24 of it and more) count for nothing."""
+    rng = np.random.default_rng(int(scale) % 1000 + n)
+    p = Pool(hip, rng, dtype, 2, 64, [200 + n])
+    p.fill()
+    q = unit(rng, (n, 8, 64)) * np.float32(64)
+    got, want, _ = p.attend([200], [n], 8, q=q, scale=scale, x_dtype=o.F32)
+    k, v = p.held(0, 200 + n)
+    for i in range(n):
+        for h in range(8):
+            s = k[:201 + i, h // 4] @ o.bf16(q[i, h]).astype(np.float64)
+            top = np.sort(s)[-2:]
+            if (top[1] - top[0]) * scale > 200 + abs(top[1]) * scale * 2.0 ** -18:
+                assert np.abs(got[i, h] - v[s.argmax(), h // 4]).max() <= np.abs(v[s.argmax(), h // 4]).max() * 2.0 ** -8
+    assert np.isfinite(got).all()
     p.free()
 
 
@@ -728,6 +787,15 @@ def test_refusals(hip, pkg):
     big = hip.paged_cache(1, 64, 1, 4096)
     with pytest.raises(pkg.XtgError, match="2\\^30 positions"):
         big.read(hip.paged_rows(pos, wide), k, k)
+    # a pool that does not fit leaves no error behind for the next call
+    with pytest.raises(pkg.XtgError, match="hipMalloc"):
+        hip.paged_cache(8, 256, 200000, 4096)
+    hip.add_norm(k, None, k, 1, 64)
+    gone = hip.array(np.zeros(2, np.int32))
+    late = hip.paged_rows(gone, table, 2)
+    gone.free()
+    with pytest.raises(pkg.XtgError, match="have been freed"):
+        c.read(late, k, k)
     # nothing to do is done
     none = hip.paged_rows(pos, table, 0, hip.array(np.zeros(3, np.int32)))
     c.append(none, k, k)

@@ -778,7 +778,15 @@ class PagedRows:
         self.args = PagedRowsArgs(n_seqs, n_rows, _device_ptr(backend, "pos", pos, n_seqs, _I32),
                                   _device_ptr(backend, "starts", starts, n_seqs + 1, _I32),
                                   _device_ptr(backend, "pages", pages, n_seqs * max_pages, _I32), max_pages)
-        self.ref = ctypes.byref(self.args)
+        self._ref = ctypes.byref(self.args)
+        self._own = [a for a in self.arrays if isinstance(a, DeviceArray)]   # whose memory can be freed while they are held
+
+    @property
+    def ref(self):
+        for a in self._own:
+            if not a.ptr:
+                raise XtgError("the positions, pages or starts of the rows have been freed")
+        return self._ref
 
 
 class PagedCache:

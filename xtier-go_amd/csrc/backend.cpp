@@ -824,6 +824,7 @@ DevPaged* Backend::paged_create(int kv_heads, int head_dim, long long pages, int
     (void)hipStreamSynchronize(stream_);
     for (void* p : {c->k, c->v, c->ks, c->vs})
       if (p) (void)hipFree(p);
+    (void)hipGetLastError();   // (no memory, say: not the next launch's error)
     throw;
   }
   return c.release();
@@ -850,7 +851,7 @@ void Backend::paged_globals(DevPaged* c, float kglobal, float vglobal) {
 // The checks that the three calls share.
 Seqs Backend::paged_rows(const char* what, const DevPaged* c, const xtg_paged_rows& r) const {
   XTG_CHECK(paged_.count(const_cast<DevPaged*>(c)), "%s: unknown cache", what);
-  XTG_CHECK(r.n_seqs >= 0 && r.n_rows >= 0 && r.n_rows < (1 << 30) && r.n_seqs < (1 << 24), "%s: %d rows of %d sequences", what,
+  XTG_CHECK(r.n_seqs >= 0 && r.n_rows >= 0 && r.n_rows < (1 << 24) && r.n_seqs < (1 << 20), "%s: %d rows of %d sequences (below 2^24 and 2^20)", what,
             r.n_rows, r.n_seqs);
   XTG_CHECK(r.starts || r.n_rows == r.n_seqs, "%s: %d rows of %d sequences without starts", what, r.n_rows, r.n_seqs);
   XTG_CHECK(r.max_pages >= 1 && (long long)r.max_pages * c->size <= (1 << 30), "%s: %d pages of %d positions a sequence (2^30 positions at most)",
@@ -909,7 +910,7 @@ void Backend::paged_attention(const DevPaged* c, const xtg_paged_rows& rows, con
   XTG_CHECK(a.x_dtype == kXF32 || a.x_dtype == kXBF16, "paged_attention: unknown row type %d", a.x_dtype);
   XTG_CHECK(a.heads >= 1 && a.heads % c->kv_heads == 0 && a.heads / c->kv_heads <= 128,
             "paged_attention: %d heads over %d KV heads (up to 128 for each)", a.heads, c->kv_heads);
-  XTG_CHECK((long long)rows.n_rows * a.heads <= (1LL << 30), "paged_attention: %d rows of %d heads (2^30 at most)", rows.n_rows, a.heads);
+  XTG_CHECK((long long)rows.n_rows * a.heads <= (1LL << 27), "paged_attention: %d rows of %d heads (2^27 at most)", rows.n_rows, a.heads);
   XTG_CHECK(std::isfinite(a.scale), "paged_attention: scale %g", double(a.scale));
   XTG_CHECK(a.softcap >= 0.f && a.softcap <= 1024.f, "paged_attention: softcap %g (0 to 1024)", double(a.softcap));
   if (rows.n_rows == 0 || rows.n_seqs == 0) return;

@@ -163,7 +163,8 @@ __host__ __device__ inline int parts_of(const Extent& x, int chunk) {
 // One long sequence takes half as many work-groups, one a CU: more than 32 records of a q-col cost the merge more than the
 // second one a CU brings (one token over 32768 BF16 positions of 8 KV heads of 128 dims: 32.2 -> 30.0 us).
 __host__ __device__ inline int first_chunk(const PagedArgs& a, float total, int blocks) {
-  const int chunk = int(total / float(blocks * 32LL < a.budget ? (a.budget + 1) / 2 : a.budget)) + 1;
+  const float share = total / float(blocks * 32LL < a.budget ? (a.budget + 1) / 2 : a.budget);
+  const int chunk = share < 1e9f ? int(share) + 1 : 1000000000;
   return chunk < kFewLeast ? kFewLeast : chunk;
 }
 __host__ __device__ inline bool next_chunk(const PagedArgs& a, int& chunk, int tasks, int blocks) {
@@ -175,8 +176,11 @@ constexpr int kChunkSteps = 3;
 
 // A launch whose error is its own return value: asking for the last error after one takes the host another 0.9 us, a quarter
 // of what the launch does.
+// The grid's threads are a 32-bit number.
 template <class... A>
 void paged_queue(void (*kernel)(A...), dim3 grid, unsigned threads, size_t lds, hipStream_t stream, A... args) {
+  XTG_CHECK((unsigned long long)grid.x * threads < (1ULL << 32), "a launch of %u work-groups of %u threads: a call of so many rows and sequences",
+            grid.x, threads);
   void* list[] = {&args...};
   HIP_CHECK(hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, dim3(threads), list, lds, stream));
 }

@@ -506,10 +506,11 @@ struct PagedStage : Stage<D, T, true> {
     if constexpr (T == kFp8) {
       load<R::kEntries / 2>(this->k, reinterpret_cast<const uint4*>(a.ck), at0, at1);
     } else {
-      const size_t at = D == 256 || tid < 128 ? at0 : at1 - 32;   // (in whole tiles' numbering: the second half's own place)
-      this->take(this->k, a.ck + at * (D / 2), tid);
+      const size_t at = D == 256 || tid < 128 ? at0 : at1;
+      const int mine = D == 256 ? tid : tid & 127;   // of the half's threads
+      this->take(this->k, a.ck + at * (D / 2), mine);
       const uint8_t* s = static_cast<const uint8_t*>(a.ks) + at * (D / 16);
-      this->ks = D == 64 ? s[tid] : reinterpret_cast<const uint16_t*>(s)[tid];
+      this->ks = D == 64 ? s[mine] : reinterpret_cast<const uint16_t*>(s)[mine];
     }
   }
   __device__ void load_v(const PagedArgs& a, size_t at0, size_t at1) {
@@ -517,11 +518,10 @@ struct PagedStage : Stage<D, T, true> {
     if constexpr (T == kFp8) {
       load<R::kEntries / 2>(this->v, reinterpret_cast<const uint4*>(a.cv), at0, at1);
     } else {
-      const size_t at = D == 256 || tid < 128 ? at0 : at1 - 32;
-      this->take_v(a.cv + at * (D / 2), part, lane);
-      const int t = D == 256 ? 0 : part >> 1;
+      const size_t at = D == 256 || tid < 128 ? at0 : at1;
+      this->take_v(a.cv + at * (D / 2), D == 256 ? part : part & 1, lane);
       const uint2* sv = reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.vs) + at * (D / 16));
-      this->vs = sv[t * (D / 4) + (lane >> 4) * (D / 16) + (lane & 15) * (D / 16) / 16];
+      this->vs = sv[(lane >> 4) * (D / 16) + (lane & 15) * (D / 16) / 16];
     }
   }
   __device__ void mask_v(int first, int lo, int hi) {
