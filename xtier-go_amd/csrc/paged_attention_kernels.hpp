@@ -136,6 +136,28 @@ __device__ inline Score paged_score(const PagedArgs& a, float global, int ex) {
   return s;
 }
 
+// Values 4 u .. +4 of a record's order into an output row: neighbours but for NVFP4's order.
+template <int D, int T, class X>
+__device__ inline void put4(X* row, int u, const float (&y)[4]) {
+  const int dim = Tile<D, T>::dim(u >> 2, 4 * (u & 3));
+  if constexpr (T == kNvfp4) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) row[Tile<D, T>::dim(u >> 2, 4 * (u & 3) + r)] = X(y[r]);
+  } else if constexpr (sizeof(X) == 2) {
+    const X z[4] = {X(y[0]), X(y[1]), X(y[2]), X(y[3])};
+    *reinterpret_cast<uint2*>(row + dim) = __builtin_bit_cast(uint2, z);
+  } else {
+    *reinterpret_cast<float4*>(row + dim) = make_float4(y[0], y[1], y[2], y[3]);
+  }
+}
+template <int D, int T>
+__device__ inline void put4(const PagedArgs& a, size_t at, int u, const float (&y)[4]) {
+  if (a.bf16)
+    put4<D, T>(static_cast<__bf16*>(a.out) + at, u, y);
+  else
+    put4<D, T>(static_cast<float*>(a.out) + at, u, y);
+}
+
 // ------------------------------------------------------------------------------------------- a q-col key by key
 
 template <int D, int T>
@@ -424,15 +446,8 @@ __device__ inline void few_piece(const PagedArgs& a, const Piece& p, int h, uint
       for (int r = 0; r < 4; ++r) bad |= p.q.n > 1 && !not_finite(l) && not_finite(y[r]);
       if (bad) atomicOr(&again, 1u << mine);
       const float inv = l == 0.f ? (out_of ? 0.f : NAN) : 1.f / l;   // (scores of minus infinity alone: NaN)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int dim = Tile<D, T>::dim(dd, 4 * g + r);
-        const size_t to = (size_t(p.q.row0 + row) * size_t(a.heads) + size_t(col_head(mine))) * D + size_t(dim);
-        if (a.bf16)
-          static_cast<__bf16*>(a.out)[to] = (__bf16)(y[r] * inv);
-        else
-          static_cast<float*>(a.out)[to] = y[r] * inv;
-      }
+      put4<D, T>(a, (size_t(p.q.row0 + row) * size_t(a.heads) + size_t(col_head(mine))) * D, 4 * dd + g,
+                 {y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv});
     } else {
       *reinterpret_cast<f32x4*>(a.acc + (rec + size_t(mine)) * D + size_t(16 * dd + 4 * g)) = y;
     }
@@ -578,32 +593,45 @@ template <int D>
 constexpr size_t kGroupLds = size_t(Rows<D>::kEntries) * 64 + size_t(Rows<D>::TK) * 16;
 template <int D, int T>
 constexpr size_t many_lds() {
-  const size_t tiles = 2 * kGroupLds<D> + 4096 * kQChunks<D, T>, states = size_t(D) * 512 + 1024, turned = 8 * 32 * (D > 128 ? 528 : D * 4 + 16);
+  const size_t tiles = 2 * kGroupLds<D> + 4096 * kQChunks<D, T>, states = size_t(D) * 512 + 1024, turned = 4 * 32 * (D > 128 ? 528 : D * 4 + 16);
   return tiles > states ? (tiles > turned ? tiles : turned) : states > turned ? states : turned;
 }
 
-// The accumulators of 128 q-cols, 32 a wave, times inv as rows of `to`, a lane's at `out` (-1: not written). A lane has a
-// q-col's values 512 bytes or more from its neighbour's: they are turned in LDS, a wave its own 32 rows.
+// The accumulators of the first four waves' 128 q-cols, 32 a wave, times inv as rows of `to`, a lane's at `out` (-1: not
+// written). A lane has a q-col's values 512 bytes or more from its neighbour's: they are turned in LDS, a wave its own 32
+// rows, four values at a time (one at a time, and by all eight waves, took 9 us of a block of 256 dims, the others' 1.4).
 template <int D, int T, class X>
 __device__ inline void turned_rows(X* to, const f32x16 (&acc)[Rows<D>::NB], float inv, long long out, uint8_t* smem) {
   using R = Rows<D>;
   constexpr int DP = sizeof(X) == 4 && D > 128 ? 128 : D, PITCH = DP + 16 / int(sizeof(X));   // dims of a pass
-  static_assert(4 * 32 * PITCH * sizeof(X) <= R::kLds, "the tiles' buffers hold the rows");
   const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) >> 6, half = lane >> 5;
-  X* mine = reinterpret_cast<X*>(smem) + wave * 32 * PITCH;
+  const bool lead = wave < 4;
+  X* mine = reinterpret_cast<X*>(smem) + (wave & 3) * 32 * PITCH;
 #pragma unroll
   for (int p = 0; p < D; p += DP) {
     if (p) __syncthreads();
+    if (lead) {
 #pragma unroll
-    for (int d = 0; d < R::NB; ++d)
+      for (int d = 0; d < R::NB; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int v = 32 * d + 8 * (r >> 2) + (r & 3);   // and 4 half
-        const int low = Tile<D, T>::dim(v >> 4, v & 15), step = Tile<D, T>::dim(0, 4) - Tile<D, T>::dim(0, 0);
-        if (low < p || low >= p + DP) continue;   // (with half = 1 on the same side)
-        mine[(lane & 31) * PITCH + low - p + half * step] = X(acc[d][r] * inv);
-      }
+        for (int j = 0; j < 4; ++j) {
+          const int v = 32 * d + 8 * j;   // and 4 half
+          const int low = Tile<D, T>::dim(v >> 4, v & 15), step = Tile<D, T>::dim(0, 4) - Tile<D, T>::dim(0, 0);
+          const int last = Tile<D, T>::dim(v >> 4, (v & 15) + 3);
+          if (T != kNvfp4 && (low < p || low >= p + DP)) continue;   // (with half = 1 on the same side)
+          if (T == kNvfp4 && (last < p || low >= p + DP)) continue;
+          X* row = mine + (lane & 31) * PITCH - p + half * step;
+          const float y[4] = {acc[d][4 * j] * inv, acc[d][4 * j + 1] * inv, acc[d][4 * j + 2] * inv, acc[d][4 * j + 3] * inv};
+          if constexpr (T == kNvfp4) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) row[Tile<D, T>::dim(v >> 4, (v & 15) + r)] = X(y[r]);
+          } else {
+            put4<D, T>(row, v / 4, y);
+          }
+        }
+    }
     __syncthreads();
+    if (!lead) continue;
     constexpr int CH = DP * int(sizeof(X)) / 16, PER = 64 / CH;   // 16-byte pieces of a row; rows at a time
 #pragma unroll
     for (int c = 0; c < 32; c += PER) {
@@ -890,14 +918,13 @@ __device__ inline void many_piece(const PagedArgs& a, const Piece& p, int h, uin
 #pragma unroll
     for (int r = 0; r < 16; ++r) bad |= mine && not_finite(acc[d][r]);
   const long long out = mine ? (long long)((size_t(p.q.row0 + row) * size_t(a.heads) + size_t(head)) * D) : -1;
+  const uint64_t again = __ballot(bad && !not_finite(l));
+  if (lane == 0 && !group) bad_cols[wave] = int(uint32_t(again) | uint32_t(again >> 32));
   __syncthreads();   // the states' place
   if (a.bf16)
     turned_rows<D, T>(static_cast<__bf16*>(a.out), acc, inv, out, smem);
   else
     turned_rows<D, T>(static_cast<float*>(a.out), acc, inv, out, smem);
-  const uint64_t again = __ballot(bad && !not_finite(l));
-  if (lane == 0 && !group) bad_cols[wave] = int(uint32_t(again) | uint32_t(again >> 32));
-  __syncthreads();
   for (int w = 0; w < 4; ++w)
     for (uint32_t bits = uint32_t(bad_cols[w]); bits; bits &= bits - 1) {
       const long long c = c0 + w * 32 + __builtin_ctz(bits);
@@ -1019,16 +1046,7 @@ __device__ inline bool merge_col(const PagedArgs& a, int id, int4 info, float4* 
   }
   if (grp != 0) return false;
   const float inv = l == 0.f ? NAN : 1.f / l;
-  const float o[4] = {y.x * inv, y.y * inv, y.z * inv, y.w * inv};
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int u = 4 * x + r;
-    const size_t at = size_t(id) * D + size_t(Tile<D, T>::dim(u >> 4, u & 15));
-    if (a.bf16)
-      static_cast<__bf16*>(a.out)[at] = (__bf16)o[r];
-    else
-      static_cast<float*>(a.out)[at] = o[r];
-  }
+  put4<D, T>(a, size_t(id) * D, x, {y.x * inv, y.y * inv, y.z * inv, y.w * inv});
   return rows > 1 && !not_finite(l) && (not_finite(y.x) || not_finite(y.y) || not_finite(y.z) || not_finite(y.w));
 }
 
