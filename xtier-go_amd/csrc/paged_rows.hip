@@ -467,75 +467,98 @@ struct PagedReadArgs {
   float kglobal, vglobal;
 };
 
-// Dealt as the append is: 8 + 8 dims of a key of K, P dims of 8 slots of V a thread.
+// 8 E2M1 codes' values times a scale.
+__device__ inline void fp4_values(uint32_t w, float s, float (&x)[8]) {
+  const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 1);
+  const auto c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 3);
+  x[0] = a[0] * s, x[1] = a[1] * s, x[2] = b[0] * s, x[3] = b[1] * s;
+  x[4] = c[0] * s, x[5] = c[1] * s, x[6] = d[0] * s, x[7] = d[1] * s;
+}
+
+// Dealt as the append is: 8 + 8 dims of a key of K, P dims of 8 slots of V a thread. Every load goes out before the first
+// store, whichever rows are the call's: the whole tile is there (32749 rows of 8 heads of 128 dims into BF16: NVFP4 44 us,
+// FP8 45, BF16 56; with the loads behind each row's branch 47, 51 and 57).
 template <int D, int T, class X>
 __global__ void __launch_bounds__(256) paged_read_kernel(PagedReadArgs a) {
-  constexpr int C = D / 16, KP = 256 / C < 32 ? 256 / C : 32, P = D / 64;
+  constexpr int C = D / 16, KP = 256 / C < 32 ? 256 / C : 32, U = 32 / KP, P = D / 64;
+  using Raw = std::conditional_t<T == kBf16, uint4, std::conditional_t<T == kFp8, uint2, uint32_t>>;   // 8 values
   TileTask t;
   if (!tile_task(a.s, a.kv_heads, int(blockIdx.x), t)) return;
   const int tid = int(threadIdx.x), size = 1 << a.s.shift;
   const bool held = t.page >= 0;
   const int hh = (held ? t.page : 0) * a.kv_heads + t.head;
-  const int c = tid % C, key0 = tid / C, v_dim = (tid & 63) * P, g = tid >> 6;
-  auto dst = [&](void* rows, int r) {
-    return static_cast<X*>(rows) + (size_t(r) * size_t(a.kv_heads) + size_t(t.head)) * D;
-  };
+  const int c = tid % C, key0 = tid / C, v_dim = (tid & 63) * P, g = tid >> 6, slot0 = t.slot + 4 * g;
+  Raw k[U][2], v[P];
+  float ks[U][2], vs[8];
 #pragma unroll
-  for (int u = 0; u < 32 / KP; ++u) {
-    const int key = u * KP + key0, slot = t.slot + (key & 31), r = key < 32 ? t.row(key) : -1;
-    if (r < 0) continue;
-    auto take = [&](int dim) {
-      float x[8] = {};
-      if (held) {
-        if constexpr (T == kBf16) {
-          load_row4(reinterpret_cast<const __bf16*>(a.ck) + kv_k_index(hh, slot, dim, size, D), x);
-        } else if constexpr (T == kFp8) {
-          fp8_values(*reinterpret_cast<const uint2*>(a.ck + kv_k8_index(hh, slot, dim, size, D)),
-                     reinterpret_cast<const float*>(a.ks)[size_t(hh) * size_t(size) + size_t(slot)], x);
-        } else {
-          const uint32_t w = *reinterpret_cast<const uint32_t*>(a.ck + k4_code(hh, slot, dim, size, D).byte);
-          const float s = __builtin_amdgcn_cvt_f32_fp8(int(a.ks[k4_scale(hh, slot, dim, size, D)]), 0) * a.kglobal;
-          const auto y0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 0), y1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 1);
-          const auto y2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 2), y3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 3);
-          x[0] = y0[0] * s, x[1] = y0[1] * s, x[2] = y1[0] * s, x[3] = y1[1] * s;
-          x[4] = y2[0] * s, x[5] = y2[1] * s, x[6] = y3[0] * s, x[7] = y3[1] * s;
-        }
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int slot = t.slot + ((u * KP + key0) & 31), dim = x * (D / 2) + 8 * c;
+      ks[u][x] = 1.f;
+      if constexpr (T == kBf16) {
+        k[u][x] = *reinterpret_cast<const Raw*>(reinterpret_cast<const __bf16*>(a.ck) + kv_k_index(hh, slot, dim, size, D));
+      } else if constexpr (T == kFp8) {
+        k[u][x] = *reinterpret_cast<const Raw*>(a.ck + kv_k8_index(hh, slot, dim, size, D));
+        ks[u][x] = x ? ks[u][0] : reinterpret_cast<const float*>(a.ks)[size_t(hh) * size_t(size) + size_t(slot)];
+      } else {
+        k[u][x] = *reinterpret_cast<const Raw*>(a.ck + k4_code(hh, slot, dim, size, D).byte);
+        ks[u][x] = __builtin_amdgcn_cvt_f32_fp8(int(a.ks[k4_scale(hh, slot, dim, size, D)]), 0) * a.kglobal;
       }
-      store_row4(dst(a.k, r) + dim, x);
-    };
-    take(8 * c);
-    take(D / 2 + 8 * c);
-  }
-  float v[P][8], scale[8];
-  const int slot0 = t.slot + 4 * g;
+    }
 #pragma unroll
   for (int x = 0; x < P; ++x) {
-    if constexpr (T == kBf16) {
-      load_row4(reinterpret_cast<const __bf16*>(a.cv) + kv_v_index(hh, slot0, v_dim + x, size, D), v[x]);
-    } else if constexpr (T == kFp8) {
-      fp8_values(*reinterpret_cast<const uint2*>(a.cv + kv_v8_index(hh, slot0, v_dim + x, size, D)), 1.f, v[x]);
-    } else {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(a.cv + v4_code(hh, slot0, v_dim + x, size, D).byte);
-      const auto y0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 0), y1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 1);
-      const auto y2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 2), y3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.f, 3);
-      v[x][0] = y0[0], v[x][1] = y0[1], v[x][2] = y1[0], v[x][3] = y1[1];
-      v[x][4] = y2[0], v[x][5] = y2[1], v[x][6] = y3[0], v[x][7] = y3[1];
-    }
+    if constexpr (T == kBf16)
+      v[x] = *reinterpret_cast<const Raw*>(reinterpret_cast<const __bf16*>(a.cv) + kv_v_index(hh, slot0, v_dim + x, size, D));
+    else if constexpr (T == kFp8)
+      v[x] = *reinterpret_cast<const Raw*>(a.cv + kv_v8_index(hh, slot0, v_dim + x, size, D));
+    else
+      v[x] = *reinterpret_cast<const Raw*>(a.cv + v4_code(hh, slot0, v_dim + x, size, D).byte);
+  }
+  if constexpr (T == kFp8) {
+    const float4* s = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.vs) + size_t(hh) * size_t(size) + size_t(slot0));
+    const float4 lo = s[0], hi = s[4];
+    vs[0] = lo.x, vs[1] = lo.y, vs[2] = lo.z, vs[3] = lo.w, vs[4] = hi.x, vs[5] = hi.y, vs[6] = hi.z, vs[7] = hi.w;
   }
   if constexpr (T == kNvfp4) {
     const uint2 w = *reinterpret_cast<const uint2*>(a.vs + v4_scale(hh, slot0, v_dim, size, D));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) scale[e] = __builtin_amdgcn_cvt_f32_fp8(int((e < 4 ? w.x : w.y) >> (8 * (e & 3)) & 0xffu), 0) * a.vglobal;
+    for (int e = 0; e < 8; ++e) vs[e] = __builtin_amdgcn_cvt_f32_fp8(int((e < 4 ? w.x : w.y) >> (8 * (e & 3)) & 0xffu), 0) * a.vglobal;
   }
+
+  auto values = [&](const Raw& w, float s, float (&x)[8]) {
+    if constexpr (T == kBf16)
+      load_row4(reinterpret_cast<const __bf16*>(&w), x);
+    else if constexpr (T == kFp8)
+      fp8_values(w, s, x);
+    else
+      fp4_values(w, s, x);
+  };
+  auto dst = [&](void* rows, int r) {
+    return static_cast<X*>(rows) + (size_t(r) * size_t(a.kv_heads) + size_t(t.head)) * D;
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int key = u * KP + key0, r = key < 32 ? t.row(key) : -1;
+    if (r < 0) continue;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      float y[8] = {};
+      if (held) values(k[u][x], ks[u][x], y);
+      store_row4(dst(a.k, r) + x * (D / 2) + 8 * c, y);
+    }
+  }
+  float y[P][8];
+#pragma unroll
+  for (int x = 0; x < P; ++x) values(v[x], 1.f, y[x]);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int r = t.row(v_slot(g, e));
     if (r < 0) continue;
-    if constexpr (T == kFp8) scale[e] = reinterpret_cast<const float*>(a.vs)[size_t(hh) * size_t(size) + size_t(t.slot + v_slot(g, e))];
-    float y[P];
+    float z[P];
 #pragma unroll
-    for (int x = 0; x < P; ++x) y[x] = !held ? 0.f : T == kBf16 ? v[x][e] : v[x][e] * scale[e];
-    store_row4(dst(a.v, r) + v_dim, y);
+    for (int x = 0; x < P; ++x) z[x] = !held ? 0.f : T == kBf16 ? y[x][e] : y[x][e] * vs[e];
+    store_row4(dst(a.v, r) + v_dim, z);
   }
 }
 
