@@ -269,10 +269,10 @@ typedef struct xtg_paged_rows {
 /* The rows' keys and values into their sequences' pages, as xtg_hip_kv_write rounds and scales them, after what the Q/K
  * producer does to q and k (xtg_hip_qk_rope_norm): rotation by the row's position (theta 0: none; pairs (i, i + head_dim / 2)
  * by pos * theta^(-2i/head_dim), an angle held in 64 bits, where the producer's are FP32 products), justnorm per head (norm != 0),
- * and q times qscale (NULL: no scale). q may be NULL; q_out, rows of q's stride, may be q. A row whose position has no page
- * is not stored (its q_out is written all the same). Rows are x_dtype, x_stride elements apart (0: packed; else a multiple of
- * 16 bytes), 16-byte aligned. A page that a call writes is in one sequence's table at that place. Queued; the first call of a
- * theta makes its table (make it before a graph capture). */
+ * and q times qscale (NULL: no scale). q may be NULL; q_out, rows of q's stride, may be q, and overlaps no input otherwise. A
+ * row whose position has no page is not stored (its q_out is written all the same). Rows are x_dtype, x_stride elements apart
+ * (0: packed; else a multiple of 16 bytes), 16-byte aligned. A page that a call writes is in one sequence's table at that
+ * place. Queued; the first call of a theta makes its table (make it before a graph capture). */
 typedef struct xtg_paged_append {
   int heads;               /* of q */
   const void* q;           /* device [n_rows][heads][head_dim], or NULL */
@@ -295,9 +295,10 @@ int xtg_hip_paged_read(xtg_hip* h, const xtg_hip_paged* c, const xtg_paged_rows*
  * position t sees positions p <= t, and p > t - window where window > 0, with scores as xtg_hip_attention_ext's: (q . k) * scale,
  * then softcap * tanh(s / softcap) where softcap > 0. Rows of a sequence that is left out get zeros; a row that sees a
  * position without a page, or whose scores are all minus infinity, NaN. What is in a page beside the positions that a row
- * sees, NaN too, is nothing to it. Rows are x_dtype (FP32 q is rounded to BF16, out is not); precision as xtg_hip_attention_ext. Up to
- * 128 q heads per KV head; n_rows * heads up to 2^27; out, packed, overlaps no input. Queued; the first call of so many rows, sequences and
- * heads sizes scratch memory, whatever the sequences' lengths (make it before a graph capture). */
+ * sees, NaN too, is nothing to it. Rows are x_dtype (FP32 q is rounded to BF16, out is not); precision as
+ * xtg_hip_attention_ext. Up to 128 q heads per KV head; n_rows * heads up to 2^27; out, packed, overlaps no input. Queued; the
+ * first call of so many rows, sequences and heads sizes scratch memory, whatever the sequences' lengths (make it before a
+ * graph capture). */
 typedef struct xtg_paged_attn {
   int heads;
   const void* q;           /* device [n_rows][heads][head_dim], q_stride elements apart (0: packed), 16-byte aligned */

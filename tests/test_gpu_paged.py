@@ -2,6 +2,7 @@
 element, within what their roundings allow: every cache dtype and head size, sequences of any length, rows of one token and
 of many, rotation and norms, strided rows, windows, pages that are reused, missing or shared, left-out sequences."""
 import ctypes
+import types
 
 import numpy as np
 import pytest
@@ -796,6 +797,10 @@ def test_refusals(hip, pkg):
     gone.free()
     with pytest.raises(pkg.XtgError, match="have been freed"):
         c.read(late, k, k)
+    other = hip.paged_rows(pos, table)
+    other.b = types.SimpleNamespace(device=hip.device + 1)
+    with pytest.raises(pkg.XtgError, match="not in the memory of the backend's device"):
+        c.read(other, k, k)
     # nothing to do is done
     none = hip.paged_rows(pos, table, 0, hip.array(np.zeros(3, np.int32)))
     c.append(none, k, k)

@@ -772,7 +772,7 @@ class PagedRows:
         if len(pages.shape) != 2:
             raise XtgError("pages is not [n_seqs][max_pages]")
         n_seqs, max_pages = (int(x) for x in pages.shape)
-        n_rows = n_seqs if n_rows is None else n_rows
+        n_rows = n_seqs if n_rows is None else int(n_rows)
         self.b, self.n_seqs, self.n_rows = backend, n_seqs, n_rows
         self.arrays = pos, pages, starts   # held as long as this is
         self.args = PagedRowsArgs(n_seqs, n_rows, _device_ptr(backend, "pos", pos, n_seqs, _I32),
@@ -781,8 +781,10 @@ class PagedRows:
         self._ref = ctypes.byref(self.args)
         self._own = [a for a in self.arrays if isinstance(a, DeviceArray)]   # whose memory can be freed while they are held
 
-    @property
-    def ref(self):
+    def of(self, backend):
+        """What a call of this backend takes."""
+        if backend.device != self.b.device:
+            raise XtgError("the rows' positions and pages are not in the memory of the backend's device")
         for a in self._own:
             if not a.ptr:
                 raise XtgError("the positions, pages or starts of the rows have been freed")
@@ -832,7 +834,7 @@ class PagedCache:
         if qscale is not None:
             qscale = _device_ptr(b, "qscale", qscale, heads * self.head_dim, X_F32)
         a = PagedAppendArgs(heads, q, q_out, k, v, q_stride, k_stride, v_stride, x_dtype, theta, norm, qscale)
-        if _lib.xtg_hip_paged_append(b.h, self.h, rows.ref, ctypes.byref(a), b._err, _ERR_LEN):
+        if _lib.xtg_hip_paged_append(b.h, self.h, rows.of(b), ctypes.byref(a), b._err, _ERR_LEN):
             _check(-1, b._err)
 
     def read(self, rows, k, v, x_dtype=X_F32):
@@ -840,7 +842,7 @@ class PagedCache:
         page (xtg_hip_paged_read)."""
         b = self.b
         k, v = _device_rows(b, k, v, rows.n_rows * self.kv_heads * self.head_dim, x_dtype)
-        if _lib.xtg_hip_paged_read(b.h, self.h, rows.ref, k, v, x_dtype, b._err, _ERR_LEN):
+        if _lib.xtg_hip_paged_read(b.h, self.h, rows.of(b), k, v, x_dtype, b._err, _ERR_LEN):
             _check(-1, b._err)
 
     def attention(self, rows, q, out, heads, x_dtype=X_F32, window=0, scale=None, softcap=0.0, q_stride=0):
@@ -851,7 +853,7 @@ class PagedCache:
         q = _device_ptr(b, "q", q, n if not q_stride else self._elems(rows, heads, q_stride), x_dtype)
         a = PagedAttnArgs(heads, q, q_stride, _device_ptr(b, "out", out, n, x_dtype), x_dtype, window,
                           d ** -0.5 if scale is None else scale, softcap)
-        if _lib.xtg_hip_paged_attention(b.h, self.h, rows.ref, ctypes.byref(a), b._err, _ERR_LEN):
+        if _lib.xtg_hip_paged_attention(b.h, self.h, rows.of(b), ctypes.byref(a), b._err, _ERR_LEN):
             _check(-1, b._err)
 
 

@@ -882,6 +882,7 @@ void Backend::paged_append(DevPaged* c, const xtg_paged_rows& rows, const xtg_pa
   XTG_CHECK(a.k && a.v, "paged_append: NULL rows");
   for (const void* p : {a.k, a.v, a.q, static_cast<const void*>(a.q_out), static_cast<const void*>(a.qscale)})
     XTG_CHECK(aligned16(p), "paged_append: rows and the scale must be 16-byte aligned");
+  const OnDevice on(device_);
   PagedAppend p = {};
   const long long kv = (long long)c->kv_heads * c->head_dim, q = (long long)a.heads * c->head_dim;
   p.heads = a.heads;
@@ -902,6 +903,7 @@ void Backend::paged_read(const DevPaged* c, const xtg_paged_rows& rows, void* k,
   if (rows.n_rows == 0 || rows.n_seqs == 0) return;
   XTG_CHECK(k && v, "paged_read: NULL rows");
   XTG_CHECK(aligned16(k) && aligned16(v), "paged_read: rows must be 16-byte aligned");
+  const OnDevice on(device_);
   timed([&] { return launch_paged_read(*c, s, k, v, x_dtype == kXBF16, stream_); });
 }
 
@@ -921,6 +923,7 @@ void Backend::paged_attention(const DevPaged* c, const xtg_paged_rows& rows, con
   p.ldq = row_stride("paged_attention", "q", a.q_stride, (long long)a.heads * c->head_dim, a.x_dtype);
   p.x_dtype = a.x_dtype, p.window = a.window, p.scale = a.scale, p.softcap = a.softcap;
   const PagedPlan plan = paged_plan(p, cus_);
+  const OnDevice on(device_);
   ensure(paged_part_, paged_part_size_, plan.bytes());
   launch_paged_attn(p, plan, paged_part_, stream_, [&](auto&& launch) { timed(launch); });
 }
@@ -931,7 +934,6 @@ const double* Backend::turn_freq(float theta, int d) {
   XTG_CHECK(!capturing_, "rotation: the frequencies for theta %g, head_dim %d must exist before a graph capture", double(theta), d);
   std::vector<double> h(size_t(d / 2));
   for (int i = 0; i < d / 2; ++i) h[size_t(i)] = 2.0 / 3.14159265358979323846 * std::pow(double(theta), -2.0 * i / d);
-  const OnDevice on(device_);
   double* p = nullptr;
   HIP_CHECK(hipMalloc(&p, h.size() * sizeof(double)));
   HIP_CHECK(hipMemcpy(p, h.data(), h.size() * sizeof(double), hipMemcpyHostToDevice));

@@ -974,7 +974,10 @@ __device__ inline int4 merge_info(const PagedArgs& a, int id, int total) {
   info = a.info[size_t(row) * size_t(a.group) + size_t(head % a.group)];
   const int splits = info.z >> 8, cols = info.y & 1 ? kManyCols : a.cols;
   const long long last = info.x + (splits - 1LL) * (info.y >> 1) * cols + cols;
-  if (splits <= 1 || info.x < 0 || last > a.records) info.z = 0;   // (past the records: only where starts decrease)
+  // (where starts decrease, a row's place may be of another call)
+  if (splits <= 1 || info.x < 0 || info.y < 0 || last > a.records || (info.z & 0xff) >= cols ||
+      uint32_t(info.w) >= uint32_t(a.s.n_seqs))
+    info.z = 0;
   return info;
 }
 
