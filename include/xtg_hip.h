@@ -297,8 +297,8 @@ int xtg_hip_paged_read(xtg_hip* h, const xtg_hip_paged* c, const xtg_paged_rows*
  * position without a page, or whose scores are all minus infinity, NaN. What is in a page beside the positions that a row
  * sees, NaN too, is nothing to it. Rows are x_dtype (FP32 q is rounded to BF16, out is not); precision as
  * xtg_hip_attention_ext. Up to 128 q heads per KV head; n_rows * heads up to 2^27; out, packed, overlaps no input. Queued; the
- * first call of so many rows, sequences and heads sizes scratch memory, whatever the sequences' lengths (make it before a
- * graph capture). */
+ * first call of so many rows, sequences and heads, and of tables for more than 128 positions, sizes scratch memory, whatever
+ * the sequences' lengths (make it before a graph capture). */
 typedef struct xtg_paged_attn {
   int heads;
   const void* q;           /* device [n_rows][heads][head_dim], q_stride elements apart (0: packed), 16-byte aligned */

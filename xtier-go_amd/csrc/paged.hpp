@@ -109,7 +109,8 @@ struct PagedPlan {
 PagedPlan paged_plan(const PagedAttnCall& a, int cus);
 
 constexpr int kManyCols = 128;
-// Fewest tiles of a part: one a wave; and of a block of many q-cols (512 rows of 256 dims over 3000 positions: 57 us with 32, 43 with 16 or 12, 46 with 8).
+// Fewest tiles of a part: one a wave; and of a block of many q-cols (300 rows of 256 dims over 3000 positions: 57 us with 32,
+// 43 with 16 or 12, 46 with 8).
 constexpr int kFewLeast = 4, kManyLeast = 16;
 
 struct PagedArgs {

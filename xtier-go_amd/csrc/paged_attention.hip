@@ -14,13 +14,14 @@ PagedPlan paged_plan(const PagedAttnCall& a, int cus) {
   PagedPlan p;
   const int kv_heads = a.cache->kv_heads, group = a.heads / kv_heads, seqs = a.seqs.n_seqs;
   const long long cols = (long long)a.seqs.n_rows * group;
-  // 32 q-cols a work-group where sequences have more than 16 on the average, but not a prompt's number
+  // 32 q-cols a work-group where sequences have more than 16 on the average, but not a prompt's number (16 sequences of 8 rows
+  // of 4 q heads a KV head over NVFP4 pages: 37 us; as blocks of many q-cols 62)
   p.cols = cols > 16LL * seqs && cols <= 32LL * seqs ? 32 : 16;
   // (heads of 256 dims: 32 do not fit a wave's registers where work-groups have eight)
   const long long most = a.seqs.starts ? cols : group;   // q-cols of a sequence
   if (a.cache->head_dim == 256 && most > p.cols) p.cols = 16;
   p.many = most > p.cols;
-  // the work-groups that are resident at once
+  // the work-groups that are resident at once (half to four times as many: within 2 % or slower)
   p.budget = std::max(1, (p.many ? cus : 2 * cus) / kv_heads);
   // a sequence's last block and a block's last part are begun ones; and total / budget is rounded, in FP32
   const long long parts = p.budget + p.budget / 64 + 1, tasks = (p.many ? cols / kManyCols : 0) + seqs + parts;
