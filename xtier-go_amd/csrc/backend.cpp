@@ -894,7 +894,7 @@ void Backend::paged_append(DevPaged* c, const xtg_paged_rows& rows, const xtg_pa
   p.freq = a.theta > 0.f ? turn_freq(a.theta, c->head_dim) : nullptr;
   p.qscale = a.qscale;
   c->written = true;
-  timed([&] { return launch_paged_append(*c, s, p, stream_); });
+  timed([&] { return launch_paged_append(*c, s, p, stream_, profile_ != 0); });
 }
 
 void Backend::paged_read(const DevPaged* c, const xtg_paged_rows& rows, void* k, void* v, int x_dtype) {
@@ -904,7 +904,7 @@ void Backend::paged_read(const DevPaged* c, const xtg_paged_rows& rows, void* k,
   XTG_CHECK(k && v, "paged_read: NULL rows");
   XTG_CHECK(aligned16(k) && aligned16(v), "paged_read: rows must be 16-byte aligned");
   const OnDevice on(device_);
-  timed([&] { return launch_paged_read(*c, s, k, v, x_dtype == kXBF16, stream_); });
+  timed([&] { return launch_paged_read(*c, s, k, v, x_dtype == kXBF16, stream_, profile_ != 0); });
 }
 
 void Backend::paged_attention(const DevPaged* c, const xtg_paged_rows& rows, const xtg_paged_attn& a) {
@@ -921,7 +921,7 @@ void Backend::paged_attention(const DevPaged* c, const xtg_paged_rows& rows, con
   PagedAttnCall p = {};
   p.cache = c, p.seqs = s, p.heads = a.heads, p.q = a.q, p.out = a.out;
   p.ldq = row_stride("paged_attention", "q", a.q_stride, (long long)a.heads * c->head_dim, a.x_dtype);
-  p.x_dtype = a.x_dtype, p.window = a.window, p.scale = a.scale, p.softcap = a.softcap;
+  p.x_dtype = a.x_dtype, p.window = a.window, p.scale = a.scale, p.softcap = a.softcap, p.named = profile_ != 0;
   const PagedPlan plan = paged_plan(p, cus_);
   const OnDevice on(device_);
   ensure(paged_part_, paged_part_size_, plan.bytes());

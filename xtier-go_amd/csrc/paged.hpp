@@ -78,9 +78,10 @@ struct PagedAppend {
   const double* freq;        // quarter turns a position of each pair (Backend::turn_freq), NULL: no rotation
   const float* qscale;
 };
-std::string launch_paged_append(const DevPaged& c, const Seqs& s, const PagedAppend& a, hipStream_t stream);
+// A launch's name is made where it is asked for (`named`): making it takes 0.1 to 0.2 us, a call 5.
+std::string launch_paged_append(const DevPaged& c, const Seqs& s, const PagedAppend& a, hipStream_t stream, bool named);
 // Rows into k, v [n_rows][kv_heads][head_dim]; zeros where there is no page, nothing behind the last sequence's rows.
-std::string launch_paged_read(const DevPaged& c, const Seqs& s, void* k, void* v, bool bf16, hipStream_t stream);
+std::string launch_paged_read(const DevPaged& c, const Seqs& s, void* k, void* v, bool bf16, hipStream_t stream, bool named);
 
 struct PagedAttnCall {
   const DevPaged* cache;
@@ -91,6 +92,7 @@ struct PagedAttnCall {
   long long ldq;
   int x_dtype, window;
   float scale, softcap;
+  bool named;
 };
 
 // How an attention call is cut up. A q-col is a (row, q head of a KV head). A sequence of up to `cols` of them (a decode or

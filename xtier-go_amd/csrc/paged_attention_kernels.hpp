@@ -1114,7 +1114,7 @@ void paged_go(const PagedAttnCall& c, const PagedPlan& p, const PagedArgs& a, hi
       go(&paged_attn_kernel<D, 2, T, MOD, true>, paged_lds<D, 2, T, true>());
     else
       fail("paged_attention: a plan of 32 q-cols for heads of 256 dims");
-    return strf("paged_attn_kernel<%d, %d, %d, %d, %d>", D, p.cols / 16, T, MOD, int(p.many));
+    return c.named ? strf("paged_attn_kernel<%d, %d, %d, %d, %d>", D, p.cols / 16, T, MOD, int(p.many)) : std::string();
   });
   if (p.records > 0) timed([&] {
     const int total = c.seqs.n_rows * c.heads, n = total <= kMergeFew ? 0 : total <= kMergeMost ? 1 : 4;
@@ -1127,7 +1127,7 @@ void paged_go(const PagedAttnCall& c, const PagedPlan& p, const PagedArgs& a, hi
       go(&paged_merge_kernel<D, T, 1, 1>, 4);
     else
       go(&paged_merge_kernel<D, T, 1, 4>, 16);
-    return strf("paged_merge_kernel<%d, %d, %d, %d>", D, T, n == 0 ? 4 : 1, n > 1 ? n : 1);
+    return c.named ? strf("paged_merge_kernel<%d, %d, %d, %d>", D, T, n == 0 ? 4 : 1, n > 1 ? n : 1) : std::string();
   });
 }
 

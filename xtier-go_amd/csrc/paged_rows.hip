@@ -439,7 +439,7 @@ static void for_shape(int d, int type, bool bf16, F&& go) {
   if (d == 256) of_type(std::integral_constant<int, 256>{});
 }
 
-std::string launch_paged_append(const DevPaged& c, const Seqs& s, const PagedAppend& p, hipStream_t stream) {
+std::string launch_paged_append(const DevPaged& c, const Seqs& s, const PagedAppend& p, hipStream_t stream, bool named) {
   AppendArgs a = {};
   a.s = s;
   a.ck = static_cast<uint8_t*>(c.k), a.cv = static_cast<uint8_t*>(c.v);
@@ -456,7 +456,7 @@ std::string launch_paged_append(const DevPaged& c, const Seqs& s, const PagedApp
   for_shape(c.head_dim, c.type, bf16, [&](auto D, auto T, auto x) {
     paged_queue(&paged_append_kernel<D(), T(), decltype(x)>, dim3(unsigned(groups)), 256, 0, stream, a);
   });
-  return strf("paged_append_kernel<%d, %d, %s>", c.head_dim, c.type, bf16 ? "bf16" : "float");
+  return named ? strf("paged_append_kernel<%d, %d, %s>", c.head_dim, c.type, bf16 ? "bf16" : "float") : std::string();
 }
 
 // ------------------------------------------------------------------------------------------------------- read
@@ -564,7 +564,7 @@ __global__ void __launch_bounds__(256) paged_read_kernel(PagedReadArgs a) {
   }
 }
 
-std::string launch_paged_read(const DevPaged& c, const Seqs& s, void* k, void* v, bool bf16, hipStream_t stream) {
+std::string launch_paged_read(const DevPaged& c, const Seqs& s, void* k, void* v, bool bf16, hipStream_t stream, bool named) {
   PagedReadArgs a = {};
   a.s = s;
   a.ck = static_cast<const uint8_t*>(c.k), a.cv = static_cast<const uint8_t*>(c.v);
@@ -575,7 +575,7 @@ std::string launch_paged_read(const DevPaged& c, const Seqs& s, void* k, void* v
   for_shape(c.head_dim, c.type, bf16, [&](auto D, auto T, auto x) {
     paged_queue(&paged_read_kernel<D(), T(), decltype(x)>, dim3(unsigned(groups)), 256, 0, stream, a);
   });
-  return strf("paged_read_kernel<%d, %d, %s>", c.head_dim, c.type, bf16 ? "bf16" : "float");
+  return named ? strf("paged_read_kernel<%d, %d, %s>", c.head_dim, c.type, bf16 ? "bf16" : "float") : std::string();
 }
 
 }  // namespace xtg::hip
