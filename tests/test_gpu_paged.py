@@ -839,3 +839,22 @@ def test_scratch_is_refused_during_a_capture(pkg):
         b.graph_destroy(b.graph_end("attention"))
     finally:
         b.close()
+
+
+def test_the_profiler_names_the_kernels(hip):
+    c = hip.paged_cache(2, 64, 16, 32)
+    pos, table = hip.array(np.array([300, 7], np.int32)), hip.array(np.arange(32, dtype=np.int32).reshape(2, 16) % 16)
+    rows = hip.paged_rows(pos, table)
+    kv, q = hip.array(np.zeros((2, 2, 64), np.float32)), hip.array(np.zeros((2, 8, 64), np.float32))
+    out = hip.array(shape=(2, 8, 64))
+    hip.profile()
+    c.append(rows, kv, kv)
+    c.read(rows, kv, kv)
+    c.attention(rows, q, out, 8)
+    names = hip.profile_report()
+    hip.profile(False)
+    assert {n.split("<")[0]: x["calls"] for n, x in names.items()} == {
+        "paged_append_kernel": 1, "paged_read_kernel": 1, "paged_attn_kernel": 1, "paged_merge_kernel": 1}
+    c.destroy()
+    for x in (pos, table, kv, q, out):
+        x.free()
