@@ -266,8 +266,9 @@ typedef struct xtg_paged_rows {
   int max_pages;
 } xtg_paged_rows;
 
-/* The rows' keys and values into their sequences' pages, as xtg_hip_kv_write rounds and scales them, after what the Q/K
- * producer does to q and k (xtg_hip_qk_rope_norm): rotation by the row's position (theta 0: none; pairs (i, i + head_dim / 2)
+/* The rows' keys and values into their sequences' pages, as xtg_hip_kv_write rounds and scales them (but that FP8 scales are
+ * amax times the FP32 number nearest to 1/448, which may differ from the quotient in the last bit, and rows of less than 2^-117
+ * are zeros), after what the Q/K producer does to q and k (xtg_hip_qk_rope_norm): rotation by the row's position (theta 0: none; pairs (i, i + head_dim / 2)
  * by pos * theta^(-2i/head_dim), an angle held in 64 bits, where the producer's are FP32 products), justnorm per head (norm != 0),
  * and q times qscale (NULL: no scale). q may be NULL; q_out, rows of q's stride, may be q, and overlaps no input otherwise. A
  * row whose position has no page is not stored (its q_out is written all the same). Rows are x_dtype, x_stride elements apart

@@ -20,6 +20,19 @@ def unit(rng, shape):
     return x / np.linalg.norm(x, axis=-1, keepdims=True)
 
 
+def stored_fp8(x):
+    """E4M3 codes of x / scale with scale amax * (1 / 448) per (row, head), in FP32 (o.stored_fp8 has the quotient)."""
+    x = np.asarray(x, np.float32)
+    amax = np.fmax.reduce(np.abs(x), axis=-1, keepdims=True, initial=np.float32(0))
+    s = np.where(amax >= np.float32(448 * 2.0 ** -126), amax * (np.float32(1) / np.float32(448)), np.float32(1)).astype(np.float32)
+    y = (x * (np.float32(1) / s)).astype(np.float64)
+    return np.minimum(o.nearest(np.abs(y), 4, 2.0 ** -9), 448.0) * np.sign(y) * s.astype(np.float64)
+
+
+def stored_pair(k, v, dtype, globals_=(1.0, 1.0)):
+    return (stored_fp8(k), stored_fp8(v)) if dtype == "fp8" else o.stored_pair(k, v, dtype, globals_)
+
+
 class Pool:
     """A pool and some sequences in it: their pages in no order, and what each of their positions holds, in FP32."""
 
@@ -74,7 +87,7 @@ class Pool:
 
     def held(self, s, n):
         """The stored values of sequence s's first n positions, in 64 bits."""
-        return o.stored_pair(self.k[s][:n], self.v[s][:n], self.dtype, self.globals_)
+        return stored_pair(self.k[s][:n], self.v[s][:n], self.dtype, self.globals_)
 
     def read(self, pos, n, x_dtype=o.F32, **kw):
         shape = (sum(n), self.kvh, self.d)
@@ -250,7 +263,7 @@ def test_rotation_and_norm(hip, d, dtype, x_dtype, theta, norm, scaled):
     got_k, got_v = p.read(pos, n)
     off = np.abs(got_k - y)
     assert (off <= bound).all(), (off / bound).max()
-    np.testing.assert_array_equal(got_v, o.stored_pair(o.rows(v, x_dtype)[1], o.rows(v, x_dtype)[1], dtype)[1].astype(np.float32))
+    np.testing.assert_array_equal(got_v, stored_pair(o.rows(v, x_dtype)[1], o.rows(v, x_dtype)[1], dtype)[1].astype(np.float32))
     for x in given + [out, sc]:
         x.free()
     p.free()
@@ -717,7 +730,7 @@ def test_offsets_beyond_32_bits(hip):
     c.append(rows, dev[0], dev[1])
     out = [hip.array(shape=(n, kvh, d)) for _ in "kv"]
     c.read(rows, out[0], out[1])
-    want = o.stored_pair(k, v, "fp8")
+    want = stored_pair(k, v, "fp8")
     for x, w in zip(out, want):
         np.testing.assert_array_equal(x.numpy(), w.astype(np.float32))
     q = unit(rng, (1, 16, d)) * np.float32(d)
@@ -858,3 +871,30 @@ def test_the_profiler_names_the_kernels(hip):
     c.destroy()
     for x in (pos, table, kv, q, out):
         x.free()
+
+
+@pytest.mark.parametrize("x_dtype", [1, 0])
+def test_fp8_rows_midway_between_codes_and_tiny_ones(hip, x_dtype):
+    """Rows whose values lie on the midpoints of their codes (amax 7 u, values M u), which the scale's last bit decides, and
+    rows whose scale would be no normal number."""
+    kvh, d = 2, 128
+    rng = np.random.default_rng(11)
+    u = np.repeat([1.0, 3.0, 5.0, 7.0], 2)[:, None, None]
+    x = rng.integers(8, 16, (8, kvh, d)) * 2 + 1
+    x = (x * u * 2.0 ** -rng.integers(3, 9, (8, kvh, d)) * rng.choice([-1, 1], (8, kvh, d))).astype(np.float32)
+    x[..., 5] = 7.0 * u[..., 0]
+    x[1] *= np.float32(2.0 ** -130)
+    x[3] *= np.float32(2.0 ** -118)
+    c = hip.paged_cache(kvh, d, 1, 32, o.KV["fp8"])
+    pos, starts, table = (hip.array(np.array(y, np.int32)) for y in ([0], [0, 8], [[0]]))
+    rows = hip.paged_rows(pos, table, 8, starts)
+    a, want = o.rows(x, x_dtype)
+    dev, k, v = hip.array(a), hip.array(shape=x.shape), hip.array(shape=x.shape)
+    c.append(rows, dev, dev, x_dtype)
+    c.read(rows, k, v)
+    hip.finish()
+    for got in (k.numpy(), v.numpy()):
+        np.testing.assert_array_equal(got, stored_fp8(want).astype(np.float32))
+    c.destroy()
+    for y in (pos, starts, table, dev, k, v):
+        y.free()
