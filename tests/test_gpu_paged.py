@@ -898,3 +898,33 @@ def test_fp8_rows_midway_between_codes_and_tiny_ones(hip, x_dtype):
     c.destroy()
     for y in (pos, starts, table, dev, k, v):
         y.free()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 5, 40])
+def test_a_nan_far_below_the_best_score_is_seen_however_the_keys_are_cut(hip, dtype, n):
+    """Scores of the first half are 460 base-2 units below the second's, so that a part's factor, and a weight, is zero in
+    FP32: a NaN value there is one of every row that sees it, in a call whose blocks are cut into parts as in a call whose
+    600 sequences are one part each."""
+    rng = np.random.default_rng(20 + n)
+    ctx, d, heads = 6000, 64, 4
+    p = Pool(hip, rng, dtype, 1, d, [ctx + n], page=64)
+    u = unit(rng, (d,))
+    k = np.where(np.arange(ctx + n)[:, None, None] < ctx // 2, np.float32(-20) * u, np.float32(20) * u).astype(np.float32)
+    v = rng.standard_normal((ctx + n, 1, d)).astype(np.float32)
+    v[100, 0, 7] = np.nan
+    p.put([0], [ctx + n], k, v)
+    q = np.broadcast_to(u * np.float32(d), (n, heads, d)).astype(np.float32)
+    got, want, tol = p.attend([ctx], [n], heads, q=q)
+    gone = np.isnan(want)
+    assert gone.all() if dtype == "nvfp4" else (gone == (np.arange(d) == 7)).all()
+    same(got, want, tol)
+    many = 600
+    dq, out = hip.array(o.bf16_bits(np.tile(q, (many, 1, 1)))), hip.array(shape=(many * n, heads, d), dtype=np.uint16)
+    p.cache.attention(p.rows([ctx] * many, [n] * many, table=np.repeat(p.table, many, 0)), dq, out, heads, o.BF16)
+    got = o.bf16_values(out.numpy()).reshape(many, n, heads, d)
+    same(got[0], want, tol)
+    np.testing.assert_array_equal(got, np.broadcast_to(got[:1], got.shape))
+    dq.free()
+    out.free()
+    p.free()

@@ -1026,8 +1026,10 @@ __device__ inline bool merge_col(const PagedArgs& a, int id, int4 info, float4* 
 #pragma unroll
     for (int k = 0; k < B; ++k) {
       const float f = __builtin_amdgcn_exp2f(w[k].x - ref);
-      l += w[k].y * f;   // (a NaN stays one: a key without a page)
-      if (f != 0.f) y.x += v[k].x * f, y.y += v[k].y * f, y.z += v[k].z * f, y.w += v[k].w * f;
+      // (a NaN stays one, of a key without a page or a value, also times zero: a row is the same however its keys are cut; one
+      // of a part that the row sees nothing of is taken back by the computation key by key)
+      l += w[k].y * f;
+      y.x += v[k].x * f, y.y += v[k].y * f, y.z += v[k].z * f, y.w += v[k].w * f;
     }
   }
   l = wave_sum(x == 0 ? l : 0.f);
