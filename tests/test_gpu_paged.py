@@ -928,3 +928,27 @@ def test_a_nan_far_below_the_best_score_is_seen_however_the_keys_are_cut(hip, dt
     dq.free()
     out.free()
     p.free()
+
+
+@pytest.mark.parametrize("x_dtype", [o.F32, o.BF16])
+def test_queries_at_positions_without_a_page_are_turned_by_them(hip, x_dtype):
+    """Up to the last 32-bit position and behind it. An angle is a product of a position and a frequency, both rounded in 64 bits,
+    here as in the reference: of 2^31 radians each is off by a few times 2^-22, together by less than 2^-19."""
+    rng = np.random.default_rng(21)
+    heads, d, theta = 4, 128, 1e4
+    pos, n = [2 ** 30 - 2, 2 ** 30 + 12345, 2 ** 31 - 3], [4, 3, 5]
+    p = Pool(hip, rng, "bf16", 1, d, [40, 40, 40])
+    total = sum(n)
+    q, k = (rng.standard_normal((total, h, d)).astype(np.float32) for h in (heads, 1))
+    given, means = o.rows(q, x_dtype)
+    dev = [hip.array(given), hip.array(o.rows(k, x_dtype)[0])]
+    p.cache.append(p.rows(pos, n), dev[1], dev[1], x_dtype, dev[0], dev[0], heads, theta)
+    got = dev[0].numpy()
+    got = o.bf16_values(got) if x_dtype else got
+    y, size = rotated(means, np.concatenate([a + np.arange(m) for a, m in zip(pos, n)]), theta)
+    tol = size * 2.0 ** -19
+    assert (np.abs(got - y) <= tol + (np.abs(y) + tol) * (2.0 ** -8 if x_dtype else 2.0 ** -24)).all()
+    assert all((x == 0).all() for x in p.read([0] * 3, [40] * 3))   # nothing is stored
+    for x in dev:
+        x.free()
+    p.free()

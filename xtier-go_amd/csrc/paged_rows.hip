@@ -34,9 +34,10 @@ struct AppendArgs {
 
 // cos and sin of p quarter turns times f, in 64 bits and rounded once (in 32 bits their own roundings nearly doubled the error
 // of a turned key: of BF16 keys 7e-6 against 4e-6, and 3 % of the time of a prompt's rows). p * f is off by 2^-53 of itself:
-// under 2^-22 radians for positions up to 2^30. The series are cut at x^13 and x^14, of |x| <= pi / 4: under 2^-36.
-__device__ inline float2 turned(int p, double f) {
-  const double t = double(p) * f, n = rint(t), x = (t - n) * 1.5707963267948966, y = x * x;
+// under 2^-22 radians for positions up to 2^30, where pages end; queries may be further on, up to an int's last and a call's rows
+// behind it (p * f, under 0.64 p, still fits an int). The series are cut at x^13 and x^14, of |x| <= pi / 4: under 2^-36.
+__device__ inline float2 turned(double p, double f) {
+  const double t = p * f, n = rint(t), x = (t - n) * 1.5707963267948966, y = x * x;
   const int quarter = int(n) & 3;
   const double s = x * fma(y, fma(y, fma(y, fma(y, fma(y, -1.0 / 39916800, 1.0 / 362880), -1.0 / 5040), 1.0 / 120), -1.0 / 6), 1.0);
   const double c = fma(y, fma(y, fma(y, fma(y, fma(y, fma(y, 1.0 / 479001600, -1.0 / 3628800), 1.0 / 40320), -1.0 / 720), 1.0 / 24), -0.5), 1.0);
@@ -377,7 +378,8 @@ __device__ inline void append_q(const AppendArgs& a, int row, float2* cs_lds) {
   const int at = row - q.row0;
   if (q.pos < 0 || uint32_t(at) >= uint32_t(q.n)) return;   // (the whole work-group)
   if (a.freq) {
-    if (int(threadIdx.x) < D / 2) cs_lds[threadIdx.x] = turned(q.pos + at, f);
+    // (seq_at's position goes no further than a page's)
+    if (int(threadIdx.x) < D / 2) cs_lds[threadIdx.x] = turned(double(s.pos[seq]) + double(at), f);
     __syncthreads();
   }
   for (int x0 = 0; x0 < chunks; x0 += 256) {
