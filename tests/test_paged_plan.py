@@ -138,3 +138,33 @@ def test_a_destroyed_pool_is_refused(pkg):
         assert rc == -1 and b"NULL argument" in err.value
     assert not lib.xtg_hip_paged_create(None, 8, 128, 4, 64, 0, err, 200)
     lib.xtg_hip_paged_destroy(None, None)
+
+
+class Ints:
+    """An int32 array in the memory of device 0, for the checks of arguments alone."""
+    dtype, shape = "torch.int32", ()
+
+    def __init__(self, *shape):
+        self.shape = shape
+
+    def numel(self):
+        return int(np.prod(self.shape))
+
+    def is_contiguous(self):
+        return True
+
+    def get_device(self):
+        return 0
+
+    def data_ptr(self):
+        return 4096
+
+
+def test_starts_want_the_number_of_rows(pkg):
+    """How many rows a call with starts has is in device memory: taken as one a sequence, those behind would be lost."""
+    import types
+    b = types.SimpleNamespace(device=0, h=1)
+    assert pkg.PagedRows(b, Ints(3), Ints(3, 4)).n_rows == 3
+    assert pkg.PagedRows(b, Ints(3), Ints(3, 4), 7, Ints(4)).n_rows == 7
+    with pytest.raises(pkg.XtgError, match="n_rows"):
+        pkg.PagedRows(b, Ints(3), Ints(3, 4), starts=Ints(4))

@@ -562,7 +562,8 @@ class HipBackend:
 
     def paged_rows(self, pos, pages, n_rows=None, starts=None):
         """Whose the rows of a call are (xtg_paged_rows), for any number of calls on pools of the same pages: device int32
-        pos [n_seqs], pages [n_seqs][max_pages] and, unless row s is sequence s's, starts [n_seqs + 1]."""
+        pos [n_seqs], pages [n_seqs][max_pages] and, unless row s is sequence s's, starts [n_seqs + 1], with which n_rows
+        says how many rows the call has."""
         return PagedRows(self, pos, pages, n_rows, starts)
 
     # ---- the Dory decode step
@@ -771,6 +772,8 @@ class PagedRows:
     def __init__(self, backend, pos, pages, n_rows=None, starts=None):
         if len(pages.shape) != 2:
             raise XtgError("pages is not [n_seqs][max_pages]")
+        if starts is not None and n_rows is None:   # (rows behind one a sequence would be lost)
+            raise XtgError("rows with starts want n_rows, the number of the call's rows")
         n_seqs, max_pages = (int(x) for x in pages.shape)
         n_rows = n_seqs if n_rows is None else int(n_rows)
         self.b, self.n_seqs, self.n_rows = backend, n_seqs, n_rows
