@@ -168,3 +168,22 @@ def test_starts_want_the_number_of_rows(pkg):
     assert pkg.PagedRows(b, Ints(3), Ints(3, 4), 7, Ints(4)).n_rows == 7
     with pytest.raises(pkg.XtgError, match="n_rows"):
         pkg.PagedRows(b, Ints(3), Ints(3, 4), starts=Ints(4))
+
+
+def test_arrays_of_a_closed_backend_are_refused(pkg):
+    """Closing a backend frees its arrays, whose addresses stay: not to be read by another backend's calls."""
+    import types
+    made, other = types.SimpleNamespace(device=0, h=1), types.SimpleNamespace(device=0, h=1)
+
+    def array(*shape):
+        a = pkg.DeviceArray.__new__(pkg.DeviceArray)
+        a.b, a.shape, a.dtype, a.ptr = made, shape, np.dtype(np.int32), 4096
+        a.nbytes = 4 * int(np.prod(shape))
+        return a
+    rows = pkg.PagedRows(other, array(3), array(3, 4), 7, array(4))
+    rows.of(other)
+    made.h = None
+    with pytest.raises(pkg.XtgError, match="have been freed"):
+        rows.of(other)
+    with pytest.raises(pkg.XtgError, match="pos has been freed"):
+        pkg.PagedRows(other, array(3), array(3, 4), 7, array(4))

@@ -225,7 +225,7 @@ def _device_ptr(b, name, a, n, kind):
     if isinstance(a, int):
         return a
     if isinstance(a, DeviceArray):
-        at, size, here, whole = a.ptr, a.nbytes // a.dtype.itemsize, a.b.device == b.device, True
+        at, size, here, whole = a.ptr if a.b.h else None, a.nbytes // a.dtype.itemsize, a.b.device == b.device, True
     elif hasattr(a, "get_device"):
         at, size, here, whole = a.data_ptr(), a.numel(), a.get_device() == b.device, a.is_contiguous()
     else:
@@ -789,7 +789,7 @@ class PagedRows:
         if backend.device != self.b.device:
             raise XtgError("the rows' positions and pages are not in the memory of the backend's device")
         for a in self._own:
-            if not a.ptr:
+            if not a.ptr or not a.b.h:   # (a backend that is closed frees its arrays)
                 raise XtgError("the positions, pages or starts of the rows have been freed")
         return self._ref
 
