@@ -952,3 +952,17 @@ def test_queries_at_positions_without_a_page_are_turned_by_them(hip, x_dtype):
     for x in dev:
         x.free()
     p.free()
+
+
+def test_memory_that_is_not_there_is_no_error_of_the_next_call(hip, pkg):
+    """What fails is told once: by the call that failed, not by the next launch as well."""
+    k = hip.array(np.ones((5, 64), np.float32))
+    for _ in range(2):
+        with pytest.raises(pkg.XtgError, match="hipMalloc"):
+            hip.alloc(1 << 46)
+        hip.add_norm(k, None, k, 5, 64)
+    with pytest.raises(pkg.XtgError, match="hipMalloc"):
+        hip.paged_cache(8, 256, 200000, 4096)
+    hip.add_norm(k, None, k, 5, 64)
+    np.testing.assert_allclose(k.numpy(), 1 / 8, rtol=1e-5)
+    k.free()

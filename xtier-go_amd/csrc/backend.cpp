@@ -824,7 +824,6 @@ DevPaged* Backend::paged_create(int kv_heads, int head_dim, long long pages, int
     (void)hipStreamSynchronize(stream_);
     for (void* p : {c->k, c->v, c->ks, c->vs})
       if (p) (void)hipFree(p);
-    (void)hipGetLastError();   // (no memory, say: not the next launch's error)
     throw;
   }
   return c.release();

@@ -49,8 +49,12 @@ namespace xtg::hip {
 void allow_lds(const void* fn, size_t lds);
 }  // namespace xtg::hip
 
-#define HIP_CHECK(expr)                                                                        \
-  do {                                                                                         \
-    hipError_t e_ = (expr);                                                                    \
-    if (e_ != hipSuccess) ::xtg::hip::fail("%s failed: %s", #expr, hipGetErrorString(e_)); \
+// A failure is this call's alone: HIP keeps it as the last error, which a launch behind would take for its own.
+#define HIP_CHECK(expr)                                                               \
+  do {                                                                                \
+    hipError_t e_ = (expr);                                                           \
+    if (e_ != hipSuccess) {                                                           \
+      (void)hipGetLastError();                                                        \
+      ::xtg::hip::fail("%s failed: %s", #expr, hipGetErrorString(e_));                \
+    }                                                                                 \
   } while (0)
