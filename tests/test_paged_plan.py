@@ -187,3 +187,46 @@ def test_arrays_of_a_closed_backend_are_refused(pkg):
         rows.of(other)
     with pytest.raises(pkg.XtgError, match="pos has been freed"):
         pkg.PagedRows(other, array(3), array(3, 4), 7, array(4))
+
+
+def test_rows_that_are_part_of_wider_ones(pkg, monkeypatch):
+    """q, k and v as views of one projection's rows, with their stride; a stride that is not the view's, rows that are not
+    packed, too few, of another type or on another device are refused. (Tensors of the CPU, whose device is -1, and a library
+    that takes the call's arguments down.)"""
+    import types
+    torch = pytest.importorskip("torch")
+    b = types.SimpleNamespace(device=-1, h=1, _err=None)
+    got = []
+
+    def taken(h, cache, rows, args, err, n):
+        got.append(args._obj)
+        return 0
+    monkeypatch.setattr(pkg, "_lib", types.SimpleNamespace(xtg_hip_paged_append=taken, xtg_hip_paged_attention=taken))
+    c = pkg.PagedCache.__new__(pkg.PagedCache)
+    c.b, c.h, c.kv_heads, c.head_dim = b, 1, 2, 64
+    rows = types.SimpleNamespace(n_rows=5, of=lambda backend: None)
+    heads, width = 8, 12 * 64
+    x = torch.zeros((6, width), dtype=torch.bfloat16)
+    q, k, v = x[:, :512], x[:, 512:640], x[:, 640:]
+    for shaped in (lambda y: y, lambda y: y.unflatten(1, (-1, 64))):
+        c.append(rows, shaped(k), shaped(v), pkg.X_BF16, shaped(q), shaped(q), heads, 1e4, q_stride=width, k_stride=width, v_stride=width)
+        c.attention(rows, shaped(q), torch.zeros((5, heads, 64), dtype=torch.bfloat16), heads, pkg.X_BF16, q_stride=width)
+        for a in got:
+            assert a.q == x.data_ptr() and a.q_stride == width
+        assert (got[0].k, got[0].v, got[0].q_out) == (x.data_ptr() + 1024, x.data_ptr() + 1280, x.data_ptr())
+        del got[:]
+    c.append(rows, x[:5], v, pkg.X_BF16, k_stride=width, v_stride=width)   # the whole rows' first elements
+
+    def refused(match, k, v=v, stride=width, x_dtype=pkg.X_BF16):
+        with pytest.raises(pkg.XtgError, match=match):
+            c.append(rows, k, v, x_dtype, k_stride=stride, v_stride=width)
+    refused("768 elements apart, not the call's 776", k, stride=776)
+    refused("k has 4 rows, the call 5", k[:4])
+    refused("64 elements, the call's rows of it take 128", k[:, :64])
+    refused("not contiguous", x[:, 512::2])
+    refused("not contiguous", x[:5].T)
+    refused("not of the call's row type BF16", x.float()[:, 512:640])
+    with pytest.raises(pkg.XtgError, match="not contiguous"):
+        c.append(rows, k, v, pkg.X_BF16)
+    b.device = 0
+    refused("not in the memory", k)

@@ -257,6 +257,21 @@ def _device_rows(b, k, v, n, kind):
     return _device_ptr(b, "k", k, n, kind), _device_ptr(b, "v", v, n, kind)
 
 
+def _rows_ptr(b, name, a, n, width, stride, kind):
+    """_device_ptr of n rows of `width` elements, `stride` elements apart (0: packed). A tensor may be part of wider rows, as q,
+    k and v of one projection are, where its rows are as far apart as the call says."""
+    if not stride:
+        return _device_ptr(b, name, a, n * width, kind)
+    if n and hasattr(a, "stride") and not a.is_contiguous():
+        at = _device_ptr(b, name, a[0], width, kind)   # a row of it
+        if a.shape[0] < n:
+            raise XtgError("%s has %d rows, the call %d" % (name, a.shape[0], n))
+        if a.stride(0) != stride:
+            raise XtgError("%s has rows %d elements apart, not the call's %d" % (name, a.stride(0), stride))
+        return at
+    return _device_ptr(b, name, a, (n - 1) * stride + width if n else 0, kind)
+
+
 class _Address(int):
     """The address of an array, which it holds: with a second reference numpy refuses to resize (move) it in place. A copy
     or a pickle of it reads its own array's."""
@@ -815,25 +830,20 @@ class PagedCache:
         err = _errbuf()
         _check(lib().xtg_hip_paged_globals(self.b.h, self.h, k_global, v_global, err, len(err)), err)
 
-    def _elems(self, rows, heads, stride):
-        """Elements of an array of the call's rows."""
-        width = heads * self.head_dim
-        return rows.n_rows * width if not stride else max(0, rows.n_rows - 1) * stride + (width if rows.n_rows else 0)
-
     def append(self, rows, k, v, x_dtype=X_F32, q=None, q_out=None, heads=0, theta=0.0, norm=False, qscale=None,
                q_stride=0, k_stride=0, v_stride=0):
         """Queued: the rows' k and v into their pages, k (and q, into q_out, which may be q) rotated by position (theta 0:
         not) and normalised per head first (norm), q then times qscale (xtg_hip_paged_append). Device rows of x_dtype,
-        packed or `stride` elements apart."""
+        packed or `stride` elements apart: views of one projection's rows, say."""
         b, kv = self.b, self.kv_heads
         if not k_stride and not v_stride:
             k, v = _device_rows(b, k, v, rows.n_rows * kv * self.head_dim, x_dtype)
         else:
-            k = _device_ptr(b, "k", k, self._elems(rows, kv, k_stride), x_dtype)
-            v = _device_ptr(b, "v", v, self._elems(rows, kv, v_stride), x_dtype)
+            k = _rows_ptr(b, "k", k, rows.n_rows, kv * self.head_dim, k_stride, x_dtype)
+            v = _rows_ptr(b, "v", v, rows.n_rows, kv * self.head_dim, v_stride, x_dtype)
         if q is not None:
-            n = self._elems(rows, heads, q_stride)
-            q, q_out = _device_ptr(b, "q", q, n, x_dtype), _device_ptr(b, "q_out", q_out, n, x_dtype)
+            n, width = rows.n_rows, heads * self.head_dim
+            q, q_out = _rows_ptr(b, "q", q, n, width, q_stride, x_dtype), _rows_ptr(b, "q_out", q_out, n, width, q_stride, x_dtype)
         if qscale is not None:
             qscale = _device_ptr(b, "qscale", qscale, heads * self.head_dim, X_F32)
         a = PagedAppendArgs(heads, q, q_out, k, v, q_stride, k_stride, v_stride, x_dtype, theta, norm, qscale)
@@ -853,7 +863,7 @@ class PagedCache:
         a row at position t sees p <= t, and p > t - window; scores softcap * tanh(scale * q.k / softcap)."""
         b, d = self.b, self.head_dim
         n = rows.n_rows * heads * d
-        q = _device_ptr(b, "q", q, n if not q_stride else self._elems(rows, heads, q_stride), x_dtype)
+        q = _rows_ptr(b, "q", q, rows.n_rows, heads * d, q_stride, x_dtype) if q_stride else _device_ptr(b, "q", q, n, x_dtype)
         a = PagedAttnArgs(heads, q, q_stride, _device_ptr(b, "out", out, n, x_dtype), x_dtype, window,
                           d ** -0.5 if scale is None else scale, softcap)
         if _lib.xtg_hip_paged_attention(b.h, self.h, rows.of(b), ctypes.byref(a), b._err, _ERR_LEN):
