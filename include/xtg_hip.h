@@ -257,7 +257,8 @@ int xtg_hip_paged_globals(xtg_hip* h, xtg_hip_paged* c, float k_global, float v_
  * is sequence s's (n_rows == n_seqs: a decode step). pos[s] < 0 leaves sequence s out. Position p of sequence s is in page
  * pages[s * max_pages + p / page_size]; a number that is no page of the pool, or a position behind the table's, is no page.
  * The arrays are device memory, read by the kernels as they run: a captured graph follows what is in them at its replay.
- * starts must not decrease. max_pages * page_size is 2^30 at most; n_rows is below 2^24, n_seqs below 2^20. */
+ * starts must not decrease. max_pages * page_size is 2^30 at most; n_rows is below 2^24, n_seqs up to 2^14 (the search for each
+ * piece of the work goes over all sequences: a call's time grows with their square where they are thousands). */
 typedef struct xtg_paged_rows {
   int n_seqs, n_rows;
   const int32_t* pos;      /* [n_seqs] */

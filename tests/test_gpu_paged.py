@@ -966,3 +966,25 @@ def test_memory_that_is_not_there_is_no_error_of_the_next_call(hip, pkg):
     hip.add_norm(k, None, k, 5, 64)
     np.testing.assert_allclose(k.numpy(), 1 / 8, rtol=1e-5)
     k.free()
+
+
+def test_more_sequences_than_a_call_takes_are_refused(hip, pkg):
+    """Every work-group looks for its piece among all sequences, so a call's time grows with the square of their number."""
+    n = 2 ** 14
+    c = hip.paged_cache(1, 64, 2, 32)
+    arrays = [hip.array(np.zeros(s, np.int32)) for s in ((n + 1,), (n + 1, 1), (n + 2,))]
+    x, out = hip.array(np.ones((4, 1, 64), np.float32)), hip.array(shape=(4, 1, 64))
+    rows = hip.paged_rows(arrays[0], arrays[1], 4, arrays[2])
+    for call in (lambda: c.append(rows, x, x), lambda: c.read(rows, out, out), lambda: c.attention(rows, x, out, 1)):
+        with pytest.raises(pkg.XtgError, match="4 rows of 16385 sequences"):
+            call()
+    # as many as it takes, the last of them with rows
+    arrays[2].upload(np.where(np.arange(n + 2) < n, 0, 4).astype(np.int32))
+    rows = hip.paged_rows(arrays[0], arrays[1], 4, arrays[2])
+    rows.args.n_seqs = n
+    c.append(rows, x, x)
+    c.attention(rows, x, out, 1)
+    np.testing.assert_allclose(out.numpy(), 1.0, rtol=2.0 ** -13)
+    c.destroy()
+    for a in arrays + [x, out]:
+        a.free()

@@ -850,8 +850,8 @@ void Backend::paged_globals(DevPaged* c, float kglobal, float vglobal) {
 // The checks that the three calls share.
 Seqs Backend::paged_rows(const char* what, const DevPaged* c, const xtg_paged_rows& r) const {
   XTG_CHECK(paged_.count(const_cast<DevPaged*>(c)), "%s: unknown cache", what);
-  XTG_CHECK(r.n_seqs >= 0 && r.n_rows >= 0 && r.n_rows < (1 << 24) && r.n_seqs < (1 << 20), "%s: %d rows of %d sequences (below 2^24 and 2^20)", what,
-            r.n_rows, r.n_seqs);
+  XTG_CHECK(r.n_seqs >= 0 && r.n_rows >= 0 && r.n_rows < (1 << 24) && r.n_seqs <= kMostSeqs, "%s: %d rows of %d sequences (below 2^24, up to %d)", what,
+            r.n_rows, r.n_seqs, kMostSeqs);
   XTG_CHECK(r.starts || r.n_rows == r.n_seqs, "%s: %d rows of %d sequences without starts", what, r.n_rows, r.n_seqs);
   XTG_CHECK(r.max_pages >= 1 && (long long)r.max_pages * c->size <= (1 << 30), "%s: %d pages of %d positions a sequence (2^30 positions at most)",
             what, r.max_pages, c->size);

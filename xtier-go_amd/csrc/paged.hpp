@@ -45,6 +45,11 @@ struct Seqs {
 // No position from here on has a page, and a call has fewer rows: sums of the two fit an int.
 constexpr int kMostPositions = 1 << 30;
 
+// Sequences of a call, at most. Every work-group looks for its piece among all of them, so that a call takes a time that grows
+// with their square beside its own work (one row each over 60 positions of 8 KV heads of 128 dims: 1024 sequences 0.18 ms, with
+// starts 0.83; 4096 2.0 and 11; 16384 29 and 170): 2^20 would take the GPU minutes.
+constexpr int kMostSeqs = 1 << 14;
+
 // A sequence's rows in the call, row0 .. row0 + n - 1, at positions pos .. pos + n - 1 (pos < 0: left out). Starts out of the
 // call's rows, or that decrease, are clamped: what they name is still in range.
 struct Seq {
