@@ -268,8 +268,8 @@ typedef struct xtg_paged_rows {
 } xtg_paged_rows;
 
 /* The rows' keys and values into their sequences' pages, as xtg_hip_kv_write rounds and scales them (but that FP8 scales are
- * amax times the FP32 number nearest to 1/448, which may differ from the quotient in the last bit, and rows of less than 2^-117
- * are zeros), after what the Q/K producer does to q and k (xtg_hip_qk_rope_norm): rotation by the row's position (theta 0: none; pairs (i, i + head_dim / 2)
+ * amax times the FP32 number nearest to 1/448, which may differ from the quotient in the last bit, so that a linear cache may
+ * hold other codes of the same row, and rows whose amax is below 448 * 2^-126, 1.75 * 2^-118, are zeros), after what the Q/K producer does to q and k (xtg_hip_qk_rope_norm): rotation by the row's position (theta 0: none; pairs (i, i + head_dim / 2)
  * by pos * theta^(-2i/head_dim), an angle held in 64 bits, where the producer's are FP32 products), justnorm per head (norm != 0),
  * and q times qscale (NULL: no scale). q may be NULL; q_out, rows of q's stride, may be q, and overlaps no input otherwise. A
  * row whose position has no page is not stored (its q_out is written all the same). Rows are x_dtype, x_stride elements apart
@@ -299,8 +299,9 @@ int xtg_hip_paged_read(xtg_hip* h, const xtg_hip_paged* c, const xtg_paged_rows*
  * position without a page, or whose scores are all minus infinity, NaN. What is in a page beside the positions that a row
  * sees, NaN too, is nothing to it. Rows are x_dtype (FP32 q is rounded to BF16, out is not); precision as
  * xtg_hip_attention_ext. Up to 128 q heads per KV head; n_rows * heads up to 2^27; out, packed, overlaps no input. Queued; the
- * first call of so many rows, sequences and heads, and of tables for more than 128 positions, sizes scratch memory, whatever
- * the sequences' lengths (make it before a graph capture). */
+ * first call of so many rows, sequences and heads, with starts or without, on a pool of so many KV heads and dims, and of tables
+ * for more than 128 positions or for fewer, sizes scratch memory, whatever the sequences' lengths (make it, alike in all of these,
+ * before a graph capture). */
 typedef struct xtg_paged_attn {
   int heads;
   const void* q;           /* device [n_rows][heads][head_dim], q_stride elements apart (0: packed), 16-byte aligned */

@@ -988,3 +988,27 @@ def test_more_sequences_than_a_call_takes_are_refused(hip, pkg):
     c.destroy()
     for a in arrays + [x, out]:
         a.free()
+
+
+def test_fp8_rows_at_the_least_scale(hip):
+    """From an amax of 448 * 2^-126 on rows have a scale, a normal number; below it they are zeros. A code's value there is the
+    nearest of FP32's subnormal numbers to its product with the scale."""
+    kvh, d = 2, 64
+    x = np.random.default_rng(22).uniform(-1, 1, (4, kvh, d)).astype(np.float64)
+    x[..., 9] = 1.0
+    least = np.float32(448 * 2.0 ** -126)
+    amax = np.array([least, np.nextafter(least, np.float32(0)), np.float32(2.0 ** -117), np.float32(2.0 ** -118)])
+    x = (x * amax.astype(np.float64)[:, None, None]).astype(np.float32)
+    c = hip.paged_cache(kvh, d, 1, 32, o.KV["fp8"])
+    arrays = [hip.array(np.array(y, np.int32)) for y in ([0], [[0]], [0, 4])]
+    rows = hip.paged_rows(arrays[0], arrays[1], 4, arrays[2])
+    dev, k, v = hip.array(x), hip.array(shape=x.shape), hip.array(shape=x.shape)
+    c.append(rows, dev, dev)
+    c.read(rows, k, v)
+    want = stored_fp8(x)
+    assert (want[[1, 3]] == 0).all() and (want[[0, 2]] != 0).any(axis=(1, 2)).all()
+    for got in (k.numpy(), v.numpy()):
+        np.testing.assert_array_equal(got, want.astype(np.float32))
+    c.destroy()
+    for y in arrays + [dev, k, v]:
+        y.free()

@@ -230,3 +230,36 @@ def test_rows_that_are_part_of_wider_ones(pkg, monkeypatch):
         c.append(rows, k, v, pkg.X_BF16)
     b.device = 0
     refused("not in the memory", k)
+
+
+@pytest.fixture(scope="module")
+def run_of(pkg, tmp_path_factory):
+    """The program for heads of other sizes, as functions of calls (their texts' lines to the program's numbers)."""
+    def made(d):
+        at = tmp_path_factory.mktemp("paged%d" % d)
+        (at / "plan.cpp").write_text(PROGRAM.replace("c.head_dim = 128", "c.head_dim = %d" % d))
+        csrc = os.path.join(ROOT, "xtier-go_amd", "csrc")
+        subprocess.run(["g++", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-I" + csrc, str(at / "plan.cpp"),
+                        pkg.LIB_PATH, "-Wl,-rpath," + os.path.dirname(pkg.LIB_PATH), "-L/opt/rocm/lib", "-lamdhip64", "-o",
+                        str(at / "plan")], check=True)
+
+        def go(calls):
+            text = "\n".join(" ".join(map(str, [*head, *pos, *(starts if head[8] else [])])) for head, pos, starts in calls)
+            out = subprocess.run([str(at / "plan")], input=text, capture_output=True, text=True, check=True).stdout
+            return [tuple(map(int, line.split())) for line in out.splitlines()]
+        return go
+    return {d: made(d) for d in (64, 256)}
+
+
+def test_scratch_goes_by_what_the_header_names(run, run_of):
+    """A call alike in rows, sequences, heads, starts (NULL or not), the pool's KV heads and dims and tables for more than 128
+    positions needs as much as the first such call, whatever the pages' size and number, the tables' length, the window and
+    the positions."""
+    rng = np.random.default_rng(4)
+    alike = [(kvh, kvh * group, n, rows) for kvh in (1, 8) for group in (1, 4, 40)
+             for n, rows in ((1, None), (70, None), (70, np.ones(70, int)), (3, np.array([300, 1, 0])), (9, np.array([8] * 9)))]
+    for go in (run, run_of[64], run_of[256]):
+        calls = [call(kvh, heads, rng.integers(0, 5000, n), rows, window=w, max_pages=m, shift=s, pages=p)
+                 for kvh, heads, n, rows in alike for w, m, s, p in ((0, 40, 6, 60), (100, 3, 12, 7), (1024, 5, 5, 1000))]
+        got = [r[5] for r in go(calls)]
+        assert len(got) == len(calls) and all(len(set(got[i:i + 3])) == 1 for i in range(0, len(got), 3))
