@@ -1012,3 +1012,62 @@ def test_fp8_rows_at_the_least_scale(hip):
     c.destroy()
     for y in arrays + [dev, k, v]:
         y.free()
+
+
+def attend_all(q, k, v, pos, scale):
+    """o.attend for many rows at once, without a window or a cap: (outputs, the sums of |weight * value| and 2^-32 of the
+    |value|s', the largest sum of |q.k| * scale)."""
+    n, heads, d = q.shape
+    kvh, group = k.shape[1], heads // k.shape[1]
+    out, size, floor, most = *(np.zeros((n, heads, d)) for _ in "osf"), 0.0
+    hide = np.arange(len(k))[None, None] > (pos + np.arange(n))[:, None, None]
+    for h in range(kvh):
+        kh, vh, at = k[:, h], v[:, h], slice(h * group, (h + 1) * group)
+        x = q[:, at].astype(np.float64).reshape(n * group, d)
+        part = np.where(hide, 0, (np.abs(x) @ np.abs(kh).T).reshape(n, group, -1) * scale)
+        most = max(most, part.max())
+        s = np.where(hide, -np.inf, (x @ kh.T).reshape(n, group, -1) * scale)
+        p = np.exp(s - s.max(-1, keepdims=True))
+        p = (p / p.sum(-1, keepdims=True)).reshape(n * group, -1)
+        out[:, at] = (p @ vh).reshape(n, group, d)
+        size[:, at] = (p @ np.abs(vh)).reshape(n, group, d)
+        floor[:, at] = (np.where(hide, 0.0, 1.0)[:, 0] @ np.abs(vh))[:, None] * 2.0 ** -32
+    return out, (size, floor), most
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,ctx", [(260, 4000), (40, 4000)])
+def test_a_chunk_beside_single_tokens_is_joined_by_any_merge(hip, d, dtype, rows, ctx):
+    """A chunk over some thousand positions, whose blocks are cut into several parts, beside single tokens: more than 8192
+    q-cols (a wave of the merge joins several) and more than 1024 (one each). Then a value in the chunk's last rows is NaN: the
+    rows that see it have one, and the others of its tiles, computed again behind the merge, do not."""
+    rng = np.random.default_rng(d + rows)
+    heads, kvh = 32, 4
+    pos, n = [ctx, 900, 30, 2000], [rows, 1, 1, 1]
+    p = Pool(hip, rng, dtype, kvh, d, [a + m for a, m in zip(pos, n)], page=64)
+    p.fill()
+    q = unit(rng, (sum(n), heads, d)) * np.float32(d)
+    means = o.bf16(q)
+    given, out = hip.array(o.bf16_bits(q)), hip.array(shape=q.shape, dtype=np.uint16)
+    call = p.rows(pos, n)
+
+    def attended(last):
+        p.cache.attention(call, given, out, heads, o.BF16)
+        got, at = o.bf16_values(out.numpy()), 0
+        for s, (a, m) in enumerate(zip(pos, n)):
+            k, v = (np.nan_to_num(x) for x in p.held(s, a + m))
+            w, size, most = attend_all(means[at:at + m], k, v, a, d ** -0.5)
+            tol = o.tolerance(w, size, most, d, 11 if dtype == "nvfp4" else 8, o.BF16)
+            if s == 0 and last is not None:   # NVFP4: the whole row is NaN for its KV head
+                w[last:, heads // 2:heads // 2 + heads // kvh, slice(None) if dtype == "nvfp4" else 7] = np.nan
+            same(got[at:at + m], w, tol)
+            at += m
+    attended(None)
+    k, v = (x[0][ctx + rows - 9:ctx + rows - 8].copy() for x in (p.k, p.v))
+    v[0, 2, 7] = np.nan
+    p.put([ctx + rows - 9, -1, -1, -1], [1, 0, 0, 0], k, v)
+    attended(rows - 9)
+    given.free()
+    out.free()
+    p.free()

@@ -263,3 +263,27 @@ def test_scratch_goes_by_what_the_header_names(run, run_of):
                  for kvh, heads, n, rows in alike for w, m, s, p in ((0, 40, 6, 60), (100, 3, 12, 7), (1024, 5, 5, 1000))]
         got = [r[5] for r in go(calls)]
         assert len(got) == len(calls) and all(len(set(got[i:i + 3])) == 1 for i in range(0, len(got), 3))
+
+
+def test_tasks_and_records_cover_any_lengths_of_other_heads(run_of):
+    """As for heads of 128 dims; those of 256 go in blocks of 16 q-cols beside blocks of many."""
+    rng = np.random.default_rng(5)
+    for go in run_of.values():
+        calls = []
+        for _ in range(200):
+            n, kvh = int(rng.integers(1, 200)), int(rng.choice([1, 2, 4, 8]))
+            heads, window = kvh * int(rng.choice([1, 2, 3, 8, 17, 24, 32, 128])), int(rng.choice([0, 0, 100, 1024]))
+            rows = [None, rng.integers(0, 2, n), rng.integers(2, 17, n), rng.integers(0, 500, n)][int(rng.integers(0, 4))]
+            calls.append(call(kvh, heads, rng.integers(-3, 2500, n), rows, window, cus=int(rng.choice([1, 64, 256]))))
+        for c, (tasks, most, records, room, bad, _) in zip(calls, go(calls)):
+            assert tasks <= most and records <= room and bad == 0, (c, tasks, most, records, room, bad)
+
+
+def test_a_chunk_beside_single_tokens_is_cut(run, run_of):
+    """The calls that the GPU's test of the merges makes have records: their chunks' blocks are in several parts."""
+    for go in (run, run_of[64], run_of[256]):
+        for rows, ctx in ((260, 4000), (40, 4000)):
+            calls = [call(4, 32, [ctx, 900, 30, 2000], [rows, 1, 1, 1], max_pages=70), call(4, 32, [ctx], [rows], max_pages=70)]
+            blocks = -(-rows * 8 // 128)
+            for (tasks, _, records, room, bad, _) in go(calls):
+                assert tasks >= 2 * blocks and room >= records >= 2 * blocks * 128 and bad == 0
