@@ -297,8 +297,10 @@ int xtg_hip_paged_read(xtg_hip* h, const xtg_hip_paged* c, const xtg_paged_rows*
  * position t sees positions p <= t, and p > t - window where window > 0, with scores as xtg_hip_attention_ext's: (q . k) * scale,
  * then softcap * tanh(s / softcap) where softcap > 0. Rows of a sequence that is left out get zeros; a row that sees a
  * position without a page, or whose scores are all minus infinity, NaN. What is in a page beside the positions that a row
- * sees, NaN too, is nothing to it. Rows are x_dtype (FP32 q is rounded to BF16, out is not); precision as
- * xtg_hip_attention_ext. Up to 128 q heads per KV head; n_rows * heads up to 2^27; out, packed, overlaps no input. Queued; the
+ * sees, NaN too, is nothing to it. Rows are x_dtype (FP32 q is rounded to BF16 as it is read, out is not). Scores, their maxima
+ * and sums and the output are held in FP32; the softmax weights enter the product with V as f16 (11 bits, NVFP4 pages) or as BF16
+ * (others, times an FP8 row's scale): a sum of two, 16 bits, for a sequence of up to 16 (row, q head of a KV head) pairs, one of 8
+ * bits for one of more, and for all of a call whose sequences have 17 to 32 on the average. Up to 128 q heads per KV head; n_rows * heads up to 2^27; out, packed, overlaps no input. Queued; the
  * first call of so many rows, sequences and heads, with starts or without, on a pool of so many KV heads and dims, and of tables
  * for more than 128 positions or for fewer, sizes scratch memory, whatever the sequences' lengths (make it, alike in all of these,
  * before a graph capture). */

@@ -1071,3 +1071,28 @@ def test_a_chunk_beside_single_tokens_is_joined_by_any_merge(hip, d, dtype, rows
     given.free()
     out.free()
     p.free()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", ["bf16", "fp8"])
+def test_weights_of_single_tokens_have_16_bits(hip, d, dtype):
+    """Over BF16 and FP8 pages a weight of a sequence of up to 16 q-cols is a sum of two BF16 values: what the first leaves of it,
+    2^-8, is rounded by 2^-8 of that."""
+    rng = np.random.default_rng(d + 23)
+    heads, kvh = HEADS[d]
+    lengths = [1, 2, 33, 700, 3000, 500, 64]
+    p = Pool(hip, rng, dtype, kvh, d, lengths, page=64)
+    p.fill()
+    for n, one_each in (([1] * 7, True), ([1, 2, 1, 3, 1, 4, 2], False)):
+        pos = [m - x for m, x in zip(lengths, n)]
+        q = unit(rng, (sum(n), heads, d)) * np.float32(d)
+        given, out = hip.array(q), hip.array(shape=q.shape)
+        p.cache.attention(p.rows(pos, n, one_each=one_each), given, out, heads)
+        got, at = out.numpy(), 0
+        for s, (a, m) in enumerate(zip(pos, n)):
+            w, size, most = attend_all(o.bf16(q[at:at + m]), *p.held(s, a + m), a, d ** -0.5)
+            same(got[at:at + m], w, o.tolerance(w, size, most, d, 16, o.F32))
+            at += m
+        given.free()
+        out.free()
+    p.free()

@@ -319,8 +319,8 @@ template <class Q>
 struct InLds<Q, std::enable_if_t<Q::kInLds>> : std::true_type {};
 
 // One tile. q(qb, c): chunk c of the operand of a lane's q-col in block qb. next_k loads the next tile's keys once this one's are used, next_v its values: each load has about half a
-// tile's work to land behind.
-template <int D, int QB, int MOD, class TILE, class Q, class NK, class NV>
+// tile's work to land behind. TWO (BF16 operands): a weight is the sum of two BF16 values, 16 bits of it, else one of 8 (f16: 11).
+template <int D, int QB, int MOD, bool TWO = false, class TILE, class Q, class NK, class NV>
 __device__ inline void few_tile(TILE& T, Q&& q, const Span (&span)[QB],
                                 const Score (&sc)[QB], FewState<D, QB>& st, int4 p0, int4 p1, NK&& next_k, NV&& next_v) {
   const int pos[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
@@ -357,7 +357,7 @@ __device__ inline void few_tile(TILE& T, Q&& q, const Span (&span)[QB],
     }
   }
   next_k();
-  X8 w[QB];
+  X8 w[QB], rest[QB];
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     float y[8];
@@ -386,6 +386,7 @@ __device__ inline void few_tile(TILE& T, Q&& q, const Span (&span)[QB],
       st.l[qb] += p;
       if constexpr (TILE::kScaled) p *= vs[e];
       w[qb][e] = p;
+      if constexpr (TWO) rest[qb][e] = p - (float)w[qb][e];
     }
   }
   T.begin_v();
@@ -393,7 +394,10 @@ __device__ inline void few_tile(TILE& T, Q&& q, const Span (&span)[QB],
   for (int dd = 0; dd < D / 16; ++dd) {
     const X8 v = T.v(dd);
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb) st.acc[qb][dd] = mfma16(v, w[qb], st.acc[qb][dd]);
+    for (int qb = 0; qb < QB; ++qb) {
+      st.acc[qb][dd] = mfma16(v, w[qb], st.acc[qb][dd]);
+      if constexpr (TWO) st.acc[qb][dd] = mfma16(v, rest[qb], st.acc[qb][dd]);
+    }
   }
   next_v();
 }

@@ -249,6 +249,14 @@ constexpr size_t few_lds() {
   return join > q ? join : q;
 }
 
+// Weights over BF16 and FP8 pages, whose values are BF16 operands, are sums of two BF16 values: with one, outputs were off by 1.4
+// times what FP32 weights and the rounding of BF16 rows are (2.3e-3 of their norm, 1.7e-3), and up to 16 q-cols, which wait for the
+// pages' bytes, take no longer with two (64 tokens over 8192 FP8 positions 90.0 us and 90.1, 256 windows over BF16 pages 169.4 and
+// 169.7). More q-cols do: 64 x 8 rows over FP8 pages 145 us and 154, and prompts, which the matrix ops bound, 49 and 56 (a chunk beside
+// single tokens 136 and 138); so 32 q-cols, and many_piece's, have one of 8 bits. NVFP4 pages' operands are f16, weights of 11 bits.
+template <int QB, int T>
+constexpr bool kTwoTerms = T != kNvfp4 && QB == 1;
+
 template <int D, int QB, class X8, bool LDS>
 struct FewQ {
   static constexpr bool kInLds = LDS;
@@ -351,7 +359,7 @@ __device__ inline void few_piece(const PagedArgs& a, const Piece& p, int h, uint
     }
     page = __builtin_amdgcn_readlane(pages, k);
     if (n < t_end) at = place_of(a, page, h, 32 * n);   // past the end: the same tile again, which is not used
-    few_tile<D, QB, MOD>(tile, q_at, span, sc, st, make_int4(base, base + 1, base + 2, base + 3),
+    few_tile<D, QB, MOD, kTwoTerms<QB, T>>(tile, q_at, span, sc, st, make_int4(base, base + 1, base + 2, base + 3),
                          make_int4(base + 16, base + 17, base + 18, base + 19), [&] { tile.load_k(a, at, lane); },
                          [&] { tile.load_v(a, at, lane); });
   }
