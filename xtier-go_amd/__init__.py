@@ -843,7 +843,10 @@ class PagedCache:
             v = _rows_ptr(b, "v", v, rows.n_rows, kv * self.head_dim, v_stride, x_dtype)
         if q is not None:
             n, width = rows.n_rows, heads * self.head_dim
-            q, q_out = _rows_ptr(b, "q", q, n, width, q_stride, x_dtype), _rows_ptr(b, "q_out", q_out, n, width, q_stride, x_dtype)
+            if q_stride:
+                q, q_out = _rows_ptr(b, "q", q, n, width, q_stride, x_dtype), _rows_ptr(b, "q_out", q_out, n, width, q_stride, x_dtype)
+            else:
+                q, q_out = _device_ptr(b, "q", q, n * width, x_dtype), _device_ptr(b, "q_out", q_out, n * width, x_dtype)
         if qscale is not None:
             qscale = _device_ptr(b, "qscale", qscale, heads * self.head_dim, X_F32)
         a = PagedAppendArgs(heads, q, q_out, k, v, q_stride, k_stride, v_stride, x_dtype, theta, norm, qscale)

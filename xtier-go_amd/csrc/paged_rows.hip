@@ -379,7 +379,7 @@ __device__ inline void append_q(const AppendArgs& a, int row, float2* cs_lds) {
   if (q.pos < 0 || uint32_t(at) >= uint32_t(q.n)) return;   // (the whole work-group)
   if (a.freq) {
     // (seq_at's position goes no further than a page's)
-    if (int(threadIdx.x) < D / 2) cs_lds[threadIdx.x] = turned(double(s.pos[seq]) + double(at), f);
+    if (int(threadIdx.x) < D / 2) cs_lds[threadIdx.x] = turned(double(uint32_t(s.pos[seq]) + uint32_t(at)), f);
     __syncthreads();
   }
   for (int x0 = 0; x0 < chunks; x0 += 256) {
