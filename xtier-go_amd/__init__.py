@@ -225,7 +225,7 @@ def _device_ptr(b, name, a, n, kind):
     if isinstance(a, int):
         return a
     if isinstance(a, DeviceArray):
-        at, size, here, whole = a.ptr if a.b.h else None, a.nbytes // a.dtype.itemsize, a.b.device == b.device, True
+        at, size, here, whole = a.ptr if a.ptr and a.b.h else None, a.nbytes // a.dtype.itemsize, a.b.device == b.device, True
     elif hasattr(a, "get_device"):
         at, size, here, whole = a.data_ptr(), a.numel(), a.get_device() == b.device, a.is_contiguous()
     else:
