@@ -268,13 +268,14 @@ typedef struct xtg_paged_rows {
 } xtg_paged_rows;
 
 /* The rows' keys and values into their sequences' pages, as xtg_hip_kv_write rounds and scales them (but that FP8 scales are
- * amax times the FP32 number nearest to 1/448, which may differ from the quotient in the last bit, so that a linear cache may
- * hold other codes of the same row, and rows whose amax is below 448 * 2^-126, 1.75 * 2^-118, are zeros), after what the Q/K producer does to q and k (xtg_hip_qk_rope_norm): rotation by the row's position (theta 0: none; pairs (i, i + head_dim / 2)
- * by pos * theta^(-2i/head_dim), an angle held in 64 bits, where the producer's are FP32 products), justnorm per head (norm != 0),
- * and q times qscale (NULL: no scale). q may be NULL; q_out, rows of q's stride, may be q, and overlaps no input otherwise. A
- * row whose position has no page is not stored (its q_out is written all the same). Rows are x_dtype, x_stride elements apart
- * (0: packed; else a multiple of 16 bytes), 16-byte aligned. A page that a call writes is in one sequence's table at that
- * place. Queued; the first call of a theta makes its table (make it before a graph capture). */
+ * amax times the FP32 number nearest to 1/448, which may differ from the quotient in the last bit, so that a linear cache
+ * may hold other codes of the same row, and rows whose amax is below 448 * 2^-126, 1.75 * 2^-118, are zeros), after what the
+ * Q/K producer does to q and k (xtg_hip_qk_rope_norm): rotation by the row's position (theta 0: none; pairs (i, i + head_dim
+ * / 2) by pos * theta^(-2i/head_dim), an angle held in 64 bits, where the producer's are FP32 products), justnorm per head
+ * (norm != 0), and q times qscale (NULL: no scale). q may be NULL; q_out, rows of q's stride, may be q, and overlaps no
+ * input otherwise. A row whose position has no page is not stored (its q_out is written all the same). Rows are x_dtype,
+ * x_stride elements apart (0: packed; else a multiple of 16 bytes), 16-byte aligned. A page that a call writes is in one
+ * sequence's table at that place. Queued; the first call of a theta makes its table (make it before a graph capture). */
 typedef struct xtg_paged_append {
   int heads;               /* of q */
   const void* q;           /* device [n_rows][heads][head_dim], or NULL */
@@ -294,16 +295,18 @@ int xtg_hip_paged_append(xtg_hip* h, xtg_hip_paged* c, const xtg_paged_rows* row
 int xtg_hip_paged_read(xtg_hip* h, const xtg_hip_paged* c, const xtg_paged_rows* rows, void* k, void* v, int x_dtype,
                        char* err, int err_len);
 /* Attention of the rows over their own sequences' pages, which hold their keys and values already (append first): a row at
- * position t sees positions p <= t, and p > t - window where window > 0, with scores as xtg_hip_attention_ext's: (q . k) * scale,
- * then softcap * tanh(s / softcap) where softcap > 0. Rows of a sequence that is left out get zeros; a row that sees a
- * position without a page, or whose scores are all minus infinity, NaN. What is in a page beside the positions that a row
- * sees, NaN too, is nothing to it. Rows are x_dtype (FP32 q is rounded to BF16 as it is read, out is not). Scores, their maxima
- * and sums and the output are held in FP32; the softmax weights enter the product with V as f16 (11 bits, NVFP4 pages) or as BF16
- * (others, times an FP8 row's scale): a sum of two, 16 bits, for a sequence of up to 16 (row, q head of a KV head) pairs, one of 8
- * bits for one of more, and for all of a call whose sequences have 17 to 32 on the average. Up to 128 q heads per KV head; n_rows * heads up to 2^27; out, packed, overlaps no input. Queued; the
- * first call of so many rows, sequences and heads, with starts or without, on a pool of so many KV heads and dims, and of tables
- * for more than 128 positions or for fewer, sizes scratch memory, whatever the sequences' lengths (make it, alike in all of these,
- * before a graph capture). */
+ * position t sees positions p <= t, and p > t - window where window > 0, with scores as xtg_hip_attention_ext's: (q . k) *
+ * scale, then softcap * tanh(s / softcap) where softcap > 0. Rows of a sequence that is left out get zeros; a row that sees
+ * a position without a page, or whose scores are all minus infinity, NaN. What is in a page beside the positions that a row
+ * sees, NaN too, is nothing to it; but in a sequence of several rows those that a value of V which is not finite reaches, or
+ * would reach through a tile that they share, are computed key by key, hundreds of times slower. Rows are x_dtype (FP32 q is
+ * rounded to BF16 as it is read, out is not). Scores, their maxima and sums and the output are held in FP32; the softmax
+ * weights enter the product with V as f16 (11 bits, NVFP4 pages) or as BF16 (others, times an FP8 row's scale): a sum of
+ * two, 16 bits, for a sequence of up to 16 (row, q head of a KV head) pairs, one of 8 bits for one of more, and for all of a
+ * call whose sequences have 17 to 32 on the average. Up to 128 q heads per KV head; n_rows * heads up to 2^27; out, packed,
+ * overlaps no input. Queued; the first call of so many rows, sequences and heads, with starts or without, on a pool of so
+ * many KV heads and dims, and of tables for more than 128 positions or for fewer, sizes scratch memory, whatever the
+ * sequences' lengths (make it, alike in all of these, before a graph capture). */
 typedef struct xtg_paged_attn {
   int heads;
   const void* q;           /* device [n_rows][heads][head_dim], q_stride elements apart (0: packed), 16-byte aligned */

@@ -4,8 +4,8 @@
 // and the 8 that they turn with, of V a wave takes a group of 8 slots and a thread a few of their dims, so that V's words,
 // which hold 8 slots, are written whole where the call has all of them. Rotation: o1 = x1 cos - x2 sin, o2 = x2 cos + x1 sin
 // with the angle pos * theta^(-2i/d), its sine and cosine in 64 bits (in 32 an angle of 30000 radians is off by 0.001).
-// HBM bounds a prompt's rows: 4311 rows of 32 q heads and 8 KV heads of 128 dims, BF16, 106 MB, in 23 us (4.6 TB/s). A decode
-// step's rows are one chain of loads and stores, 4 to 6 us.
+// HBM bounds a prompt's rows: 4311 rows of 32 q heads and 8 KV heads of 128 dims, BF16, 106 MB, in 23 to 24 us (4.4 to 4.6 TB/s); into
+// FP8 and NVFP4 pages, 97 and 93 MB, in 24. A decode step's rows are one chain of loads and stores, 4 to 7 us.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
