@@ -302,7 +302,7 @@ int xtg_hip_paged_read(xtg_hip* h, const xtg_hip_paged* c, const xtg_paged_rows*
  * would reach through a tile that they share, are computed key by key, hundreds of times slower. Rows are x_dtype (FP32 q is
  * rounded to BF16 as it is read, out is not). Scores, their maxima and sums and the output are held in FP32; the softmax
  * weights enter the product with V as f16 (11 bits, NVFP4 pages) or as BF16 (others, times an FP8 row's scale): a sum of
- * two, 16 bits, for a sequence of up to 16 (row, q head of a KV head) pairs, one of 8 bits for one of more, and for all of a
+ * two, 15 bits, for a sequence of up to 16 (row, q head of a KV head) pairs, one of 8 bits for one of more, and for all of a
  * call whose sequences have 17 to 32 on the average. Up to 128 q heads per KV head; n_rows * heads up to 2^27; out, packed,
  * overlaps no input. Queued; the first call of so many rows, sequences and heads, with starts or without, on a pool of so
  * many KV heads and dims, and of tables for more than 128 positions or for fewer, sizes scratch memory, whatever the

@@ -319,7 +319,7 @@ template <class Q>
 struct InLds<Q, std::enable_if_t<Q::kInLds>> : std::true_type {};
 
 // One tile. q(qb, c): chunk c of the operand of a lane's q-col in block qb. next_k loads the next tile's keys once this one's are used, next_v its values: each load has about half a
-// tile's work to land behind. TWO (BF16 operands): a weight is the sum of two BF16 values, 16 bits of it, else one of 8 (f16: 11).
+// tile's work to land behind. TWO (BF16 operands): a weight is the sum of two BF16 values, 15 bits of it, else one of 8 (f16: 11).
 template <int D, int QB, int MOD, bool TWO = false, class TILE, class Q, class NK, class NV>
 __device__ inline void few_tile(TILE& T, Q&& q, const Span (&span)[QB],
                                 const Score (&sc)[QB], FewState<D, QB>& st, int4 p0, int4 p1, NK&& next_k, NV&& next_v) {
@@ -385,8 +385,12 @@ __device__ inline void few_tile(TILE& T, Q&& q, const Span (&span)[QB],
       float p = __builtin_amdgcn_exp2f(y[e] - ref);
       st.l[qb] += p;
       if constexpr (TILE::kScaled) p *= vs[e];
+      if constexpr (TWO) {   // cut, not rounded, and 2^-17 more: both above zero, so that an infinite value times both is one
+        const float cut = __uint_as_float(__float_as_uint(p) & 0xffff0000u);
+        rest[qb][e] = fmaf(p, 1.f + 0x1p-17f, -cut);
+        p = cut;
+      }
       w[qb][e] = p;
-      if constexpr (TWO) rest[qb][e] = p - (float)w[qb][e];
     }
   }
   T.begin_v();
